@@ -22,6 +22,11 @@ WSP_FLOAT32 = 0
 WSP_FLOAT16 = 1
 WSP_BFLOAT16 = 2
 
+WSP_CACHE_FLOAT16 = 1
+WSP_CACHE_BFLOAT16 = 2
+WSP_CACHE_E4M3 = 3
+WSP_CACHE_INT8 = 4
+
 TRACE_SECTIONS = ("wait", "compute", "barrier", "epilogue", "norm", "attention", "ops", "query", "join",
                   "out_projection", "self_item", "logits", "norm_load", "norm_rest", "logits_tiles",
                   "logits_fold")
@@ -63,8 +68,28 @@ class CEncoderShape(ctypes.Structure):
         "mel_bins", "width", "heads", "layers", "feed_forward_width", "input_frames")]
 
 
-# Every entry point include/wsp_decoder.h and include/wsp_encoder.h declare,
-# with its ctypes signature.
+class CCacheShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("heads", "head_width", "page_rows", "pages", "storage")]
+
+
+class CCacheMemory(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("keys", "values", "key_scales", "value_scales")] + \
+               [(n, ctypes.c_int64) for n in ("page_stride", "head_stride", "row_stride")]
+
+
+class CCacheBatch(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lengths", "starts")] + \
+               [("table_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("table_columns", "sequences", "max_rows")]
+
+
+class CCacheRows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("dtype", ctypes.c_int32)]
+
+
+# Every entry point include/wsp_decoder.h, include/wsp_encoder.h and
+# include/wsp_cache.h declare, with its ctypes signature.
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 SIGNATURES = {
@@ -104,6 +129,14 @@ SIGNATURES = {
     "wsp_encoder_log_mel": ([_P, _P, _I, _P], _I),
     "wsp_encoder_encode": ([_P, _P, _P], _I),
     "wsp_encoder_encode_samples": ([_P, _P, _I, _P], _I),
+    "wsp_cache_create": ([_P, _I, _P, ctypes.POINTER(_P)], _I),
+    "wsp_cache_destroy": ([_P], None),
+    "wsp_cache_get_memory": ([_P, _P], _I),
+    "wsp_cache_append": ([_P, _P, _I, _P, _P, _P], _I),
+    "wsp_cache_read": ([_P, _P, _I, _P, _P, _P], _I),
+    "wsp_cache_attend": ([_P, _P, _I, _I, _P, _P, _P, ctypes.c_float, _I, _P, ctypes.c_size_t, _P], _I),
+    "wsp_cache_attend_workspace": ([_P, _P, _I, _I, ctypes.POINTER(ctypes.c_size_t)], _I),
+    "wsp_cache_check": ([_P], _I),
 }
 
 _lib = None

@@ -1,0 +1,484 @@
+// The paged key/value cache: the C ABI of include/wsp_cache.h, and the
+// kernels that write rows into the pages and read them back (sm_100a).
+#include "../../include/wsp_cache.h"
+
+#include "cache.cuh"
+#include "cache_attend.cuh"
+#include "host.h"
+
+#include <memory>
+
+namespace wsp {
+namespace {
+
+// ---------------------------------------------------------- append and read
+//
+// A thread holds 8 elements of one row of one head, of the key and of the
+// value: D / 8 neighbouring lanes hold a row.  16 bytes of a 16-bit row and 8
+// of an 8-bit one are in flight per thread and side, which is what these two
+// kernels live on: they are bound by the bytes of the rows and the pages.
+
+struct RowsView {
+    unsigned char* data;
+    long long row_bytes, head_bytes;
+};
+
+struct CopyArgs {
+    CacheView cache;
+    CacheBatchView batch;
+    RowsView keys, values;
+    int rows, first_row;  // rows of the arrays; the first row of this launch
+};
+
+// dtype codes of wsp_decoder.h as types
+template <int T> struct RowType;
+template <> struct RowType<WSP_FLOAT32> { static constexpr int bytes = 4; };
+template <> struct RowType<WSP_FLOAT16> { static constexpr int bytes = 2; using type = __half; };
+template <> struct RowType<WSP_BFLOAT16> { static constexpr int bytes = 2; using type = __nv_bfloat16; };
+
+template <int T>
+__device__ __forceinline__ void load8(const unsigned char* p, float (&x)[8]) {
+    if constexpr (T == WSP_FLOAT32) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const uint4 v = load_stream(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = Half16<typename RowType<T>::type>::pair_to_float2(w[e]);
+            x[2 * e] = f.x;
+            x[2 * e + 1] = f.y;
+        }
+    }
+}
+
+template <int T>
+__device__ __forceinline__ void store8(unsigned char* p, const float (&x)[8]) {
+    if constexpr (T == WSP_FLOAT32) {
+        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(p + 16) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = Half16<typename RowType<T>::type>::pack2(x[2 * e], x[2 * e + 1]);
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// The scale byte of a row whose largest magnitude is `top`: E + 127 with E
+// the smallest integer for which top <= L 2^E.  top = m 2^e with m in [1, 2)
+// (the exponent bits), and L = 448 is 1.75 2^8, 127 is 1.984375 2^6: E is e
+// minus L's exponent, and one more where m is above L's mantissa.  Magnitudes
+// so small that E would be below -126 keep E = -126.
+template <int S>
+__device__ __forceinline__ uint32_t scale_byte(float top) {
+    const uint32_t bits = __float_as_uint(top);
+    if (bits >= 0x7f800000u) return 255u;
+    constexpr int kExponent = S == kCacheE4m3 ? 8 : 6;
+    constexpr uint32_t kMantissa = S == kCacheE4m3 ? 0x600000u : 0x7e0000u;
+    const int e = (int)(bits >> 23) - kExponent + ((bits & 0x7fffffu) > kMantissa ? 1 : 0);
+    return (uint32_t)max(e, 1);
+}
+
+// Writes 8 elements of a row; the D / 8 lanes of a row agree on its scale.
+template <int S, int D>
+__device__ __forceinline__ void write8(unsigned char* p, uint8_t* scale, const float (&x)[8], bool valid) {
+    if constexpr (!cache_eight(S)) {
+        if (valid) store8<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
+    } else {
+        // The largest magnitude through its bits, which order as the values
+        // do and keep NaN on top.
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = D / 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const uint32_t byte = scale_byte<S>(__uint_as_float(top));
+        // 2^(127 - byte): exact, subnormal only for 254 (never chosen)
+        const float inverse = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+        uint32_t w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = byte == 255u ? 0.f : x[4 * h + e] * inverse;
+            if constexpr (S == kCacheE4m3) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+                w[h] = lo | (hi << 16);
+            } else {
+                w[h] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[h] |= ((uint32_t)__float2int_rn(y[e]) & 0xffu) << (8 * e);
+            }
+        }
+        if (valid) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+            if ((threadIdx.x & (D / 8 - 1)) == 0) *scale = (uint8_t)byte;
+        }
+    }
+}
+
+template <int S>
+__device__ __forceinline__ void read8(const unsigned char* p, const uint8_t* scale, float (&x)[8]) {
+    if constexpr (!cache_eight(S)) {
+        load8<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        const float s = cache_scale(*scale);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = cache_pair<S>(((e < 2 ? v.x : v.y) >> (16 * (e & 1))) & 0xffffu);
+            x[2 * e] = f.x * s;
+            x[2 * e + 1] = f.y * s;
+        }
+    }
+}
+
+// The sequence that row r belongs to: the last s with starts[s] <= r, if r
+// is below starts[sequences]; -1 if none.
+__device__ __forceinline__ int sequence_of(const CacheBatchView& b, int r) {
+    int low = 0, high = b.sequences;
+    if (r < __ldg(b.starts) || r >= __ldg(b.starts + high)) return -1;
+    while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (__ldg(b.starts + mid) <= r) low = mid;
+        else high = mid;
+    }
+    return low;
+}
+
+constexpr int kCopyThreads = 256;
+
+template <int S, int T, int D, bool kWrite>
+__global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const CopyArgs a) {
+    constexpr int kLanes = D / 8;  // lanes of a row
+    const long long item = ((long long)blockIdx.x * kCopyThreads + threadIdx.x) / kLanes;
+    const int piece = threadIdx.x % kLanes;
+    const long long row64 = item / a.cache.heads;
+    const int head = (int)(item - row64 * a.cache.heads);
+    const int r = (int)min(row64, (long long)a.rows);
+    int page = -1, slot = 0;
+    bool mine = r < a.rows;
+    if (mine) {
+        const int s = sequence_of(a.batch, r);
+        mine = s >= 0;
+        if (mine) {
+            const CacheSequence q = cache_sequence(a.batch, s);
+            const int position = q.length - q.rows + (r - q.first);
+            page = cache_page(a.cache, a.batch, s, position);
+            slot = position & ((1 << a.cache.page_shift) - 1);
+        }
+    }
+    const long long key_at = (long long)r * a.keys.row_bytes + head * a.keys.head_bytes + piece * 8 * RowType<T>::bytes;
+    const long long value_at =
+        (long long)r * a.values.row_bytes + head * a.values.head_bytes + piece * 8 * RowType<T>::bytes;
+    const long long at = cache_offset(a.cache, page, head, slot) + piece * 8 * cache_bytes(S);
+    const long long si = cache_eight(S) ? cache_scale_index(a.cache, page, head, slot) : 0;
+    float k[8], v[8];
+    if constexpr (kWrite) {
+        // The row's lanes take the same branches; all stay for the shuffles.
+        const bool valid = page >= 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
+        if (valid) {
+            load8<T>(a.keys.data + key_at, k);
+            load8<T>(a.values.data + value_at, v);
+        }
+        write8<S, D>(a.cache.keys + at, a.cache.key_scales + si, k, valid);
+        write8<S, D>(a.cache.values + at, a.cache.value_scales + si, v, valid);
+    } else {
+        if (!mine) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
+        if (page >= 0) {
+            read8<S>(a.cache.keys + at, a.cache.key_scales + si, k);
+            read8<S>(a.cache.values + at, a.cache.value_scales + si, v);
+        }
+        store8<T>(a.keys.data + key_at, k);
+        store8<T>(a.values.data + value_at, v);
+    }
+}
+
+template <int S, int T, bool kWrite>
+void launch_copy(const CopyArgs& a, int width, cudaStream_t stream) {
+    const long long threads = (long long)a.rows * a.cache.heads * (width / 8);
+    const unsigned grid = (unsigned)((threads + kCopyThreads - 1) / kCopyThreads);
+    if (width == 64) cache_copy_kernel<S, T, 64, kWrite><<<grid, kCopyThreads, 0, stream>>>(a);
+    else cache_copy_kernel<S, T, 128, kWrite><<<grid, kCopyThreads, 0, stream>>>(a);
+}
+
+template <int S, bool kWrite>
+void launch_copy(const CopyArgs& a, int dtype, int width, cudaStream_t stream) {
+    if (dtype == WSP_FLOAT32) launch_copy<S, WSP_FLOAT32, kWrite>(a, width, stream);
+    else if (dtype == WSP_FLOAT16) launch_copy<S, WSP_FLOAT16, kWrite>(a, width, stream);
+    else launch_copy<S, WSP_BFLOAT16, kWrite>(a, width, stream);
+}
+
+template <bool kWrite>
+void launch_copy(const CopyArgs& a, int storage, int dtype, int width, cudaStream_t stream) {
+    if (storage == kCacheF16) launch_copy<kCacheF16, kWrite>(a, dtype, width, stream);
+    else if (storage == kCacheBf16) launch_copy<kCacheBf16, kWrite>(a, dtype, width, stream);
+    else if (storage == kCacheE4m3) launch_copy<kCacheE4m3, kWrite>(a, dtype, width, stream);
+    else launch_copy<kCacheInt8, kWrite>(a, dtype, width, stream);
+}
+
+// ------------------------------------------------------------------- host
+
+class CurrentDevice {
+public:
+    explicit CurrentDevice(int device) {
+        CUDA_CHECK(cudaGetDevice(&before_));
+        if (before_ != device) CUDA_CHECK(cudaSetDevice(device));
+        else before_ = -1;
+    }
+    ~CurrentDevice() {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
+    CurrentDevice(const CurrentDevice&) = delete;
+    CurrentDevice& operator=(const CurrentDevice&) = delete;
+
+private:
+    int before_ = -1;
+};
+
+int row_size(int dtype) { return dtype == WSP_FLOAT32 ? 4 : 2; }
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace wsp
+
+struct wsp_cache {
+    wsp_cache_shape shape;
+    wsp_cache_memory memory;
+    wsp::CacheView view;
+    int device = 0;
+    int sms = 0;
+    wsp::DeviceBuffer owned[4];
+};
+
+namespace wsp {
+namespace {
+
+using std::to_string;
+
+const wsp_cache& checked(const wsp_cache* cache) {
+    if (!cache) throw InvalidArgument("cache must not be NULL");
+    return *cache;
+}
+
+void check_batch(const wsp_cache_batch* b, int rows) {
+    if (!b) throw InvalidArgument("batch must not be NULL");
+    if (rows < 0) throw InvalidArgument("rows must not be negative, got " + to_string(rows));
+    if (b->sequences < 0 || b->table_columns < 0 || b->max_rows < 0)
+        throw InvalidArgument("a batch's sequences, table_columns and max_rows must not be negative");
+    if (b->sequences == 0) return;
+    if (!b->lengths || !b->starts || (!b->table && b->table_columns > 0))
+        throw InvalidArgument("a batch's table, lengths and starts must not be NULL");
+    if (b->sequences > 1 && b->table_stride < b->table_columns)
+        throw InvalidArgument("table_stride (" + to_string(b->table_stride) + ") must hold table_columns (" +
+                              to_string(b->table_columns) + ")");
+    for (const void* p : {(const void*)b->table, (const void*)b->lengths, (const void*)b->starts})
+        if (reinterpret_cast<uintptr_t>(p) & 3) throw InvalidArgument("a batch's arrays must be 4-byte aligned");
+}
+
+// A row array's view; heads 1 wide need no head stride.
+RowsView check_rows(const wsp_cache_rows* r, const char* name, int rows, int heads, int width) {
+    if (!r) throw InvalidArgument(std::string(name) + " must not be NULL");
+    if (r->dtype != WSP_FLOAT32 && r->dtype != WSP_FLOAT16 && r->dtype != WSP_BFLOAT16)
+        throw InvalidArgument(std::string(name) + ": not a wsp_dtype: " + to_string(r->dtype));
+    if (rows > 0 && !r->data) throw InvalidArgument(std::string(name) + "' data must not be NULL");
+    const int size = row_size(r->dtype);
+    if (!aligned(r->data) || (rows > 1 && r->row_stride * size % 16) || (heads > 1 && r->head_stride * size % 16))
+        throw InvalidArgument(std::string(name) + " must be 16-byte aligned, its strides multiples of 16 bytes");
+    if ((rows > 1 && r->row_stride < width) || (heads > 1 && r->head_stride < width))
+        throw InvalidArgument(std::string(name) + ": strides must be at least head_width (" + to_string(width) + ")");
+    return {static_cast<unsigned char*>(r->data), r->row_stride * size, r->head_stride * size};
+}
+
+CacheBatchView batch_view(const wsp_cache_batch& b) {
+    return {b.table, b.lengths, b.starts, b.table_stride, b.table_columns, b.sequences};
+}
+
+template <bool kWrite>
+void copy_rows(wsp_cache* cache, const wsp_cache_batch* batch, int rows, const wsp_cache_rows* keys,
+               const wsp_cache_rows* values, void* stream) {
+    const wsp_cache& c = checked(cache);
+    check_batch(batch, rows);
+    CopyArgs a{};
+    a.keys = check_rows(keys, "keys", rows, c.shape.heads, c.shape.head_width);
+    a.values = check_rows(values, "values", rows, c.shape.heads, c.shape.head_width);
+    if (keys->dtype != values->dtype) throw InvalidArgument("keys and values must have one dtype");
+    if (rows == 0 || batch->sequences == 0) return;
+    if ((long long)rows * c.shape.heads * (c.shape.head_width / 8) > (long long)kCopyThreads * 0x7fffffff)
+        throw InvalidArgument("too many rows for one call: " + to_string(rows));
+    a.cache = c.view;
+    a.batch = batch_view(*batch);
+    a.rows = rows;
+    CurrentDevice device(c.device);
+    launch_copy<kWrite>(a, c.shape.storage, keys->dtype, c.shape.head_width, static_cast<cudaStream_t>(stream));
+    CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace
+}  // namespace wsp
+
+using wsp::guarded;
+
+extern "C" {
+
+int wsp_cache_create(const wsp_cache_shape* shape, int device, const wsp_cache_memory* memory, wsp_cache** out) {
+    return guarded([&] {
+        using wsp::ModelError;
+        using std::to_string;
+        if (!shape || !out) throw wsp::InvalidArgument("shape and out must not be NULL");
+        const wsp_cache_shape& s = *shape;
+        if (s.storage < WSP_CACHE_FLOAT16 || s.storage > WSP_CACHE_INT8)
+            throw ModelError("a cache's storage is one of WSP_CACHE_FLOAT16, _BFLOAT16, _E4M3 and _INT8, not " +
+                             to_string(s.storage));
+        if (s.head_width != 64 && s.head_width != 128)
+            throw ModelError("a cache's heads are 64 or 128 wide, not " + to_string(s.head_width));
+        if (s.page_rows < 16 || s.page_rows > 256 || (s.page_rows & (s.page_rows - 1)))
+            throw ModelError("a page has 16, 32, 64, 128 or 256 rows, not " + to_string(s.page_rows));
+        if (s.heads <= 0 || s.pages <= 0) throw ModelError("a cache needs heads and pages");
+        if (s.heads > 65535) throw ModelError("a cache has at most 65535 heads, not " + to_string(s.heads));
+        const bool eight = wsp::cache_eight(s.storage);
+        const int size = wsp::cache_bytes(s.storage);
+        if (memory) {
+            const wsp_cache_memory& m = *memory;
+            if (!m.keys || !m.values || (eight && (!m.key_scales || !m.value_scales)))
+                throw wsp::InvalidArgument("a cache's memory must not be NULL");
+            for (int64_t stride : {m.page_stride, m.head_stride, m.row_stride})
+                if (stride < s.head_width || stride * size % 16)
+                    throw wsp::InvalidArgument("a pool's strides are at least head_width and multiples of 16 bytes, not " +
+                                               to_string(stride) + " elements");
+            if (!wsp::aligned(m.keys) || !wsp::aligned(m.values))
+                throw wsp::InvalidArgument("the pools must be 16-byte aligned");
+        }
+        int count = 0;
+        wsp::cuda_check(cudaGetDeviceCount(&count), "cudaGetDeviceCount");
+        if (device < 0 || device >= count) throw wsp::InvalidArgument("no CUDA device " + to_string(device));
+        wsp::CurrentDevice current(device);
+        std::unique_ptr<wsp_cache> c(new wsp_cache{});
+        c->shape = s;
+        c->device = device;
+        wsp::cuda_check(cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, device),
+                        "cudaDeviceGetAttribute");
+        if (memory) {
+            c->memory = *memory;
+            if (!eight) c->memory.key_scales = c->memory.value_scales = nullptr;
+        } else {
+            const size_t rows = (size_t)s.pages * s.heads * s.page_rows;
+            for (int i = 0; i < 2; ++i) {
+                c->owned[i].allocate(rows * s.head_width * size);
+                if (eight) c->owned[2 + i].allocate(rows);
+            }
+            c->memory = {c->owned[0].get(), c->owned[1].get(), c->owned[2].get<uint8_t>(), c->owned[3].get<uint8_t>(),
+                         (int64_t)s.heads * s.page_rows * s.head_width, (int64_t)s.page_rows * s.head_width,
+                         s.head_width};
+        }
+        const wsp_cache_memory& m = c->memory;
+        int shift = 0;
+        while ((1 << shift) < s.page_rows) ++shift;
+        c->view = {static_cast<unsigned char*>(m.keys), static_cast<unsigned char*>(m.values), m.key_scales,
+                   m.value_scales, m.page_stride * size, m.head_stride * size, m.row_stride * size, s.heads, s.pages,
+                   shift};
+        *out = c.release();
+    });
+}
+
+void wsp_cache_destroy(wsp_cache* cache) {
+    if (!cache) return;
+    guarded([&] {
+        wsp::CurrentDevice current(cache->device);
+        delete cache;
+    });
+}
+
+int wsp_cache_get_memory(const wsp_cache* cache, wsp_cache_memory* memory) {
+    return guarded([&] {
+        if (!memory) throw wsp::InvalidArgument("memory must not be NULL");
+        *memory = wsp::checked(cache).memory;
+    });
+}
+
+int wsp_cache_append(wsp_cache* cache, const wsp_cache_batch* batch, int rows, const wsp_cache_rows* keys,
+                     const wsp_cache_rows* values, void* stream) {
+    return guarded([&] { wsp::copy_rows<true>(cache, batch, rows, keys, values, stream); });
+}
+
+int wsp_cache_read(wsp_cache* cache, const wsp_cache_batch* batch, int rows, const wsp_cache_rows* keys,
+                   const wsp_cache_rows* values, void* stream) {
+    return guarded([&] { wsp::copy_rows<false>(cache, batch, rows, keys, values, stream); });
+}
+
+int wsp_cache_attend_workspace(const wsp_cache* cache, const wsp_cache_batch* batch, int rows, int query_heads,
+                               size_t* bytes) {
+    return guarded([&] {
+        const wsp_cache& c = wsp::checked(cache);
+        if (!bytes) throw wsp::InvalidArgument("bytes must not be NULL");
+        wsp::check_batch(batch, rows);
+        if (query_heads <= 0 || query_heads % c.shape.heads)
+            throw wsp::ModelError("query_heads (" + std::to_string(query_heads) + ") must be a multiple of the cache's heads (" +
+                                  std::to_string(c.shape.heads) + ")");
+        *bytes = wsp::cache_attend_workspace(c.shape.head_width, batch->max_rows, query_heads / c.shape.heads, c.sms);
+    });
+}
+
+int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, int query_heads,
+                     const wsp_cache_rows* queries, const wsp_cache_rows* out, float* lse, float scale, int causal,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        using std::to_string;
+        const wsp_cache& c = wsp::checked(cache);
+        size_t needed = 0;
+        if (const int status = wsp_cache_attend_workspace(cache, batch, rows, query_heads, &needed)) {
+            const std::string text = wsp::last_error_text();
+            if (status == WSP_MODEL_ERROR) throw wsp::ModelError(text);
+            throw wsp::InvalidArgument(text);
+        }
+        const wsp::RowsView q = wsp::check_rows(queries, "queries", rows, query_heads, c.shape.head_width);
+        const wsp::RowsView o = wsp::check_rows(out, "out", rows, query_heads, c.shape.head_width);
+        if (queries->dtype != out->dtype || queries->dtype == WSP_FLOAT32)
+            throw wsp::ModelError("queries and out are of one 16-bit type");
+        if (!wsp::cache_eight(c.shape.storage) && queries->dtype != c.shape.storage)
+            throw wsp::ModelError("queries of a 16-bit cache have its type");
+        if (!(scale == scale) || scale - scale != 0.f) throw wsp::InvalidArgument("scale must be finite");
+        if (reinterpret_cast<uintptr_t>(lse) & 3) throw wsp::InvalidArgument("lse must be 4-byte aligned");
+        if (rows == 0 || batch->sequences == 0) return;
+        if (needed && (!workspace || !wsp::aligned(workspace) || workspace_bytes < needed))
+            throw wsp::InvalidArgument("the workspace must be 16-byte aligned and hold " + to_string(needed) + " bytes, not " +
+                                       to_string(workspace ? workspace_bytes : 0));
+        wsp::CacheAttendArgs a{};
+        a.cache = c.view;
+        a.batch = wsp::batch_view(*batch);
+        a.queries = q.data;
+        a.q_row = q.row_bytes;
+        a.q_head = q.head_bytes;
+        a.out = o.data;
+        a.o_row = o.row_bytes;
+        a.o_head = o.head_bytes;
+        a.lse = lse;
+        a.rows = rows;
+        a.query_heads = query_heads;
+        a.group = query_heads / c.shape.heads;
+        a.scale = scale;
+        a.causal = causal != 0;
+        wsp::CurrentDevice device(c.device);
+        wsp::launch_cache_attend(a, c.shape.storage, queries->dtype == WSP_BFLOAT16, c.shape.head_width, batch->max_rows,
+                                 c.sms, workspace, static_cast<cudaStream_t>(stream));
+        wsp::cuda_check(cudaGetLastError(), "cache attention launch");
+    });
+}
+
+int wsp_cache_check(wsp_cache* cache) {
+    return guarded([&] {
+        const wsp_cache& c = wsp::checked(cache);
+        wsp::CurrentDevice device(c.device);
+        wsp::cuda_check(cudaDeviceSynchronize(), "wsp_cache_check");
+    });
+}
+
+}  // extern "C"
