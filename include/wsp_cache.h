@@ -58,7 +58,8 @@ typedef struct wsp_cache_shape {
  * The two pools, [pages, heads, page_rows, head_width] in any order of the
  * first three (strides in elements, at least head_width and multiples of 16
  * bytes; the base 16-byte aligned; distinct rows must not overlap), and the
- * scale bytes [pages, heads, page_rows], contiguous (8-bit storage only).
+ * scale bytes [pages, heads, page_rows], contiguous and 16-byte aligned (8-bit
+ * storage only).
  */
 typedef struct wsp_cache_memory {
     void* keys;

@@ -6,6 +6,7 @@
 #include "cache_attend.cuh"
 #include "host.h"
 
+#include <algorithm>
 #include <memory>
 
 namespace wsp {
@@ -254,9 +255,11 @@ struct wsp_cache {
     wsp_cache_shape shape;
     wsp_cache_memory memory;
     wsp::CacheView view;
+    wsp::CacheMaps maps;
     int device = 0;
     int sms = 0;
     wsp::DeviceBuffer owned[4];
+    wsp::DeviceBuffer status;  // which wait of a kernel gave up
 };
 
 namespace wsp {
@@ -300,6 +303,46 @@ RowsView check_rows(const wsp_cache_rows* r, const char* name, int rows, int hea
 
 CacheBatchView batch_view(const wsp_cache_batch& b) {
     return {b.table, b.lengths, b.starts, b.table_stride, b.table_columns, b.sequences};
+}
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled found = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult result{};
+        CUDA_CHECK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &result));
+        if (result != cudaDriverEntryPointSuccess || !f) throw CudaFailure("the driver has no cuTensorMapEncodeTiled", false);
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return found;
+}
+
+// A pool as the copy engine sees it: [pages][heads][page_rows][width], a box
+// a page's rows (64 at most) of up to 128 bytes, swizzled over its row.
+CUtensorMap pool_map(const wsp_cache_shape& s, const wsp_cache_memory& m, void* pool) {
+    const int size = cache_bytes(s.storage);
+    const cuuint64_t extents[4] = {(cuuint64_t)s.head_width, (cuuint64_t)s.page_rows, (cuuint64_t)s.heads,
+                                   (cuuint64_t)s.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)(m.row_stride * size), (cuuint64_t)(m.head_stride * size),
+                                   (cuuint64_t)(m.page_stride * size)};
+    const cuuint32_t columns = std::min(s.head_width, 128 / size);
+    const cuuint32_t box[4] = {columns, (cuuint32_t)std::min(s.page_rows, 64), 1, 1}, steps[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = s.storage == WSP_CACHE_FLOAT16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : s.storage == WSP_CACHE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                       : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    CUtensorMap map;
+    const CUresult result = encode_tiled()(&map, type, 4, pool, extents, strides, box, steps,
+                                           CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                           columns * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (result != CUDA_SUCCESS)
+        throw ModelError("the pools' strides are not ones the copy engine takes (status " + to_string((int)result) + ")");
+    return map;
+}
+
+CacheAttendShape attend_shape(const wsp_cache& c, int dtype, int max_rows) {
+    return {c.shape.storage, dtype == WSP_BFLOAT16, c.shape.head_width, max_rows, c.sms};
 }
 
 template <bool kWrite>
@@ -354,8 +397,9 @@ int wsp_cache_create(const wsp_cache_shape* shape, int device, const wsp_cache_m
                 if (stride < s.head_width || stride * size % 16)
                     throw wsp::InvalidArgument("a pool's strides are at least head_width and multiples of 16 bytes, not " +
                                                to_string(stride) + " elements");
-            if (!wsp::aligned(m.keys) || !wsp::aligned(m.values))
-                throw wsp::InvalidArgument("the pools must be 16-byte aligned");
+            if (!wsp::aligned(m.keys) || !wsp::aligned(m.values) ||
+                (eight && (!wsp::aligned(m.key_scales) || !wsp::aligned(m.value_scales))))
+                throw wsp::InvalidArgument("the pools and the scale bytes must be 16-byte aligned");
         }
         int count = 0;
         wsp::cuda_check(cudaGetDeviceCount(&count), "cudaGetDeviceCount");
@@ -385,6 +429,10 @@ int wsp_cache_create(const wsp_cache_shape* shape, int device, const wsp_cache_m
         c->view = {static_cast<unsigned char*>(m.keys), static_cast<unsigned char*>(m.values), m.key_scales,
                    m.value_scales, m.page_stride * size, m.head_stride * size, m.row_stride * size, s.heads, s.pages,
                    shift};
+        c->maps.keys = wsp::pool_map(s, m, m.keys);
+        c->maps.values = wsp::pool_map(s, m, m.values);
+        wsp::prepare_cache_attend(s.storage, s.head_width);
+        c->status.allocate(sizeof(int));
         *out = c.release();
     });
 }
@@ -423,7 +471,7 @@ int wsp_cache_attend_workspace(const wsp_cache* cache, const wsp_cache_batch* ba
         if (query_heads <= 0 || query_heads % c.shape.heads)
             throw wsp::ModelError("query_heads (" + std::to_string(query_heads) + ") must be a multiple of the cache's heads (" +
                                   std::to_string(c.shape.heads) + ")");
-        *bytes = wsp::cache_attend_workspace(c.shape.head_width, batch->max_rows, query_heads / c.shape.heads, c.sms);
+        *bytes = wsp::cache_attend_workspace(wsp::attend_shape(c, WSP_FLOAT16, batch->max_rows), query_heads / c.shape.heads);
     });
 }
 
@@ -466,10 +514,11 @@ int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, i
         a.group = query_heads / c.shape.heads;
         a.scale = scale;
         a.causal = causal != 0;
+        a.status = c.status.get<int>();
+        a.workspace = static_cast<unsigned char*>(workspace);
         wsp::CurrentDevice device(c.device);
-        wsp::launch_cache_attend(a, c.shape.storage, queries->dtype == WSP_BFLOAT16, c.shape.head_width, batch->max_rows,
-                                 c.sms, workspace, static_cast<cudaStream_t>(stream));
-        wsp::cuda_check(cudaGetLastError(), "cache attention launch");
+        wsp::launch_cache_attend(a, c.maps, wsp::attend_shape(c, queries->dtype, batch->max_rows),
+                                 static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -478,6 +527,9 @@ int wsp_cache_check(wsp_cache* cache) {
         const wsp_cache& c = wsp::checked(cache);
         wsp::CurrentDevice device(c.device);
         wsp::cuda_check(cudaDeviceSynchronize(), "wsp_cache_check");
+        int status = 0;
+        wsp::cuda_check(cudaMemcpy(&status, c.status.get(), sizeof status, cudaMemcpyDeviceToHost), "wsp_cache_check");
+        if (status) throw wsp::CudaFailure("a wait of the cache's attention gave up (" + std::to_string(status) + ")", false);
     });
 }
 

@@ -1,9 +1,14 @@
-// The attention over a paged cache: arguments and launches (cache_attend.cu).
+// The attention over a paged cache: arguments and launches.
 #pragma once
 
 #include "cache.cuh"
 
+#include <cuda.h>
+
 namespace wsp {
+
+// Rows of the box a tensor map of a pool copies: a page's rows, or 64 of them.
+__host__ __device__ constexpr int cache_box_shift(int page_shift) { return page_shift < 6 ? page_shift : 6; }
 
 struct CacheAttendArgs {
     CacheView cache;
@@ -16,11 +21,28 @@ struct CacheAttendArgs {
     int rows, query_heads, group;  // group = query heads of a key head
     float scale;
     int causal;
+    int* status;                   // which wait gave up, 0: none
+    unsigned char* workspace;
 };
 
-// storage: the cache's; bf16: the type of queries and out; width: 64 or 128.
-void launch_cache_attend(const CacheAttendArgs& args, int storage, bool bf16, int width, int max_rows, int sms,
-                         void* workspace, cudaStream_t stream);
-size_t cache_attend_workspace(int width, int max_rows, int group, int sms);
+// The pools as tensor maps: [pages][heads][page_rows][head_width], a box one
+// page's (or 64) rows of up to 128 bytes, swizzled over as many.
+struct CacheMaps {
+    CUtensorMap keys, values;
+};
+
+// What a launch needs to know beside its arguments: the cache's storage, the
+// type of queries and out, the heads' width, the bound of a sequence's rows.
+struct CacheAttendShape {
+    int storage;
+    bool bf16;
+    int width, max_rows, sms;
+};
+
+// Raises the kernels' limits of shared memory on the current device.
+void prepare_cache_attend(int storage, int width);
+void launch_cache_attend(const CacheAttendArgs& args, const CacheMaps& maps, const CacheAttendShape& shape,
+                         cudaStream_t stream);
+size_t cache_attend_workspace(const CacheAttendShape& shape, int group);
 
 }  // namespace wsp

@@ -1,0 +1,187 @@
+// Device pieces the cache's attention kernels share: bounded waits, bulk
+// tensor copies, 8-bit widening, and the row that is computed alone.
+#pragma once
+
+#include "cache_attend.cuh"
+#include "umma.cuh"
+
+#include <type_traits>
+
+namespace wsp {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// ------------------------------------------------------------------- waits
+
+constexpr unsigned long long kCacheTimeoutNs = 2000000000ull;
+
+__device__ __forceinline__ unsigned long long cache_clock_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+__device__ __forceinline__ bool cache_phase_done(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_address(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// Waits for the phase of `parity`.  After 2 s, or once another wait of the CTA
+// has given up, it records `kind` and returns false, and so does every later
+// wait at once: the roles then run through their loops without waiting, so
+// all meet at the barriers between them, and the results are void.
+static __device__ __noinline__ bool cache_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
+                                                    int kind) {
+    const unsigned long long start = cache_clock_ns();
+    for (unsigned spin = 1;; ++spin) {
+        if (cache_phase_done(bar, parity)) return true;
+        if ((spin & 15) != 0) continue;
+        if (*abort) return false;
+        if (cache_clock_ns() - start > kCacheTimeoutNs) {
+            atomicCAS(status, 0, kind);
+            *abort = 1;
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool cache_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int kind) {
+    if (cache_phase_done(bar, parity)) return true;
+    return cache_wait_slow(bar, parity, abort, status, kind);
+}
+
+__device__ __forceinline__ void cache_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_address(bar)) : "memory");
+}
+__device__ __forceinline__ void cache_arrive_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_address(bar)), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void cache_barrier_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_address(bar)), "r"(count) : "memory");
+}
+
+// ------------------------------------------------------------------- copies
+
+// One box of a pool: columns x.., rows y.. of a head's page.  x is 0 or 64
+// 16-bit columns, so the copy starts on 16 bytes; a page outside the pool
+// reads as zeros.
+__device__ __forceinline__ void cache_copy_box(void* to, const CUtensorMap* map, int x, int y, int head, int page,
+                                               uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_address(to)),
+        "l"(map), "r"(x), "r"(y), "r"(head), "r"(page), "r"(smem_address(bar))
+        : "memory");
+}
+__device__ __forceinline__ void cache_copy_bytes(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_address(to)),
+                 "l"(from), "r"(bytes), "r"(smem_address(bar))
+                 : "memory");
+}
+// Orders this thread's shared-memory accesses before later bulk copies and
+// tensor-core reads of the same memory.
+__device__ __forceinline__ void cache_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ----------------------------------------------------------------- numbers
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ------------------------------------------------- a row that is done alone
+
+// One row of one query head by one warp, key by key: o = sum_j p_j v_j / sum_j
+// p_j with p_j = exp(s_j - max), the maximum and both sums running.  Only keys
+// the row sees are read.  The tiled kernels multiply whole tiles, where an
+// infinity or NaN among the values of a key behind the row (0 times it) makes
+// the row NaN; such rows, which see fewer keys than the sequence holds, come
+// here.
+template <typename T, int S, int D>
+__device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int first, int rows, int length, int i,
+                                        int head) {
+    constexpr int kPer = D / 32;  // a lane's elements
+    const int lane = threadIdx.x & 31;
+    const int keys = a.causal ? min(length - rows + i + 1, length) : length;
+    const long long row = (long long)first + i;
+    const int kv = head / a.group;
+    float qv[kPer], o[kPer];
+    const unsigned char* qp = a.queries + row * a.q_row + head * a.q_head + lane * (kPer * 2);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+        const float2 f = Half16<T>::pair_to_float2(*reinterpret_cast<const uint32_t*>(qp + e * 2));
+        qv[e] = f.x;
+        qv[e + 1] = f.y;
+        o[e] = o[e + 1] = 0.f;
+    }
+    float top = -INFINITY, total = 0.f;
+    for (int j = 0; j < keys; ++j) {
+        const int page = cache_page(a.cache, a.batch, s, j);
+        float k[kPer], v[kPer], ks = 1.f, vs = 1.f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) k[e] = v[e] = 0.f;
+        if (page >= 0) {
+            const int slot = j & ((1 << a.cache.page_shift) - 1);
+            const long long at = cache_offset(a.cache, page, kv, slot) + lane * kPer * cache_bytes(S);
+#pragma unroll
+            for (int e = 0; e < kPer; e += 2) {
+                using Pair = typename std::conditional<cache_eight(S), uint16_t, uint32_t>::type;
+                const float2 fk = cache_pair<S>(*reinterpret_cast<const Pair*>(a.cache.keys + at + e * cache_bytes(S)));
+                const float2 fv = cache_pair<S>(*reinterpret_cast<const Pair*>(a.cache.values + at + e * cache_bytes(S)));
+                k[e] = fk.x, k[e + 1] = fk.y, v[e] = fv.x, v[e + 1] = fv.y;
+            }
+            if (cache_eight(S)) {
+                const long long si = cache_scale_index(a.cache, page, kv, slot);
+                ks = cache_scale(a.cache.key_scales[si]);
+                vs = cache_scale(a.cache.value_scales[si]);
+            }
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) dot += qv[e] * k[e];
+        const float score = warp_sum(dot) * ks * a.scale;
+        const float higher = fmaxf(top, score);
+        const float from = higher == -INFINITY ? 0.f : higher;
+        const float keep = expf(top - from), p = expf(score - from);
+        total = total * keep + p;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[e] = o[e] * keep + p * (v[e] * vs);
+        top = higher;
+    }
+    const float inverse = keys > 0 ? 1.f / total : 0.f;
+    unsigned char* op = a.out + row * a.o_row + head * a.o_head + lane * (kPer * 2);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2)
+        *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(o[e] * inverse, o[e + 1] * inverse);
+    if (a.lse && lane == 0) a.lse[row * a.query_heads + head] = keys > 0 ? top + logf(total) : -INFINITY;
+}
+
+// ------------------------------------------------------------ a tile's rows
+
+// Packed row R of a sequence's n * group rows of one key head is token R /
+// group of query head R % group.
+struct TileRow {
+    int token, head, seen;  // seen: the keys it sees
+    bool valid;
+};
+__device__ __forceinline__ TileRow tile_row(const CacheAttendArgs& a, const CacheSequence& q, int kv, int packed) {
+    TileRow r;
+    r.token = a.group == 1 ? packed : packed / a.group;
+    r.head = kv * a.group + packed - r.token * a.group;
+    const long long row = (long long)q.first + r.token;
+    r.valid = r.token < q.rows && row >= 0 && row < a.rows;
+    r.seen = a.causal ? max(0, min(q.length - q.rows + r.token + 1, q.length)) : max(q.length, 0);
+    return r;
+}
+
+}  // namespace wsp
