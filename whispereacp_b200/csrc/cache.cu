@@ -496,6 +496,8 @@ int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, i
         if (!(scale == scale) || scale - scale != 0.f) throw wsp::InvalidArgument("scale must be finite");
         if (reinterpret_cast<uintptr_t>(lse) & 3) throw wsp::InvalidArgument("lse must be 4-byte aligned");
         if (rows == 0 || batch->sequences == 0) return;
+        if ((long long)rows * query_heads > 0x7fff0000ll)
+            throw wsp::InvalidArgument("too many rows for one call: " + to_string(rows));
         if (needed && (!workspace || !wsp::aligned(workspace) || workspace_bytes < needed))
             throw wsp::InvalidArgument("the workspace must be 16-byte aligned and hold " + to_string(needed) + " bytes, not " +
                                        to_string(workspace ? workspace_bytes : 0));

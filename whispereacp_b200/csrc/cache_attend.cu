@@ -29,8 +29,7 @@
 // multiplies its probability, relative to the warp's largest so far, so that
 // the product stays in fp16's range whatever the scales are.  bf16 queries
 // become fp16 after a power of two a row brings them near 1.
-#include "cache_device.cuh"
-#include "host.h"
+#include "cache_join.cuh"
 
 #include <algorithm>
 
@@ -69,32 +68,21 @@ struct TokenLayout {
     static_assert(stages >= 2 && stages <= 14, "a ring");
 };
 
-// Workspace: a record for each CTA whose run begins inside an item, then two
-// partial results for each CTA: [0] of the item its run begins in, [1] of the
-// item its run ends in.
-struct CutItem {
-    int parts;  // partial results of the item, if this CTA's is the second; else 0
-    int sequence, head, tile;
-};
-template <int D, int NT>
-struct Partial {
-    static constexpr int rows = 8 * NT;
-    static constexpr int floats = rows * (D + 2);  // o, then m, then sum
-};
-
 template <int kKeys>
 __device__ __forceinline__ int item_units(int length) {
     return max(1, (length + kKeys - 1) / kKeys);
 }
 
-// The items of a sequence of one head: tiles of its n * group rows.
+// The items of a sequence of one head: tiles of its n * group rows, none where
+// those are more than this kernel is to take.
 template <int kRows>
-__device__ __forceinline__ int item_tiles(const CacheSequence& q, int group) {
-    return q.rows > 0 ? (int)(((long long)q.rows * group + kRows - 1) / kRows) : 0;
+__device__ __forceinline__ int item_tiles(const CacheSequence& q, const CacheAttendArgs& a) {
+    const long long rows = (long long)q.rows * a.group;
+    return rows > 0 && rows <= a.few ? (int)((rows + kRows - 1) / kRows) : 0;
 }
 template <int kKeys, int kRows>
-__device__ __forceinline__ long long sequence_units(const CacheSequence& q, int group, int heads) {
-    return (long long)item_tiles<kRows>(q, group) * heads * item_units<kKeys>(q.length);
+__device__ __forceinline__ long long sequence_units(const CacheSequence& q, const CacheAttendArgs& a) {
+    return (long long)item_tiles<kRows>(q, a) * a.cache.heads * item_units<kKeys>(q.length);
 }
 
 // Where a unit lies; every warp finds it for itself.
@@ -106,19 +94,10 @@ struct Place {
     int units, tiles; // of the item; items of a head
 };
 
-__device__ __forceinline__ long long warp_scan(long long v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += up;
-    }
-    return v;
-}
-
 template <int kKeys, int kRows>
-__device__ __forceinline__ long long all_units(const CacheBatchView& b, int group, int heads, int lane) {
+__device__ __forceinline__ long long all_units(const CacheAttendArgs& a, int lane) {
     long long sum = 0;
-    for (int s = lane; s < b.sequences; s += 32) sum += sequence_units<kKeys, kRows>(cache_sequence(b, s), group, heads);
+    for (int s = lane; s < a.batch.sequences; s += 32) sum += sequence_units<kKeys, kRows>(cache_sequence(a.batch, s), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
@@ -126,13 +105,13 @@ __device__ __forceinline__ long long all_units(const CacheBatchView& b, int grou
 
 // The place of unit u (below all_units); a warp.
 template <int kKeys, int kRows>
-__device__ __forceinline__ Place find_unit(const CacheBatchView& b, int group, int heads, long long u, int lane) {
+__device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u, int lane) {
     Place p{};
-    for (int base = 0; base < b.sequences; base += 32) {
+    for (int base = 0; base < a.batch.sequences; base += 32) {
         const int s = base + lane;
         CacheSequence q{};
-        if (s < b.sequences) q = cache_sequence(b, s);
-        const long long mine = s < b.sequences ? sequence_units<kKeys, kRows>(q, group, heads) : 0;
+        if (s < a.batch.sequences) q = cache_sequence(a.batch, s);
+        const long long mine = s < a.batch.sequences ? sequence_units<kKeys, kRows>(q, a) : 0;
         const long long upto = warp_scan(mine, lane);
         const unsigned holds = __ballot_sync(0xffffffffu, u < upto);
         if (holds) {
@@ -143,7 +122,7 @@ __device__ __forceinline__ Place find_unit(const CacheBatchView& b, int group, i
             p.q.rows = __shfl_sync(0xffffffffu, q.rows, at);
             p.q.length = __shfl_sync(0xffffffffu, q.length, at);
             p.units = item_units<kKeys>(p.q.length);
-            p.tiles = item_tiles<kRows>(p.q, group);
+            p.tiles = item_tiles<kRows>(p.q, a);
             const long long item = inside / p.units;
             p.unit = (int)(inside - item * p.units);
             p.head = (int)(item / p.tiles);
@@ -157,15 +136,15 @@ __device__ __forceinline__ Place find_unit(const CacheBatchView& b, int group, i
 
 // The next item's first unit.
 template <int kKeys, int kRows>
-__device__ __forceinline__ void next_item(Place& p, const CacheBatchView& b, int group, int heads) {
+__device__ __forceinline__ void next_item(Place& p, const CacheAttendArgs& a) {
     p.unit = 0;
     if (++p.tile < p.tiles) return;
     p.tile = 0;
-    if (++p.head < heads) return;
+    if (++p.head < a.cache.heads) return;
     p.head = 0;
-    while (++p.s < b.sequences) {
-        p.q = cache_sequence(b, p.s);
-        p.tiles = item_tiles<kRows>(p.q, group);
+    while (++p.s < a.batch.sequences) {
+        p.q = cache_sequence(a.batch, p.s);
+        p.tiles = item_tiles<kRows>(p.q, a);
         if (p.tiles > 0) break;
     }
     p.units = item_units<kKeys>(p.q.length);
@@ -347,7 +326,7 @@ __device__ __forceinline__ void token_producer(const CacheAttendArgs& a, const C
             }
         }
         if (*abort) break;
-        next_item<Layout::keys, Layout::rows>(p, a.batch, a.group, a.cache.heads);
+        next_item<Layout::keys, Layout::rows>(p, a);
     }
     if (*abort)  // the copies in flight land before the CTA's memory is given up
         for (int i = max(0, n - Layout::stages); i < n; ++i) {
@@ -375,7 +354,6 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     volatile int* abort = reinterpret_cast<volatile int*>(empty + Layout::stages);
     int* redo = reinterpret_cast<int*>(empty + Layout::stages) + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int heads = a.cache.heads;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < Layout::stages; ++i) {
@@ -386,16 +364,16 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         *redo = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const long long total = all_units<Layout::keys, kRows>(a.batch, a.group, heads, lane);
+    const long long total = all_units<Layout::keys, kRows>(a, lane);
     const long long per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
     const long long begin = min(total, blockIdx.x * per), end = min(total, begin + per);
-    Place p = begin < end ? find_unit<Layout::keys, kRows>(a.batch, a.group, heads, begin, lane) : Place{};
+    Place p = begin < end ? find_unit<Layout::keys, kRows>(a, begin, lane) : Place{};
     if (threadIdx.x == 0) {
         CutItem cut{};
         const long long first = begin - p.unit;  // the item's
         if (begin < end && p.unit > 0 && first >= begin - per)
             cut = {(int)((first + p.units - 1) / per - blockIdx.x) + 2, p.s, p.head, p.tile};
-        reinterpret_cast<CutItem*>(a.workspace)[blockIdx.x] = cut;
+        cut_items(a)[blockIdx.x] = cut;
     }
     __syncthreads();
     if (begin >= end) return;
@@ -405,7 +383,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     }
 
     // ----------------------------------------------------------- consumers
-    float* partials = reinterpret_cast<float*>(a.workspace + ((sizeof(CutItem) * gridDim.x + 255) / 256) * 256);
+    float* partials = cut_partials(a, gridDim.x);
     const int g = lane >> 2, t4 = lane & 3;
     float* join = reinterpret_cast<float*>(smem + Layout::join_at);
     float* ml = reinterpret_cast<float*>(smem + Layout::ml_at);
@@ -436,7 +414,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         Place pn = p;
         const bool more = u + (last - p.unit) < end;
         if (more) {
-            next_item<Layout::keys, kRows>(pn, a.batch, a.group, heads);
+            next_item<Layout::keys, kRows>(pn, a);
             load_queries<T, S, D, NT>(a, pn, qn, lane);
         }
         float o[kSteps][NT][4];
@@ -709,7 +687,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const bool whole = p.unit == 0 && last == p.units;
         constexpr int kRowThreads = D / 2;  // a thread two columns of a row
-        float* part = partials + ((long long)blockIdx.x * 2 + (p.unit > 0 ? 0 : 1)) * Partial<D, NT>::floats;
+        float* part = partials + ((long long)blockIdx.x * 2 + (p.unit > 0 ? 0 : 1)) * Partial<D, kRows>::floats;
         for (int row = threadIdx.x / kRowThreads; row < valid; row += 128 / kRowThreads) {
             const int d = (threadIdx.x % kRowThreads) * 2;
             float top = -INFINITY, all = 0.f;
@@ -764,93 +742,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     }
 }
 
-// ----------------------------------------------------------------- the join
-
-constexpr int kJoinRows = 4;
-
-// Block (c, y) joins rows 4 y .. of the item that the border between the runs
-// of CTAs c and c + 1 cuts, if no earlier border does.  Its warps share out
-// the rows and each row's partial results.
-template <typename T, int S, int D, int NT, int kThreads>
-__global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_constant__ CacheAttendArgs a, int grid) {
-    constexpr int kPer = D / 32;
-    constexpr int kJoinWarps = kThreads / 32;
-    constexpr int kRows = 8 * NT;
-    __shared__ float shared_o[kJoinWarps][D];
-    __shared__ float shared_ml[kJoinWarps][2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = blockIdx.x + 1;
-    const int4 record = *reinterpret_cast<const int4*>(reinterpret_cast<const CutItem*>(a.workspace) + c);
-    const CutItem cut = {record.x, record.y, record.z, record.w};
-    if (cut.parts == 0) return;
-    const float* partials = reinterpret_cast<const float*>(a.workspace + ((sizeof(CutItem) * grid + 255) / 256) * 256);
-    const CacheSequence q = cache_sequence(a.batch, cut.sequence);
-    const int all_rows = (int)min((long long)kRows, (long long)q.rows * a.group - (long long)cut.tile * kRows);
-    for (int first = (int)blockIdx.y * kJoinRows; first < all_rows; first += (int)gridDim.y * kJoinRows) {
-        const int rows = min(kJoinRows, all_rows - first);
-        int share = 1;  // warps of a row
-        while (share * 2 * rows <= kJoinWarps && share < cut.parts) share *= 2;
-        const int local = warp / share, sub = warp % share, row = first + local;
-        const bool active = local < rows;
-        float m = -INFINITY, sum = 0.f, o[kPer];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-        const auto add = [&](float pm, float ps, const float* v) {
-            const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
-            const float keep = exp2_fast(m - base), gain = exp2_fast(pm - base);
-            sum = sum * keep + ps * gain;
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) o[e] = o[e] * keep + v[e] * gain;
-            m = top;
-        };
-        if (active) {
-            const int from = (int)((long long)cut.parts * sub / share), to = (int)((long long)cut.parts * (sub + 1) / share);
-#pragma unroll 4
-            for (int i = from; i < to; ++i) {
-                const float* part = partials + ((long long)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * Partial<D, NT>::floats;
-                float v[kPer];
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) v[e] = part[row * D + lane * kPer + e];
-                add(part[kRows * D + row], part[kRows * (D + 1) + row], v);
-            }
-        }
-        if (share > 1) {
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) shared_o[warp][lane * kPer + e] = o[e];
-            if (lane == 0) {
-                shared_ml[warp][0] = m;
-                shared_ml[warp][1] = sum;
-            }
-            __syncthreads();
-            if (sub == 0)
-                for (int w = warp + 1; w < warp + share; ++w) add(shared_ml[w][0], shared_ml[w][1], &shared_o[w][lane * kPer]);
-        }
-        if (!active || sub != 0) continue;
-        const TileRow r = tile_row(a, q, cut.head, cut.tile * kRows + row);
-        if (!r.valid) continue;
-        const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
-        const long long at = (long long)q.first + r.token;
-        unsigned char* op = a.out + at * a.o_row + r.head * a.o_head + lane * (kPer * 2);
-        bool fine = true;
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) {
-            const float x = o[e] * inverse, y = o[e + 1] * inverse;
-            fine = fine && fabsf(x) + fabsf(y) < INFINITY;
-            *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(x, y);
-        }
-        if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
-        if (__any_sync(0xffffffffu, !fine) && r.seen < q.length && r.seen > 0)
-            attend_row<T, S, D>(a, cut.sequence, q.first, q.rows, q.length, r.token, r.head);
-    }
-}
-
 // ------------------------------------------------------------------- launch
-
-size_t token_workspace(long long grid, int width, int rows) {
-    return (sizeof(CutItem) * grid + 255) / 256 * 256 + grid * 2 * rows * (width + 2) * 4;
-}
 
 // CTAs of the few-row kernel: all that the SMs hold, or as many as there can
 // be units (the table bounds a sequence's, the rows the tiles).
@@ -867,47 +759,26 @@ void launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, cud
     const int grid = (int)token_grid<Layout>(a, sms);
     cache_tokens_kernel<T, S, D, NT><<<grid, kTokenThreads, Layout::bytes, stream>>>(a, maps);
     CUDA_CHECK(cudaGetLastError());
-    if (grid == 1) return;
-    // The join's launch overlaps the end of the kernel it waits for.  Where
-    // items are far fewer than CTAs, 16 warps share a row's many parts.
-    const bool many = grid > 8ll * a.cache.heads * a.batch.sequences;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid - 1, NT * 8 / kJoinRows);
-    config.blockDim = dim3(many ? 512 : 128);
-    config.stream = stream;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, many ? cache_join_kernel<T, S, D, NT, 512> : cache_join_kernel<T, S, D, NT, 128>,
-                                  a, grid));
-}
-
-template <typename F>
-void with_types(int storage, bool bf16, int width, F&& f) {
-    const auto typed = [&](auto t, auto s) {
-        if (width == 64) f(t, s, std::integral_constant<int, 64>{});
-        else f(t, s, std::integral_constant<int, 128>{});
-    };
-    if (storage == kCacheF16) typed(__half{}, std::integral_constant<int, kCacheF16>{});
-    else if (storage == kCacheBf16) typed(__nv_bfloat16{}, std::integral_constant<int, kCacheBf16>{});
-    else if (storage == kCacheE4m3 && bf16) typed(__nv_bfloat16{}, std::integral_constant<int, kCacheE4m3>{});
-    else if (storage == kCacheE4m3) typed(__half{}, std::integral_constant<int, kCacheE4m3>{});
-    else if (bf16) typed(__nv_bfloat16{}, std::integral_constant<int, kCacheInt8>{});
-    else typed(__half{}, std::integral_constant<int, kCacheInt8>{});
+    launch_join<T, S, D, Layout::rows>(a, grid, stream);
 }
 
 }  // namespace
 
-size_t cache_attend_workspace(const CacheAttendShape& shape, int) {
-    // 3 CTAs of 8-row tiles, or 2 of 16-row tiles
-    return std::max(token_workspace(shape.sms * 3, shape.width, 8), token_workspace(shape.sms * 2, shape.width, 16));
+// Rows of a key head up to which a sequence is the few-row kernel's: one of
+// its larger tiles.
+constexpr int kFewRows = 16;
+
+size_t cache_attend_workspace(const CacheAttendShape& shape, int group) {
+    // 3 CTAs of 8-row tiles, or 2 of 16-row tiles; the kernels of a call, one
+    // after the other, share it
+    const size_t few = std::max(cut_workspace(shape.sms * 3, shape.width, 8), cut_workspace(shape.sms * 2, shape.width, 16));
+    const bool chunks = cache_chunk_takes(shape.storage) && (long long)shape.max_rows * group > kFewRows;
+    return chunks ? std::max(few, cache_chunk_workspace(shape)) : few;
 }
 
 void prepare_cache_attend(int storage, int width) {
     for (bool bf16 : {false, true})
-        with_types(storage, bf16, width, [&](auto t, auto s, auto d) {
+        with_cache_types(storage, bf16, width, [&](auto t, auto s, auto d) {
             using T = decltype(t);
             constexpr int S = s.value, D = d.value;
             CUDA_CHECK(cudaFuncSetAttribute(cache_tokens_kernel<T, S, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -915,14 +786,21 @@ void prepare_cache_attend(int storage, int width) {
             CUDA_CHECK(cudaFuncSetAttribute(cache_tokens_kernel<T, S, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             TokenLayout<S, D, 2>::bytes));
         });
+    prepare_cache_chunk(storage, width);
 }
 
-void launch_cache_attend(const CacheAttendArgs& a, const CacheMaps& maps, const CacheAttendShape& shape,
+void launch_cache_attend(const CacheAttendArgs& args, const CacheMaps& maps, const CacheAttendShape& shape,
                          cudaStream_t stream) {
+    CacheAttendArgs a = args;
+    const long long most = (long long)shape.max_rows * a.group;
+    a.few = 0x7fffffffffffll;
+    if (most > kFewRows && cache_chunk_takes(shape.storage)) {
+        a.few = kFewRows;
+        launch_cache_chunk(a, maps, shape, stream);
+    }
     // Tiles of 8 rows where every sequence's rows of a head fit one.
-    const bool few = (long long)shape.max_rows * a.group <= 8;
-    with_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
-        if (few) launch_tokens<decltype(t), s.value, d.value, 1>(a, maps, shape.sms, stream);
+    with_cache_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
+        if (most <= 8) launch_tokens<decltype(t), s.value, d.value, 1>(a, maps, shape.sms, stream);
         else launch_tokens<decltype(t), s.value, d.value, 2>(a, maps, shape.sms, stream);
     });
 }

@@ -21,6 +21,7 @@ struct CacheAttendArgs {
     int rows, query_heads, group;  // group = query heads of a key head
     float scale;
     int causal;
+    long long few;                 // rows * group up to which a sequence is the few-row kernel's
     int* status;                   // which wait gave up, 0: none
     unsigned char* workspace;
 };
@@ -38,6 +39,14 @@ struct CacheAttendShape {
     bool bf16;
     int width, max_rows, sms;
 };
+
+// The kernel of many rows (cache_chunk.cu): sequences of more than `few` rows
+// of a key head.
+void prepare_cache_chunk(int storage, int width);
+void launch_cache_chunk(const CacheAttendArgs& args, const CacheMaps& maps, const CacheAttendShape& shape,
+                        cudaStream_t stream);
+size_t cache_chunk_workspace(const CacheAttendShape& shape);
+bool cache_chunk_takes(int storage);
 
 // Raises the kernels' limits of shared memory on the current device.
 void prepare_cache_attend(int storage, int width);

@@ -1,0 +1,640 @@
+// The attention of chunks of new rows over a paged cache, on the tcgen05 tensor
+// cores (sm_100a).  The mathematics is cache_attend.cu's; here a key or value
+// meets hundreds of rows, so the products and the exponentials bound it.
+//
+// An item is (sequence, key head, 256 packed rows): two tiles of 128 rows (the
+// products' M) over the blocks of 128 keys that their last row sees.  A tile's
+// 128 x 128 scores cost 128 x 128 exponentials, 1024 cycles of an SM's 16 a
+// cycle, next to 4 x 128 x 128 x D flop, 512 (D 64) or 1024 cycles of the tensor
+// cores: neither may wait for the other.  So two tiles take turns:
+//
+//   warps 0-3, 4-7  the softmax of tile 0 and of tile 1, a thread a row: read
+//                   the scores from tensor memory, p = 2^(s - m), P as 16-bit
+//                   values back into the scores' columns (rounded once: what
+//                   the products take), the sum of p in a register.  The
+//                   maximum moves only when it grows by more than 2^8; then
+//                   the thread rescales its row of o in tensor memory.
+//   warp 8          issues the products: S_t = Q_t K^T (both from shared
+//                   memory) and O_t += P_t V (P from tensor memory), those of
+//                   one tile while the other's softmax runs.
+//   warp 9          copies the blocks' keys and values into a ring, a box a
+//                   page, as the 128-byte-swizzled tiles the products read:
+//                   keys K-major, values MN-major, as they lie in the cache.
+//
+// Tensor memory: S_0, S_1 (128 columns each, P in the first 64), O_0, O_1 (D
+// columns each).  The order of products on one issuing thread is the order of
+// their execution, so S_t of the next block may follow P_t V in P_t's place,
+// and the commit behind S_t also says that O_t stands still.
+//
+// The blocks of all items form one list, dealt evenly over the SMs as in
+// cache_attend.cu; cut items leave partial results for the join.
+#include "cache_join.cuh"
+
+#include <algorithm>
+
+namespace wsp {
+namespace {
+
+constexpr int kBlockKeys = 128;
+constexpr int kTile = 128;          // rows of a tile
+constexpr int kPair = 2 * kTile;    // rows of an item
+constexpr int kMmaWarp = 8;
+constexpr int kCopyWarp = 9;
+constexpr int kChunkThreads = 320;
+constexpr int kHalfBytes = kTile * 128;  // 128 rows of 64 16-bit columns
+
+enum ChunkWait : int { kWaitBlock = 11, kWaitSlot = 12, kWaitScores = 13, kWaitP = 14, kWaitQueries = 15, kWaitO = 16,
+                       kWaitDone = 17 };
+
+template <int S, int D>
+struct ChunkLayout {
+    static constexpr int halves = D / 64;
+    static constexpr int tile_bytes = halves * kHalfBytes;  // of Q_t, or of a block's keys or values
+    static constexpr int stages = D == 64 ? 8 : 5;
+    static constexpr int ring_at = 2 * tile_bytes;
+    static constexpr int bar_at = ring_at + stages * tile_bytes;
+    // full, empty; per tile: scores, P, queries, O; done
+    static constexpr int bars = 2 * stages + 8 + 1;
+    static constexpr int bytes = bar_at + bars * 8 + 16;
+};
+
+// ------------------------------------------------------------ the block list
+
+struct ChunkPlace {
+    int s;
+    CacheSequence q;
+    int head, pair;
+    int block, blocks;  // the item's first in this run; its blocks
+    int pairs;
+};
+
+__device__ __forceinline__ int chunk_pairs(const CacheSequence& q, const CacheAttendArgs& a) {
+    const long long rows = (long long)q.rows * a.group;
+    return rows > a.few ? (int)((rows + kPair - 1) / kPair) : 0;
+}
+
+// Keys that any of the first `rows` packed rows sees.
+__device__ __forceinline__ int chunk_seen(const CacheSequence& q, const CacheAttendArgs& a, long long rows) {
+    if (!a.causal) return max(q.length, 0);
+    const int token = (int)((min(rows, (long long)q.rows * a.group) - 1) / a.group);
+    return max(0, min(q.length - q.rows + token + 1, q.length));
+}
+__device__ __forceinline__ int chunk_blocks(const CacheSequence& q, const CacheAttendArgs& a, int pair) {
+    return max(1, (chunk_seen(q, a, (long long)(pair + 1) * kPair) + kBlockKeys - 1) / kBlockKeys);
+}
+__device__ __forceinline__ long long chunk_units(const CacheSequence& q, const CacheAttendArgs& a) {
+    const int pairs = chunk_pairs(q, a);
+    long long sum = 0;
+    if (!a.causal) sum = pairs ? (long long)pairs * chunk_blocks(q, a, 0) : 0;
+    else
+        for (int p = 0; p < pairs; ++p) sum += chunk_blocks(q, a, p);
+    return sum * a.cache.heads;
+}
+
+__device__ long long all_blocks(const CacheAttendArgs& a, int lane) {
+    long long sum = 0;
+    for (int s = lane; s < a.batch.sequences; s += 32) sum += chunk_units(cache_sequence(a.batch, s), a);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
+__device__ ChunkPlace find_block(const CacheAttendArgs& a, long long u, int lane) {
+    ChunkPlace p{};
+    for (int base = 0; base < a.batch.sequences; base += 32) {
+        const int s = base + lane;
+        CacheSequence q{};
+        if (s < a.batch.sequences) q = cache_sequence(a.batch, s);
+        const long long mine = s < a.batch.sequences ? chunk_units(q, a) : 0;
+        const long long upto = warp_scan(mine, lane);
+        const unsigned holds = __ballot_sync(0xffffffffu, u < upto);
+        if (holds) {
+            const int at = __ffs(holds) - 1;
+            long long inside = __shfl_sync(0xffffffffu, u - (upto - mine), at);
+            p.s = base + at;
+            p.q.first = __shfl_sync(0xffffffffu, q.first, at);
+            p.q.rows = __shfl_sync(0xffffffffu, q.rows, at);
+            p.q.length = __shfl_sync(0xffffffffu, q.length, at);
+            p.pairs = chunk_pairs(p.q, a);
+            const long long head = __shfl_sync(0xffffffffu, mine, at) / a.cache.heads;  // blocks of a head
+            p.head = (int)(inside / head);
+            inside -= p.head * head;
+            for (;; ++p.pair) {
+                p.blocks = chunk_blocks(p.q, a, p.pair);
+                if (inside < p.blocks) break;
+                inside -= p.blocks;
+            }
+            p.block = (int)inside;
+            return p;
+        }
+        u -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return p;
+}
+
+__device__ __forceinline__ void next_pair(ChunkPlace& p, const CacheAttendArgs& a) {
+    p.block = 0;
+    if (++p.pair >= p.pairs) {
+        p.pair = 0;
+        if (++p.head >= a.cache.heads) {
+            p.head = 0;
+            while (++p.s < a.batch.sequences) {
+                p.q = cache_sequence(a.batch, p.s);
+                p.pairs = chunk_pairs(p.q, a);
+                if (p.pairs > 0) break;
+            }
+        }
+    }
+    p.blocks = chunk_blocks(p.q, a, p.pair);
+}
+
+// The blocks of tile t of an item: 0 if it has no rows, else one at least.
+__device__ __forceinline__ int tile_blocks(const ChunkPlace& p, const CacheAttendArgs& a, int t) {
+    const long long first = (long long)p.pair * kPair + t * kTile;
+    if (first >= (long long)p.q.rows * a.group) return 0;
+    return max(1, (chunk_seen(p.q, a, first + kTile) + kBlockKeys - 1) / kBlockKeys);
+}
+
+// ------------------------------------------------------------ tensor pieces
+
+// The value tile as a product's B, MN-major: 128-byte rows of 64 columns, 8 of
+// them (keys) 1024 bytes apart from the next 8, the next 64 columns a half on.
+__device__ __forceinline__ uint64_t value_desc(uint32_t address) {
+    return (uint64_t)((address >> 4) & 0x3FFF) | ((uint64_t)(kHalfBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// D[tmem] (+)= A[tmem] . B, one thread.
+__device__ __forceinline__ void umma_mma_p(uint32_t tmem, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 columns of this warp's lanes on their way into r; tmem_arrived waits for
+// every such load so far, and r may be used behind it.
+__device__ __forceinline__ void tmem_load32_begin(uint32_t address, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(address)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            address),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(address),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// ---------------------------------------------------------------- the roles
+
+struct ChunkBars {
+    uint64_t *full, *empty, *scores, *p, *queries, *o, *done;
+};
+
+template <int S, int D>
+__device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsigned char* smem, const ChunkBars& bar,
+                           volatile int* abort, ChunkPlace p, long long begin, long long end, int lane) {
+    using Layout = ChunkLayout<S, D>;
+    const int box_shift = cache_box_shift(a.cache.page_shift);
+    const int box_rows = 1 << box_shift;
+    const int boxes = kBlockKeys >> box_shift;
+    int stage = 0, n = 0;
+    uint32_t parity = 1;
+    for (long long u = begin; u < end;) {
+        const int last = (int)min((long long)p.blocks, p.block + (end - u));
+        const int seen = chunk_seen(p.q, a, (long long)(p.pair + 1) * kPair);
+        for (int j = p.block; j < last; ++j, ++u) {
+            const int position = j * kBlockKeys + (min(lane, boxes - 1) << box_shift);
+            const int row = position & ((1 << a.cache.page_shift) - 1);
+            const bool mine = lane < boxes && position < seen;
+            int page = mine ? cache_page(a.cache, a.batch, p.s, position) : -1;
+            if (page < 0) page = a.cache.pages;  // outside: zeros
+            const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * (uint32_t)(box_rows * D * 2);
+            for (int v = 0; v < 2; ++v) {
+                if (n >= Layout::stages && !cache_wait(bar.empty + stage, parity, abort, a.status, kWaitSlot)) break;
+                if (*abort) break;
+                unsigned char* to = smem + Layout::ring_at + stage * Layout::tile_bytes + lane * box_rows * 128;
+                if (lane == 0) cache_arrive_expect(bar.full + stage, bytes);
+                __syncwarp();
+                if (mine)
+#pragma unroll
+                    for (int h = 0; h < Layout::halves; ++h)
+                        cache_copy_box(to + h * kHalfBytes, v ? &maps.values : &maps.keys, h * 64, row, p.head, page,
+                                       bar.full + stage);
+                ++n;
+                if (++stage == Layout::stages) {
+                    stage = 0;
+                    parity ^= 1;
+                }
+            }
+            if (*abort) break;
+        }
+        if (*abort) break;
+        next_pair(p, a);
+    }
+    if (*abort)  // the copies in flight land before the CTA's memory is given up
+        for (int i = max(0, n - Layout::stages); i < n; ++i) {
+            const unsigned long long start = cache_clock_ns();
+            while (!cache_phase_done(bar.full + i % Layout::stages, (uint32_t)((i / Layout::stages) & 1)) &&
+                   cache_clock_ns() - start < kCacheTimeoutNs) {
+            }
+        }
+}
+
+template <typename T, int S, int D>
+__device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, uint32_t tmem,
+                               volatile int* abort, ChunkPlace p, long long begin, long long end, int lane) {
+    using Layout = ChunkLayout<S, D>;
+    const uint32_t score_desc = umma_idesc<T>(kBlockKeys), out_desc = umma_idesc<T>(D) | (1u << 16);
+    const uint32_t q_at = smem_address(smem), ring = smem_address(smem + Layout::ring_at);
+    int stage = 0;
+    uint32_t parity = 0, p_parity[2] = {0, 0}, q_parity[2] = {0, 0};
+    const auto advance = [&] {
+        if (++stage == Layout::stages) {
+            stage = 0;
+            parity ^= 1;
+        }
+    };
+    const auto scores = [&](int t, uint32_t keys) {
+        if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t at = (uint32_t)((k / 4) * kHalfBytes + (k % 4) * 32);
+                umma_mma(tmem + t * 128, umma_desc(q_at + t * Layout::tile_bytes + at), umma_desc(keys + at), score_desc,
+                         k != 0);
+            }
+            umma_commit(bar.scores + t);
+        }
+        __syncwarp();
+    };
+    for (long long u = begin; u < end;) {
+        const int last = (int)min((long long)p.blocks, p.block + (end - u));
+        const int blocks[2] = {min(last, tile_blocks(p, a, 0)), min(last, tile_blocks(p, a, 1))};
+        const int seen = chunk_seen(p.q, a, (long long)(p.pair + 1) * kPair);
+        // The first block's scores.
+        cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
+        for (int t = 0; t < 2; ++t)
+            if (p.block < blocks[t]) {
+                cache_wait(bar.queries + t, q_parity[t], abort, a.status, kWaitQueries);
+                q_parity[t] ^= 1;
+                tmem_fence_after();
+                scores(t, ring + stage * Layout::tile_bytes);
+            }
+        if (lane == 0) umma_commit(bar.empty + stage);
+        __syncwarp();
+        advance();
+        for (int j = p.block; j < last; ++j, ++u) {
+            const int v_stage = stage;
+            cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
+            const uint32_t values = ring + stage * Layout::tile_bytes;
+            if ((j + 1) * kBlockKeys > seen) {
+                // What lies behind the last row that the item sees was not
+                // copied or may be anything, and 0 times a NaN is one.
+                unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
+                const int from = max(0, seen - j * kBlockKeys);
+                for (int h = 0; h < Layout::halves; ++h)
+                    for (int i = from * 8 + lane; i < kBlockKeys * 8; i += 32)
+                        *reinterpret_cast<uint4*>(tile + h * kHalfBytes + i * 16) = make_uint4(0, 0, 0, 0);
+                cache_proxy_fence();
+                __syncwarp();
+            }
+            advance();
+            const int k_stage = stage;
+            if (j + 1 < last) {
+                cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
+                advance();
+            }
+            for (int t = 0; t < 2; ++t) {
+                if (j >= blocks[t]) continue;
+                cache_wait(bar.p + t, p_parity[t], abort, a.status, kWaitP);
+                p_parity[t] ^= 1;
+                tmem_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < kBlockKeys / 16; ++k)
+                        umma_mma_p(tmem + 256 + t * D, tmem + t * 128 + k * 8, value_desc(values + k * 2048), out_desc,
+                                   j > p.block || k != 0);
+                    if (j + 1 >= blocks[t]) umma_commit(bar.o + t);
+                }
+                __syncwarp();
+                if (j + 1 < blocks[t]) scores(t, ring + k_stage * Layout::tile_bytes);
+            }
+            if (lane == 0) {
+                umma_commit(bar.empty + v_stage);
+                if (j + 1 < last) umma_commit(bar.empty + k_stage);
+            }
+            __syncwarp();
+        }
+        next_pair(p, a);
+    }
+    // Every product has completed before the tensor memory goes.
+    if (lane == 0) {
+        umma_commit(bar.done);
+        const unsigned long long start = cache_clock_ns();
+        while (!cache_phase_done(bar.done, 0))
+            if (cache_clock_ns() - start > kCacheTimeoutNs) {
+                atomicCAS(a.status, 0, kWaitDone);
+                break;
+            }
+    }
+    __syncwarp();
+}
+
+template <typename T, int S, int D>
+__device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, uint32_t tmem,
+                              volatile int* abort, ChunkPlace p, long long begin, long long end, int t) {
+    using Layout = ChunkLayout<S, D>;
+    // fp16 keeps 2^-14 .. 2^15 whole: P's largest, 2^8 by the lazy maximum, is
+    // put at 2^15.  bf16 has fp32's range.
+    constexpr float kShift = std::is_same<T, __half>::value ? 7.f : 0.f;
+    constexpr float kLimit = 8.f + kShift;
+    const int row = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(row & ~31) << 16;
+    const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * D + lanes;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // the sign goes into the queries
+    const float to_log2 = fabsf(a.scale) * kLog2e;
+    uint32_t s_parity = 0, o_parity = 0;
+    for (long long u = begin; u < end;) {
+        const int last = (int)min((long long)p.blocks, p.block + (end - u));
+        const int blocks = min(last, tile_blocks(p, a, t));
+        const long long packed = (long long)p.pair * kPair + t * kTile;
+        const bool active = p.block < blocks;
+        const TileRow r = tile_row(a, p.q, p.head, (int)packed + row);
+        const long long at = (long long)p.q.first + r.token;
+        float from = 0.f, limit = -INFINITY, sum = 0.f;
+        if (active) {
+            // The row's queries, swizzled as the copy engine does it.
+            const unsigned char* qp = a.queries + at * a.q_row + r.head * a.q_head;
+#pragma unroll
+            for (int h = 0; h < Layout::halves; ++h)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r.valid) v = *reinterpret_cast<const uint4*>(qp + h * 128 + c * 16);
+                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                    *reinterpret_cast<uint4*>(smem + t * Layout::tile_bytes + h * kHalfBytes + row * 128 +
+                                              ((c ^ (row & 7)) << 4)) = v;
+                }
+            cache_proxy_fence();
+            cache_arrive(bar.queries + t);
+            // Keys below `clear` are seen by every row of the tile.
+            const int clear = tile_row(a, p.q, p.head, (int)packed).seen;
+            for (int j = p.block; j < blocks; ++j) {
+                cache_wait(bar.scores + t, s_parity, abort, a.status, kWaitScores);
+                s_parity ^= 1;
+                tmem_fence_after();
+                // The scores are read twice, 32 at a time with the next 32 on
+                // their way: for the maximum, then for P, whose columns trail
+                // the scores' that were read.
+                uint32_t s[2][32];
+                const bool masked = (j + 1) * kBlockKeys > clear;
+                const int seen = r.seen - j * kBlockKeys;
+                const auto take = [&](int c) {
+                    tmem_arrived(s[c & 1]);
+                    if (c < 7) tmem_load32_begin(s_at + ((c + 1) & 3) * 32, s[(c + 1) & 1]);
+                    if (masked)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if ((c & 3) * 32 + e >= seen) s[c & 1][e] = 0xff800000u;
+                };
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_load32_begin(s_at, s[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    take(c);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c & 1][e]));
+                }
+                const float higher = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * to_log2;
+                // -infinity times a scale of 0 is no number, and no maximum
+                const bool grows = higher - from > limit;
+                if (__any_sync(0xffffffffu, grows)) {
+                    float keep = 1.f;
+                    if (grows) {
+                        keep = limit == -INFINITY ? 0.f : exp2_fast(from - (higher - kShift));
+                        from = higher - kShift;
+                        limit = kLimit;
+                        sum *= keep;
+                    }
+                    if (j > p.block) {
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_load32(o_at + c * 32, o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_store32(o_at + c * 32, o);
+                        }
+                    }
+                }
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 4; c < 8; ++c) {
+                    take(c);
+                    uint32_t packed16[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float x = exp2_fast(fmaf(__uint_as_float(s[c & 1][e]), to_log2, -from));
+                        const float y = exp2_fast(fmaf(__uint_as_float(s[c & 1][e + 1]), to_log2, -from));
+                        part[e & 2] += x;
+                        part[(e & 2) + 1] += y;
+                        packed16[e / 2] = Half16<T>::pack2(x, y);
+                    }
+                    tmem_store16(s_at + (c & 3) * 16, packed16);
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                tmem_store_wait();
+                tmem_fence_before();
+                cache_arrive(bar.p + t);
+            }
+            cache_wait(bar.o + t, o_parity, abort, a.status, kWaitO);
+            o_parity ^= 1;
+            tmem_fence_after();
+        }
+        const bool whole = p.block == 0 && last == p.blocks;
+        const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
+        const float log_sum = limit == -INFINITY ? -INFINITY : from;
+        float* part = cut_partials(a, gridDim.x) + ((long long)blockIdx.x * 2 + (p.block > 0 ? 0 : 1)) * Partial<D, kPair>::floats;
+        bool fine = true;
+        unsigned char* op = a.out + at * a.o_row + r.head * a.o_head;
+        if (active || !whole) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                if (active) tmem_load32(o_at + c * 32, o);
+                else
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                if (!r.valid) continue;
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = __uint_as_float(o[e + 2 * i]) * inverse, y = __uint_as_float(o[e + 2 * i + 1]) * inverse;
+                            fine = fine && fabsf(x) + fabsf(y) < INFINITY;
+                            w[i] = Half16<T>::pack2(x, y);
+                        }
+                        *reinterpret_cast<uint4*>(op + c * 64 + e * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(part + (t * kTile + row) * D + c * 32 + e) =
+                            make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+        }
+        if (r.valid && whole && a.lse) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (log_sum + log2f(sum)) * kLn2 : -INFINITY;
+        if (r.valid && !whole) {
+            part[kPair * D + t * kTile + row] = log_sum;
+            part[kPair * (D + 1) + t * kTile + row] = sum;
+        }
+        // Rows that a key behind them made no number.
+        unsigned again = __ballot_sync(0xffffffffu, whole && r.valid && !fine && r.seen > 0 && r.seen < p.q.length);
+        while (again) {
+            const int i = __ffs(again) - 1;
+            again &= again - 1;
+            const int token = __shfl_sync(0xffffffffu, r.token, i), head = __shfl_sync(0xffffffffu, r.head, i);
+            __syncwarp();
+            attend_row<T, S, D>(a, p.s, p.q.first, p.q.rows, p.q.length, token, head);
+        }
+        tmem_fence_before();  // this tile's reads, before the products that the next arrival lets run
+        u += last - p.block;
+        next_pair(p, a);
+    }
+}
+
+template <typename T, int S, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    cache_chunk_kernel(const __grid_constant__ CacheAttendArgs a, const __grid_constant__ CacheMaps maps) {
+    using Layout = ChunkLayout<S, D>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Layout::bar_at);
+    const ChunkBars bar = {bars, bars + Layout::stages, bars + 2 * Layout::stages, bars + 2 * Layout::stages + 2,
+                           bars + 2 * Layout::stages + 4, bars + 2 * Layout::stages + 6, bars + 2 * Layout::stages + 8};
+    volatile int* abort = reinterpret_cast<volatile int*>(bars + Layout::bars);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + Layout::bars) + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2 * Layout::stages; ++i) cache_barrier_init(bars + i, 1);
+        for (int t = 0; t < 2; ++t) {
+            cache_barrier_init(bar.scores + t, 1);
+            cache_barrier_init(bar.p + t, kTile);
+            cache_barrier_init(bar.queries + t, kTile);
+            cache_barrier_init(bar.o + t, 1);
+        }
+        cache_barrier_init(bar.done, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(slot)),
+                     "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    const long long total = all_blocks(a, lane);
+    const long long per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
+    const long long begin = min(total, blockIdx.x * per), end = min(total, begin + per);
+    const ChunkPlace p = begin < end ? find_block(a, begin, lane) : ChunkPlace{};
+    if (threadIdx.x == 0) {
+        CutItem cut{};
+        const long long first = begin - p.block;  // the item's
+        if (begin < end && p.block > 0 && first >= begin - per)
+            cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.pair};
+        cut_items(a)[blockIdx.x] = cut;
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *slot;
+    if (begin < end) {
+        if (warp == kCopyWarp) chunk_copy<S, D>(a, maps, smem, bar, abort, p, begin, end, lane);
+        else if (warp == kMmaWarp) chunk_products<T, S, D>(a, smem, bar, tmem, abort, p, begin, end, lane);
+        else chunk_softmax<T, S, D>(a, smem, bar, tmem, abort, p, begin, end, warp >> 2);
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    if (warp == kMmaWarp)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// ------------------------------------------------------------------- launch
+
+template <typename T, int S, int D>
+void launch_chunk(const CacheAttendArgs& a, const CacheMaps& maps, int sms, cudaStream_t stream) {
+    using Layout = ChunkLayout<S, D>;
+    // As many CTAs as there can be blocks, one an SM at most.
+    const long long pairs = (long long)a.rows * a.group / kPair + a.batch.sequences;
+    const long long blocks = (((long long)a.batch.columns << a.cache.page_shift) + kBlockKeys - 1) / kBlockKeys;
+    const int grid = (int)std::min((double)sms, (double)pairs * a.cache.heads * std::max(1ll, blocks));
+    cache_chunk_kernel<T, S, D><<<grid, kChunkThreads, Layout::bytes, stream>>>(a, maps);
+    CUDA_CHECK(cudaGetLastError());
+    launch_join<T, S, D, kPair>(a, grid, stream);
+}
+
+template <typename F>
+void with_chunk_types(int storage, bool bf16, int width, F&& f) {
+    with_cache_types(storage, bf16, width, [&](auto t, auto s, auto d) {
+        if constexpr (!cache_eight(decltype(s)::value)) f(t, s, d);
+    });
+}
+
+}  // namespace
+
+bool cache_chunk_takes(int storage) { return !cache_eight(storage); }
+
+size_t cache_chunk_workspace(const CacheAttendShape& shape) { return cut_workspace(shape.sms, shape.width, kPair); }
+
+void prepare_cache_chunk(int storage, int width) {
+    for (bool bf16 : {false, true})
+        with_chunk_types(storage, bf16, width, [&](auto t, auto s, auto d) {
+            CUDA_CHECK(cudaFuncSetAttribute(cache_chunk_kernel<decltype(t), s.value, d.value>,
+                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            ChunkLayout<s.value, d.value>::bytes));
+        });
+}
+
+void launch_cache_chunk(const CacheAttendArgs& a, const CacheMaps& maps, const CacheAttendShape& shape,
+                        cudaStream_t stream) {
+    with_chunk_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
+        launch_chunk<decltype(t), s.value, d.value>(a, maps, shape.sms, stream);
+    });
+}
+
+}  // namespace wsp

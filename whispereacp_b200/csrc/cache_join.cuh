@@ -1,0 +1,154 @@
+// Items of the cache's attention that the CTAs' runs cut: what a CTA leaves of
+// them in the workspace, and the kernel that joins it.
+#pragma once
+
+#include "cache_device.cuh"
+#include "host.h"
+
+namespace wsp {
+namespace {
+
+// Workspace: a record for each CTA whose run begins inside an item, then two
+// partial results for each CTA: [0] of the item its run begins in, [1] of the
+// item its run ends in.
+struct CutItem {
+    int parts;  // partial results of the item, if this CTA's is the second; else 0
+    int sequence, head, tile;
+};
+template <int D, int kRows>
+struct Partial {
+    static constexpr int floats = kRows * (D + 2);  // o, then m, then sum
+};
+inline size_t cut_workspace(long long grid, int width, int rows) {
+    return (sizeof(CutItem) * grid + 255) / 256 * 256 + grid * 2 * rows * (width + 2) * 4;
+}
+__device__ __forceinline__ CutItem* cut_items(const CacheAttendArgs& a) { return reinterpret_cast<CutItem*>(a.workspace); }
+__device__ __forceinline__ float* cut_partials(const CacheAttendArgs& a, int grid) {
+    return reinterpret_cast<float*>(a.workspace + ((sizeof(CutItem) * grid + 255) / 256) * 256);
+}
+
+__device__ __forceinline__ long long warp_scan(long long v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
+// ----------------------------------------------------------------- the join
+
+constexpr int kJoinRows = 4;
+
+// Block (c, y) joins rows 4 y .. of the item that the border between the runs
+// of CTAs c and c + 1 cuts, if no earlier border does.  Its warps share out
+// the rows and each row's partial results.
+template <typename T, int S, int D, int kRows, int kThreads>
+__global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_constant__ CacheAttendArgs a, int grid) {
+    constexpr int kPer = D / 32;
+    constexpr int kJoinWarps = kThreads / 32;
+    __shared__ float shared_o[kJoinWarps][D];
+    __shared__ float shared_ml[kJoinWarps][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int c = blockIdx.x + 1;
+    const int4 record = *reinterpret_cast<const int4*>(cut_items(a) + c);
+    const CutItem cut = {record.x, record.y, record.z, record.w};
+    if (cut.parts == 0) return;
+    const float* partials = cut_partials(a, grid);
+    const CacheSequence q = cache_sequence(a.batch, cut.sequence);
+    const int all_rows = (int)min((long long)kRows, (long long)q.rows * a.group - (long long)cut.tile * kRows);
+    for (int first = (int)blockIdx.y * kJoinRows; first < all_rows; first += (int)gridDim.y * kJoinRows) {
+        const int rows = min(kJoinRows, all_rows - first);
+        int share = 1;  // warps of a row
+        while (share * 2 * rows <= kJoinWarps && share < cut.parts) share *= 2;
+        const int local = warp / share, sub = warp % share, row = first + local;
+        const bool active = local < rows;
+        float m = -INFINITY, sum = 0.f, o[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+        const auto add = [&](float pm, float ps, const float* v) {
+            const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
+            const float keep = exp2_fast(m - base), gain = exp2_fast(pm - base);
+            sum = sum * keep + ps * gain;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) o[e] = o[e] * keep + v[e] * gain;
+            m = top;
+        };
+        if (active) {
+            const int from = (int)((long long)cut.parts * sub / share), to = (int)((long long)cut.parts * (sub + 1) / share);
+#pragma unroll 4
+            for (int i = from; i < to; ++i) {
+                const float* part = partials + ((long long)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * Partial<D, kRows>::floats;
+                float v[kPer];
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) v[e] = part[row * D + lane * kPer + e];
+                add(part[kRows * D + row], part[kRows * (D + 1) + row], v);
+            }
+        }
+        if (share > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) shared_o[warp][lane * kPer + e] = o[e];
+            if (lane == 0) {
+                shared_ml[warp][0] = m;
+                shared_ml[warp][1] = sum;
+            }
+            __syncthreads();
+            if (sub == 0)
+                for (int w = warp + 1; w < warp + share; ++w) add(shared_ml[w][0], shared_ml[w][1], &shared_o[w][lane * kPer]);
+        }
+        if (!active || sub != 0) continue;
+        const TileRow r = tile_row(a, q, cut.head, cut.tile * kRows + row);
+        if (!r.valid) continue;
+        const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
+        const long long at = (long long)q.first + r.token;
+        unsigned char* op = a.out + at * a.o_row + r.head * a.o_head + lane * (kPer * 2);
+        bool fine = true;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+            const float x = o[e] * inverse, y = o[e + 1] * inverse;
+            fine = fine && fabsf(x) + fabsf(y) < INFINITY;
+            *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(x, y);
+        }
+        if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
+        if (__any_sync(0xffffffffu, !fine) && r.seen < q.length && r.seen > 0)
+            attend_row<T, S, D>(a, cut.sequence, q.first, q.rows, q.length, r.token, r.head);
+    }
+}
+
+template <typename T, int S, int D, int kRows>
+void launch_join(const CacheAttendArgs& a, int grid, cudaStream_t stream) {
+    if (grid == 1) return;
+    // The join's launch overlaps the end of the kernel it waits for.  Where
+    // items are far fewer than CTAs, 16 warps share a row's many parts.
+    const bool many = grid > 8ll * a.cache.heads * a.batch.sequences;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid - 1, kRows / kJoinRows);
+    config.blockDim = dim3(many ? 512 : 128);
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    CUDA_CHECK(cudaLaunchKernelEx(
+        &config, many ? cache_join_kernel<T, S, D, kRows, 512> : cache_join_kernel<T, S, D, kRows, 128>, a, grid));
+}
+
+template <typename F>
+void with_cache_types(int storage, bool bf16, int width, F&& f) {
+    const auto typed = [&](auto t, auto s) {
+        if (width == 64) f(t, s, std::integral_constant<int, 64>{});
+        else f(t, s, std::integral_constant<int, 128>{});
+    };
+    if (storage == kCacheF16) typed(__half{}, std::integral_constant<int, kCacheF16>{});
+    else if (storage == kCacheBf16) typed(__nv_bfloat16{}, std::integral_constant<int, kCacheBf16>{});
+    else if (storage == kCacheE4m3 && bf16) typed(__nv_bfloat16{}, std::integral_constant<int, kCacheE4m3>{});
+    else if (storage == kCacheE4m3) typed(__half{}, std::integral_constant<int, kCacheE4m3>{});
+    else if (bf16) typed(__nv_bfloat16{}, std::integral_constant<int, kCacheInt8>{});
+    else typed(__half{}, std::integral_constant<int, kCacheInt8>{});
+}
+
+}  // namespace
+}  // namespace wsp
