@@ -44,7 +44,7 @@ constexpr int kChunkThreads = 320;
 constexpr int kHalfBytes = kTile * 128;  // 128 rows of 64 16-bit columns
 
 enum ChunkWait : int { kWaitBlock = 11, kWaitSlot = 12, kWaitScores = 13, kWaitP = 14, kWaitQueries = 15, kWaitO = 16,
-                       kWaitDone = 17 };
+                       kWaitDone = 17, kWaitFirst = 18 };
 
 template <int S, int D>
 struct ChunkLayout {
@@ -53,8 +53,8 @@ struct ChunkLayout {
     static constexpr int stages = D == 64 ? 8 : 5;
     static constexpr int ring_at = 2 * tile_bytes;
     static constexpr int bar_at = ring_at + stages * tile_bytes;
-    // full, empty; per tile: scores, P, queries, O; done
-    static constexpr int bars = 2 * stages + 8 + 1;
+    // full, empty; per tile: scores, P's halves, first half, queries, O; done
+    static constexpr int bars = 2 * stages + 12 + 1;
     static constexpr int bytes = bar_at + bars * 8 + 16;
 };
 
@@ -73,25 +73,29 @@ __device__ __forceinline__ int chunk_pairs(const CacheSequence& q, const CacheAt
     return rows > a.few ? (int)((rows + kPair - 1) / kPair) : 0;
 }
 
-// Keys that any of the first `rows` packed rows sees.
-__device__ __forceinline__ int chunk_seen(const CacheSequence& q, const CacheAttendArgs& a, long long rows) {
+// Keys that any of the first `rows` packed rows sees; rows * group of a call
+// fit 31 bits.
+__device__ __forceinline__ int chunk_seen(const CacheSequence& q, const CacheAttendArgs& a, int rows) {
     if (!a.causal) return max(q.length, 0);
-    const int token = (int)((min(rows, (long long)q.rows * a.group) - 1) / a.group);
+    const int token = min((rows - 1) / a.group, q.rows - 1);
     return max(0, min(q.length - q.rows + token + 1, q.length));
 }
 __device__ __forceinline__ int chunk_blocks(const CacheSequence& q, const CacheAttendArgs& a, int pair) {
-    return max(1, (chunk_seen(q, a, (long long)(pair + 1) * kPair) + kBlockKeys - 1) / kBlockKeys);
+    return max(1, (chunk_seen(q, a, (pair + 1) * kPair) + kBlockKeys - 1) / kBlockKeys);
 }
+// The blocks of the first `pairs` items of one head, one lane's: whole heads'
+// items of a sequence rise from the first's blocks to the last's.
 __device__ __forceinline__ long long chunk_units(const CacheSequence& q, const CacheAttendArgs& a) {
     const int pairs = chunk_pairs(q, a);
+    if (pairs == 0) return 0;
     long long sum = 0;
-    if (!a.causal) sum = pairs ? (long long)pairs * chunk_blocks(q, a, 0) : 0;
+    if (!a.causal) sum = (long long)pairs * chunk_blocks(q, a, 0);
     else
         for (int p = 0; p < pairs; ++p) sum += chunk_blocks(q, a, p);
     return sum * a.cache.heads;
 }
 
-__device__ long long all_blocks(const CacheAttendArgs& a, int lane) {
+__device__ __forceinline__ long long all_blocks(const CacheAttendArgs& a, int lane) {
     long long sum = 0;
     for (int s = lane; s < a.batch.sequences; s += 32) sum += chunk_units(cache_sequence(a.batch, s), a);
 #pragma unroll
@@ -99,7 +103,7 @@ __device__ long long all_blocks(const CacheAttendArgs& a, int lane) {
     return sum;
 }
 
-__device__ ChunkPlace find_block(const CacheAttendArgs& a, long long u, int lane) {
+__device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long long u, int lane) {
     ChunkPlace p{};
     for (int base = 0; base < a.batch.sequences; base += 32) {
         const int s = base + lane;
@@ -119,13 +123,20 @@ __device__ ChunkPlace find_block(const CacheAttendArgs& a, long long u, int lane
             const long long head = __shfl_sync(0xffffffffu, mine, at) / a.cache.heads;  // blocks of a head
             p.head = (int)(inside / head);
             inside -= p.head * head;
-            for (;; ++p.pair) {
-                p.blocks = chunk_blocks(p.q, a, p.pair);
-                if (inside < p.blocks) break;
-                inside -= p.blocks;
+            // 32 items at a time
+            for (;; p.pair += 32) {
+                const int blocks = p.pair + lane < p.pairs ? chunk_blocks(p.q, a, p.pair + lane) : 0;
+                const long long to = warp_scan(blocks, lane);
+                const unsigned in = __ballot_sync(0xffffffffu, inside < to);
+                if (in) {
+                    const int i = __ffs(in) - 1;
+                    p.block = (int)__shfl_sync(0xffffffffu, inside - (to - blocks), i);
+                    p.blocks = __shfl_sync(0xffffffffu, blocks, i);
+                    p.pair += i;
+                    return p;
+                }
+                inside -= __shfl_sync(0xffffffffu, to, 31);
             }
-            p.block = (int)inside;
-            return p;
         }
         u -= __shfl_sync(0xffffffffu, upto, 31);
     }
@@ -150,28 +161,49 @@ __device__ __forceinline__ void next_pair(ChunkPlace& p, const CacheAttendArgs& 
 
 // The blocks of tile t of an item: 0 if it has no rows, else one at least.
 __device__ __forceinline__ int tile_blocks(const ChunkPlace& p, const CacheAttendArgs& a, int t) {
-    const long long first = (long long)p.pair * kPair + t * kTile;
-    if (first >= (long long)p.q.rows * a.group) return 0;
+    const int first = p.pair * kPair + t * kTile;
+    if (first >= p.q.rows * a.group) return 0;
     return max(1, (chunk_seen(p.q, a, first + kTile) + kBlockKeys - 1) / kBlockKeys);
 }
 
 // ------------------------------------------------------------ tensor pieces
 
-// The value tile as a product's B, MN-major: 128-byte rows of 64 columns, 8 of
-// them (keys) 1024 bytes apart from the next 8, the next 64 columns a half on.
-__device__ __forceinline__ uint64_t value_desc(uint32_t address) {
-    return (uint64_t)((address >> 4) & 0x3FFF) | ((uint64_t)(kHalfBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory descriptors as two words: the upper one is fixed, and 16-byte
+// steps in a tile add to the lower one.  Queries and keys, K-major, are
+// umma_desc's tiles.  Values as they lie are MN-major: 128-byte rows of 64
+// columns, 8 of them (keys) 1024 bytes apart from the next 8, the next 64
+// columns a half on.
+constexpr uint32_t kDescUpper = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t key_desc(uint32_t address) { return (address >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t value_desc(uint32_t address) {
+    return (address >> 4) | ((uint32_t)(kHalfBytes >> 4) << 16);
 }
 
-// D[tmem] (+)= A[tmem] . B, one thread.
-__device__ __forceinline__ void umma_mma_p(uint32_t tmem, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A . B of one k16 step, one thread: A from shared memory, or from
+// tensor memory.
+__device__ __forceinline__ void product_ss(uint32_t tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}\n" ::"r"(tmem),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescUpper)
         : "memory");
 }
+__device__ __forceinline__ void product_ts(uint32_t tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tmov.b64 y, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}\n" ::"r"(tmem),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescUpper)
+        : "memory");
+}
+// One lane of the warp, the same every time; the compiler then keeps what the
+// products take in uniform registers.
+__device__ __forceinline__ bool elected() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // 32 columns of this warp's lanes on their way into r; tmem_arrived waits for
 // every such load so far, and r may be used behind it.
@@ -214,6 +246,59 @@ __device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t (&
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// Two fp32 values of a register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 pair_values(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ float2 exp2_pair(uint64_t v) {
+    const float2 x = pair_values(v);
+    return make_float2(exp2_fast(x.x), exp2_fast(x.y));
+}
+// 2^x by arithmetic, for some of the elements, since the 16 exponentials a
+// cycle of an SM are what a softmax waits for: x = n + f with n the nearest
+// integer (adding 1.5 2^23 rounds to it and leaves it in the low bits), 2^f by
+// the polynomial of degree 4 whose largest relative error on [-1/2, 1/2] is the
+// smallest, 2^-18.5 (found by Remez's exchange), and n added to the exponent.
+// What is no number, or above 2^127, becomes 2^127 or more: the caller's check
+// of the sum finds it.
+__device__ __forceinline__ float2 exp2_computed(uint64_t v) {
+    const float2 y = pair_values(v);
+    const auto clamped = [](float z) {
+        float r;  // a NaN stays one, and its bits plus n's are a huge number's
+        asm("{\n\t.reg .f32 m;\n\tmax.NaN.f32 m, %1, 0fC2FC0000;\n\tmin.NaN.f32 %0, m, 0f42FE0000;\n\t}" : "=f"(r) : "f"(z));
+        return r;
+    };
+    const uint64_t x = pair_of(clamped(y.x), clamped(y.y));
+    const uint64_t t = add_pair(x, pair_of(12582912.f, 12582912.f));
+    const uint64_t n = add_pair(t, pair_of(-12582912.f, -12582912.f));
+    const uint64_t f = fma_pair(n, pair_of(-1.f, -1.f), x);
+    uint64_t p = fma_pair(f, pair_of(0x1.3997d6p-7f, 0x1.3997d6p-7f), pair_of(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    p = fma_pair(f, p, pair_of(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    p = fma_pair(f, p, pair_of(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    p = fma_pair(f, p, pair_of(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    const float2 a = pair_values(p), b = pair_values(t);
+    return make_float2(__uint_as_float(__float_as_uint(a.x) + (__float_as_uint(b.x) << 23)),
+                       __uint_as_float(__float_as_uint(a.y) + (__float_as_uint(b.y) << 23)));
+}
+
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -221,7 +306,7 @@ __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence
 // ---------------------------------------------------------------- the roles
 
 struct ChunkBars {
-    uint64_t *full, *empty, *scores, *p, *queries, *o, *done;
+    uint64_t *full, *empty, *scores, *p, *first, *queries, *o, *done;
 };
 
 template <int S, int D>
@@ -235,7 +320,7 @@ __device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsi
     uint32_t parity = 1;
     for (long long u = begin; u < end;) {
         const int last = (int)min((long long)p.blocks, p.block + (end - u));
-        const int seen = chunk_seen(p.q, a, (long long)(p.pair + 1) * kPair);
+        const int seen = chunk_seen(p.q, a, (p.pair + 1) * kPair);
         for (int j = p.block; j < last; ++j, ++u) {
             const int position = j * kBlockKeys + (min(lane, boxes - 1) << box_shift);
             const int row = position & ((1 << a.cache.page_shift) - 1);
@@ -275,11 +360,12 @@ __device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsi
 }
 
 template <typename T, int S, int D>
-__device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, uint32_t tmem,
+__device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, uint32_t tmem_base,
                                volatile int* abort, ChunkPlace p, long long begin, long long end, int lane) {
     using Layout = ChunkLayout<S, D>;
     const uint32_t score_desc = umma_idesc<T>(kBlockKeys), out_desc = umma_idesc<T>(D) | (1u << 16);
-    const uint32_t q_at = smem_address(smem), ring = smem_address(smem + Layout::ring_at);
+    const uint32_t tmem = (uint32_t)uniform((int)tmem_base);
+    const uint32_t queries = key_desc(smem_address(smem)), ring = smem_address(smem + Layout::ring_at);
     int stage = 0;
     uint32_t parity = 0, p_parity[2] = {0, 0}, q_parity[2] = {0, 0};
     const auto advance = [&] {
@@ -289,37 +375,38 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
         }
     };
     const auto scores = [&](int t, uint32_t keys) {
-        if (lane == 0) {
+        if (elected()) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-                const uint32_t at = (uint32_t)((k / 4) * kHalfBytes + (k % 4) * 32);
-                umma_mma(tmem + t * 128, umma_desc(q_at + t * Layout::tile_bytes + at), umma_desc(keys + at), score_desc,
-                         k != 0);
+                const uint32_t at = (uint32_t)((k / 4) * kHalfBytes + (k % 4) * 32) >> 4;
+                product_ss(tmem + t * 128, queries + ((uint32_t)(t * Layout::tile_bytes) >> 4) + at, keys + at, score_desc,
+                           k != 0);
             }
             umma_commit(bar.scores + t);
         }
         __syncwarp();
     };
-    for (long long u = begin; u < end;) {
-        const int last = (int)min((long long)p.blocks, p.block + (end - u));
-        const int blocks[2] = {min(last, tile_blocks(p, a, 0)), min(last, tile_blocks(p, a, 1))};
-        const int seen = chunk_seen(p.q, a, (long long)(p.pair + 1) * kPair);
+    for (int todo = uniform((int)(end - begin)); todo > 0;) {
+        const int first = uniform(p.block), last = uniform(min(p.blocks, p.block + todo));
+        const int blocks[2] = {uniform(min(last, tile_blocks(p, a, 0))), uniform(min(last, tile_blocks(p, a, 1)))};
+        const int seen = uniform(chunk_seen(p.q, a, (p.pair + 1) * kPair));
         // The first block's scores.
         cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
+#pragma unroll
         for (int t = 0; t < 2; ++t)
-            if (p.block < blocks[t]) {
+            if (first < blocks[t]) {
                 cache_wait(bar.queries + t, q_parity[t], abort, a.status, kWaitQueries);
                 q_parity[t] ^= 1;
                 tmem_fence_after();
-                scores(t, ring + stage * Layout::tile_bytes);
+                scores(t, key_desc(ring + stage * Layout::tile_bytes));
             }
-        if (lane == 0) umma_commit(bar.empty + stage);
+        if (elected()) umma_commit(bar.empty + stage);
         __syncwarp();
         advance();
-        for (int j = p.block; j < last; ++j, ++u) {
+        for (int j = first; j < last; ++j) {
             const int v_stage = stage;
             cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
-            const uint32_t values = ring + stage * Layout::tile_bytes;
+            const uint32_t values = value_desc(ring + stage * Layout::tile_bytes);
             if ((j + 1) * kBlockKeys > seen) {
                 // What lies behind the last row that the item sees was not
                 // copied or may be anything, and 0 times a NaN is one.
@@ -337,31 +424,37 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
                 cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
                 advance();
             }
+#pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if (j >= blocks[t]) continue;
-                cache_wait(bar.p + t, p_parity[t], abort, a.status, kWaitP);
-                p_parity[t] ^= 1;
-                tmem_fence_after();
-                if (lane == 0) {
 #pragma unroll
-                    for (int k = 0; k < kBlockKeys / 16; ++k)
-                        umma_mma_p(tmem + 256 + t * D, tmem + t * 128 + k * 8, value_desc(values + k * 2048), out_desc,
-                                   j > p.block || k != 0);
-                    if (j + 1 >= blocks[t]) umma_commit(bar.o + t);
+                for (int half = 0; half < 2; ++half) {
+                    cache_wait(bar.p + 2 * t + half, p_parity[t], abort, a.status, kWaitP);
+                    tmem_fence_after();
+                    if (elected()) {
+#pragma unroll
+                        for (int k = half * 4; k < half * 4 + 4; ++k)
+                            product_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, values + k * (2048 >> 4), out_desc,
+                                       k != 0 ? 1u : (uint32_t)(j > first));
+                        if (half == 0) umma_commit(bar.first + t);
+                        else if (j + 1 >= blocks[t]) umma_commit(bar.o + t);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (j + 1 < blocks[t]) scores(t, ring + k_stage * Layout::tile_bytes);
+                p_parity[t] ^= 1;
+                if (j + 1 < blocks[t]) scores(t, key_desc(ring + k_stage * Layout::tile_bytes));
             }
-            if (lane == 0) {
+            if (elected()) {
                 umma_commit(bar.empty + v_stage);
                 if (j + 1 < last) umma_commit(bar.empty + k_stage);
             }
             __syncwarp();
         }
+        todo -= last - first;
         next_pair(p, a);
     }
     // Every product has completed before the tensor memory goes.
-    if (lane == 0) {
+    if (elected()) {
         umma_commit(bar.done);
         const unsigned long long start = cache_clock_ns();
         while (!cache_phase_done(bar.done, 0))
@@ -377,24 +470,30 @@ template <typename T, int S, int D>
 __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, uint32_t tmem,
                               volatile int* abort, ChunkPlace p, long long begin, long long end, int t) {
     using Layout = ChunkLayout<S, D>;
-    // fp16 keeps 2^-14 .. 2^15 whole: P's largest, 2^8 by the lazy maximum, is
-    // put at 2^15.  bf16 has fp32's range.
-    constexpr float kShift = std::is_same<T, __half>::value ? 7.f : 0.f;
-    constexpr float kLimit = 8.f + kShift;
-    const int row = threadIdx.x & 127;
+    // The reference of a row's exponentials comes from the maximum of the first
+    // block it sees and stays as long as a block's sum of P says that no P left
+    // the 16-bit type's range: fp16 keeps 2^-14 .. 2^15 whole, so P starts at
+    // 2^4 at most; bf16 has fp32's range.
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr float kShift = kHalf ? 4.f : 0.f;
+    constexpr float kMost = kHalf ? 32768.f : 0x1p60f;
+    // Of 8 pairs of exponentials, those that the multipliers take.
+    constexpr int kComputed = 0;
+    const int lane = threadIdx.x & 31, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(row & ~31) << 16;
     const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * D + lanes;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // the sign goes into the queries
-    const float to_log2 = fabsf(a.scale) * kLog2e;
-    uint32_t s_parity = 0, o_parity = 0;
+    const float to_log2 = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-126f);  // a masked score of -infinity stays one at scale 0
+    uint32_t s_parity = 0, o_parity = 0, h_parity = 0;
     for (long long u = begin; u < end;) {
         const int last = (int)min((long long)p.blocks, p.block + (end - u));
         const int blocks = min(last, tile_blocks(p, a, t));
-        const long long packed = (long long)p.pair * kPair + t * kTile;
+        const int packed = p.pair * kPair + t * kTile;
         const bool active = p.block < blocks;
-        const TileRow r = tile_row(a, p.q, p.head, (int)packed + row);
+        const TileRow r = tile_row(a, p.q, p.head, packed + row);
         const long long at = (long long)p.q.first + r.token;
-        float from = 0.f, limit = -INFINITY, sum = 0.f;
+        float from = 0.f, sum = 0.f;
+        bool unset = true;  // no key seen yet
         if (active) {
             // The row's queries, swizzled as the copy engine does it.
             const unsigned char* qp = a.queries + at * a.q_row + r.head * a.q_head;
@@ -409,76 +508,109 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                                               ((c ^ (row & 7)) << 4)) = v;
                 }
             cache_proxy_fence();
-            cache_arrive(bar.queries + t);
+            __syncwarp();
+            if (lane == 0) cache_arrive(bar.queries + t);
             // Keys below `clear` are seen by every row of the tile.
-            const int clear = tile_row(a, p.q, p.head, (int)packed).seen;
+            const int clear = tile_row(a, p.q, p.head, packed).seen;
             for (int j = p.block; j < blocks; ++j) {
                 cache_wait(bar.scores + t, s_parity, abort, a.status, kWaitScores);
                 s_parity ^= 1;
                 tmem_fence_after();
-                // The scores are read twice, 32 at a time with the next 32 on
-                // their way: for the maximum, then for P, whose columns trail
-                // the scores' that were read.
-                uint32_t s[2][32];
                 const bool masked = (j + 1) * kBlockKeys > clear;
-                const int seen = r.seen - j * kBlockKeys;
+                // 32 scores at a time, the next 32 to 64 on their way.  Half a
+                // block's P goes out at a time: the products of the first 64
+                // keys' run while the second 64 are computed.
+                uint32_t s[2][32], w[2][16];
                 const auto take = [&](int c) {
                     tmem_arrived(s[c & 1]);
-                    if (c < 7) tmem_load32_begin(s_at + ((c + 1) & 3) * 32, s[(c + 1) & 1]);
-                    if (masked)
+                    if (masked) {
+                        const int seen = r.seen - j * kBlockKeys;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if ((c & 3) * 32 + e >= seen) s[c & 1][e] = 0xff800000u;
+                            if (c * 32 + e >= seen) s[c & 1][e] = 0xff800000u;
+                    }
                 };
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                tmem_load32_begin(s_at, s[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    take(c);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c & 1][e]));
-                }
-                const float higher = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * to_log2;
-                // -infinity times a scale of 0 is no number, and no maximum
-                const bool grows = higher - from > limit;
-                if (__any_sync(0xffffffffu, grows)) {
-                    float keep = 1.f;
-                    if (grows) {
-                        keep = limit == -INFINITY ? 0.f : exp2_fast(from - (higher - kShift));
-                        from = higher - kShift;
-                        limit = kLimit;
-                        sum *= keep;
-                    }
-                    if (j > p.block) {
-#pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_load32(o_at + c * 32, o);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tmem_store32(o_at + c * 32, o);
-                        }
-                    }
-                }
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 4; c < 8; ++c) {
-                    take(c);
-                    uint32_t packed16[16];
+                uint64_t sums[2];
+                const auto exponentials = [&](int c, auto computed) {
+                    const uint64_t scale2 = pair_of(to_log2, to_log2), from2 = pair_of(-from, -from);
+                    if ((c & 1) == 0) sums[0] = sums[1] = 0;
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float x = exp2_fast(fmaf(__uint_as_float(s[c & 1][e]), to_log2, -from));
-                        const float y = exp2_fast(fmaf(__uint_as_float(s[c & 1][e + 1]), to_log2, -from));
-                        part[e & 2] += x;
-                        part[(e & 2) + 1] += y;
-                        packed16[e / 2] = Half16<T>::pack2(x, y);
+                        const uint64_t x = fma_pair(
+                            pair_of(__uint_as_float(s[c & 1][e]), __uint_as_float(s[c & 1][e + 1])), scale2, from2);
+                        const float2 p = (e / 2) % 8 < decltype(computed)::value ? exp2_computed(x) : exp2_pair(x);
+                        sums[(e >> 1) & 1] = add_pair(sums[(e >> 1) & 1], pair_of(p.x, p.y));
+                        w[c & 1][e / 2] = Half16<T>::pack2(p.x, p.y);
                     }
-                    tmem_store16(s_at + (c & 3) * 16, packed16);
+                };
+                const auto half_sum = [&] {
+                    const float2 v = pair_values(add_pair(sums[0], sums[1]));
+                    return v.x + v.y;
+                };
+                tmem_load32_begin(s_at, s[0]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    // A warp whose rows all have a reference tries it.
+                    bool again = __any_sync(0xffffffffu, unset);
+                    float part = 0.f;
+                    take(2 * half);
+                    tmem_load32_begin(s_at + half * 64 + 32, s[1]);
+                    if (!again) {
+                        exponentials(2 * half, std::integral_constant<int, kComputed>{});
+                        take(2 * half + 1);
+                        if (half == 0) tmem_load32_begin(s_at + 64, s[0]);
+                        exponentials(2 * half + 1, std::integral_constant<int, kComputed>{});
+                        part = half_sum();
+                        again = __any_sync(0xffffffffu, !(part <= kMost));
+                    }
+                    if (again) {
+                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int c = 2 * half; c < 2 * half + 2; ++c) {
+                            tmem_arrived(s[c & 1]);  // whatever is on its way
+                            tmem_load32_begin(s_at + c * 32, s[c & 1]);
+                            take(c);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c & 1][e]));
+                        }
+                        const float higher = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * to_log2 - kShift;
+                        float keep = 1.f;
+                        if (higher > (unset ? -INFINITY : from)) {
+                            keep = unset ? 0.f : exp2_fast(from - higher);
+                            from = higher;
+                            unset = false;
+                            sum *= keep;
+                        }
+                        if ((j > p.block || half) && __any_sync(0xffffffffu, keep != 1.f)) {
+                            // The products behind these scores are done; those
+                            // of the first half's P have a barrier.
+                            if (half) {
+                                cache_wait(bar.first + t, h_parity, abort, a.status, kWaitFirst);
+                                tmem_fence_after();
+                            }
+#pragma unroll
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_load32(o_at + c * 32, o);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                                tmem_store32(o_at + c * 32, o);
+                            }
+                        }
+                        exponentials(2 * half, std::integral_constant<int, 0>{});
+                        exponentials(2 * half + 1, std::integral_constant<int, 0>{});
+                        part = half_sum();
+                        if (half == 0) tmem_load32_begin(s_at + 64, s[0]);
+                    }
+                    sum += part;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) tmem_store16(s_at + half * 32 + c * 16, w[c]);
+                    tmem_store_wait();
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) cache_arrive(bar.p + 2 * t + half);
                 }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                tmem_store_wait();
-                tmem_fence_before();
-                cache_arrive(bar.p + t);
+                h_parity ^= 1;
             }
             cache_wait(bar.o + t, o_parity, abort, a.status, kWaitO);
             o_parity ^= 1;
@@ -486,7 +618,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         }
         const bool whole = p.block == 0 && last == p.blocks;
         const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
-        const float log_sum = limit == -INFINITY ? -INFINITY : from;
+        const float log_sum = unset ? -INFINITY : from;
         float* part = cut_partials(a, gridDim.x) + ((long long)blockIdx.x * 2 + (p.block > 0 ? 0 : 1)) * Partial<D, kPair>::floats;
         bool fine = true;
         unsigned char* op = a.out + at * a.o_row + r.head * a.o_head;
@@ -546,7 +678,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Layout::bar_at);
     const ChunkBars bar = {bars, bars + Layout::stages, bars + 2 * Layout::stages, bars + 2 * Layout::stages + 2,
-                           bars + 2 * Layout::stages + 4, bars + 2 * Layout::stages + 6, bars + 2 * Layout::stages + 8};
+                           bars + 2 * Layout::stages + 6, bars + 2 * Layout::stages + 8, bars + 2 * Layout::stages + 10,
+                           bars + 2 * Layout::stages + 12};
     volatile int* abort = reinterpret_cast<volatile int*>(bars + Layout::bars);
     uint32_t* slot = reinterpret_cast<uint32_t*>(bars + Layout::bars) + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -554,8 +687,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (int i = 0; i < 2 * Layout::stages; ++i) cache_barrier_init(bars + i, 1);
         for (int t = 0; t < 2; ++t) {
             cache_barrier_init(bar.scores + t, 1);
-            cache_barrier_init(bar.p + t, kTile);
-            cache_barrier_init(bar.queries + t, kTile);
+            cache_barrier_init(bar.p + 2 * t, kTile / 32);
+            cache_barrier_init(bar.p + 2 * t + 1, kTile / 32);
+            cache_barrier_init(bar.first + t, 1);
+            cache_barrier_init(bar.queries + t, kTile / 32);
             cache_barrier_init(bar.o + t, 1);
         }
         cache_barrier_init(bar.done, 1);

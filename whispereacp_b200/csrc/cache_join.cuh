@@ -5,6 +5,8 @@
 #include "cache_device.cuh"
 #include "host.h"
 
+#include <algorithm>
+
 namespace wsp {
 namespace {
 
@@ -122,7 +124,8 @@ void launch_join(const CacheAttendArgs& a, int grid, cudaStream_t stream) {
     if (grid == 1) return;
     // The join's launch overlaps the end of the kernel it waits for.  Where
     // items are far fewer than CTAs, 16 warps share a row's many parts.
-    const bool many = grid > 8ll * a.cache.heads * a.batch.sequences;
+    const long long items = std::max((long long)a.batch.sequences, (long long)a.rows * a.group / kRows) * a.cache.heads;
+    const bool many = grid > 8 * items;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(grid - 1, kRows / kJoinRows);
     config.blockDim = dim3(many ? 512 : 128);
