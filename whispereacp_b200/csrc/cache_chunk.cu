@@ -493,7 +493,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         const TileRow r = tile_row(a, p.q, p.head, packed + row);
         const long long at = (long long)p.q.first + r.token;
         float from = 0.f, sum = 0.f;
-        bool unset = true;  // no key seen yet
+        bool unset = true, ready = false;  // no key seen yet; every row of the warp has seen one
         if (active) {
             // The row's queries, swizzled as the copy engine does it.
             const unsigned char* qp = a.queries + at * a.q_row + r.head * a.q_head;
@@ -517,10 +517,13 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                 s_parity ^= 1;
                 tmem_fence_after();
                 const bool masked = (j + 1) * kBlockKeys > clear;
-                // 32 scores at a time, the next 32 to 64 on their way.  Half a
-                // block's P goes out at a time: the products of the first 64
-                // keys' run while the second 64 are computed.
+                // 32 scores at a time, the next 32 on their way.  Half a block's
+                // P goes out at a time, so that the products of the first 64
+                // keys' run while the second 64 are computed; its check, its
+                // store and the store's wait each stand behind later work.
                 uint32_t s[2][32], w[2][16];
+                float part[2];
+                uint64_t sums[2];
                 const auto take = [&](int c) {
                     tmem_arrived(s[c & 1]);
                     if (masked) {
@@ -530,7 +533,6 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                             if (c * 32 + e >= seen) s[c & 1][e] = 0xff800000u;
                     }
                 };
-                uint64_t sums[2];
                 const auto exponentials = [&](int c, auto computed) {
                     const uint64_t scale2 = pair_of(to_log2, to_log2), from2 = pair_of(-from, -from);
                     if ((c & 1) == 0) sums[0] = sums[1] = 0;
@@ -542,74 +544,88 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                         sums[(e >> 1) & 1] = add_pair(sums[(e >> 1) & 1], pair_of(p.x, p.y));
                         w[c & 1][e / 2] = Half16<T>::pack2(p.x, p.y);
                     }
-                };
-                const auto half_sum = [&] {
-                    const float2 v = pair_values(add_pair(sums[0], sums[1]));
-                    return v.x + v.y;
-                };
-                tmem_load32_begin(s_at, s[0]);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    // A warp whose rows all have a reference tries it.
-                    bool again = __any_sync(0xffffffffu, unset);
-                    float part = 0.f;
-                    take(2 * half);
-                    tmem_load32_begin(s_at + half * 64 + 32, s[1]);
-                    if (!again) {
-                        exponentials(2 * half, std::integral_constant<int, kComputed>{});
-                        take(2 * half + 1);
-                        if (half == 0) tmem_load32_begin(s_at + 64, s[0]);
-                        exponentials(2 * half + 1, std::integral_constant<int, kComputed>{});
-                        part = half_sum();
-                        again = __any_sync(0xffffffffu, !(part <= kMost));
+                    if (c & 1) {
+                        const float2 v = pair_values(add_pair(sums[0], sums[1]));
+                        part[c >> 1] = v.x + v.y;
                     }
-                    if (again) {
-                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                };
+                // The half's rows get a reference from their maximum, and what
+                // stands in o follows it.
+                const auto refer = [&](int half) {
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int c = 2 * half; c < 2 * half + 2; ++c) {
-                            tmem_arrived(s[c & 1]);  // whatever is on its way
-                            tmem_load32_begin(s_at + c * 32, s[c & 1]);
-                            take(c);
+                    for (int c = 2 * half; c < 2 * half + 2; ++c) {
+                        tmem_arrived(s[c & 1]);  // whatever is on its way
+                        tmem_load32_begin(s_at + c * 32, s[c & 1]);
+                        take(c);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c & 1][e]));
-                        }
-                        const float higher = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * to_log2 - kShift;
-                        float keep = 1.f;
-                        if (higher > (unset ? -INFINITY : from)) {
-                            keep = unset ? 0.f : exp2_fast(from - higher);
-                            from = higher;
-                            unset = false;
-                            sum *= keep;
-                        }
-                        if ((j > p.block || half) && __any_sync(0xffffffffu, keep != 1.f)) {
-                            // The products behind these scores are done; those
-                            // of the first half's P have a barrier.
-                            if (half) {
-                                cache_wait(bar.first + t, h_parity, abort, a.status, kWaitFirst);
-                                tmem_fence_after();
-                            }
-#pragma unroll
-                            for (int c = 0; c < D / 32; ++c) {
-                                uint32_t o[32];
-                                tmem_load32(o_at + c * 32, o);
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                                tmem_store32(o_at + c * 32, o);
-                            }
-                        }
-                        exponentials(2 * half, std::integral_constant<int, 0>{});
-                        exponentials(2 * half + 1, std::integral_constant<int, 0>{});
-                        part = half_sum();
-                        if (half == 0) tmem_load32_begin(s_at + 64, s[0]);
+                        for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c & 1][e]));
                     }
-                    sum += part;
+                    const float higher = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * to_log2 - kShift;
+                    float keep = 1.f;
+                    if (higher > (unset ? -INFINITY : from)) {
+                        keep = unset ? 0.f : exp2_fast(from - higher);
+                        from = higher;
+                        unset = false;
+                        sum *= keep;
+                    }
+                    ready = !__any_sync(0xffffffffu, unset);
+                    if ((j > p.block || half) && __any_sync(0xffffffffu, keep != 1.f)) {
+                        // The products behind these scores are done; those of
+                        // the first half's P have a barrier.
+                        if (half) {
+                            cache_wait(bar.first + t, h_parity, abort, a.status, kWaitFirst);
+                            tmem_fence_after();
+                        }
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) tmem_store16(s_at + half * 32 + c * 16, w[c]);
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_load32(o_at + c * 32, o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_store32(o_at + c * 32, o);
+                        }
+                    }
+                    exponentials(2 * half, std::integral_constant<int, 0>{});
+                    exponentials(2 * half + 1, std::integral_constant<int, 0>{});
+                };
+                const auto store = [&](int half) {
+                    sum += part[half];
+                    tmem_store16(s_at + half * 32, w[0]);
+                    tmem_store16(s_at + half * 32 + 16, w[1]);
+                };
+                const auto hand_over = [&](int half) {
                     tmem_store_wait();
                     tmem_fence_before();
                     __syncwarp();
                     if (lane == 0) cache_arrive(bar.p + 2 * t + half);
+                };
+                const std::integral_constant<int, kComputed> computed;
+                tmem_load32_begin(s_at, s[0]);
+                take(0);
+                tmem_load32_begin(s_at + 32, s[1]);
+                if (ready) {
+                    exponentials(0, computed);
+                    take(1);
+                    tmem_load32_begin(s_at + 64, s[0]);
+                    exponentials(1, computed);
+                } else {
+                    part[0] = INFINITY;
                 }
+                if (__any_sync(0xffffffffu, !(part[0] <= kMost))) {
+                    refer(0);
+                    tmem_load32_begin(s_at + 64, s[0]);
+                }
+                store(0);
+                take(2);
+                tmem_load32_begin(s_at + 96, s[1]);
+                exponentials(2, computed);
+                hand_over(0);
+                take(3);
+                exponentials(3, computed);
+                if (__any_sync(0xffffffffu, !(part[1] <= kMost))) refer(1);
+                store(1);
+                hand_over(1);
                 h_parity ^= 1;
             }
             cache_wait(bar.o + t, o_parity, abort, a.status, kWaitO);
