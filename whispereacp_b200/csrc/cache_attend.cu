@@ -257,6 +257,10 @@ __device__ __forceinline__ float narrow_queries(uint32_t (&qf)[D / 16][2]) {
     return fine ? __uint_as_float((uint32_t)(e - 8) << 23) : 1.f;  // 2^(e - 135)
 }
 
+// A grid that was launched behind another, whose results it does not read,
+// ends behind it all the same: who waits for this one waits for both.
+__device__ __forceinline__ void ends_behind() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The producer warp: every unit of the run into the ring.
 template <int S, int D, int NT>
 __device__ __forceinline__ void token_producer(const CacheAttendArgs& a, const CacheMaps& maps, unsigned char* smem,
@@ -373,17 +377,21 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         const long long first = begin - p.unit;  // the item's
         if (begin < end && p.unit > 0 && first >= begin - per)
             cut = {(int)((first + p.units - 1) / per - blockIdx.x) + 2, p.s, p.head, p.tile};
-        cut_items(a)[blockIdx.x] = cut;
+        cut_items(a.workspace)[blockIdx.x] = cut;
     }
     __syncthreads();
-    if (begin >= end) return;
+    if (begin >= end) {
+        ends_behind();
+        return;
+    }
     if (warp == kWorkers) {
         token_producer<S, D, NT>(a, maps, smem, full, empty, abort, p, begin, end, lane);
+        ends_behind();
         return;
     }
 
     // ----------------------------------------------------------- consumers
-    float* partials = cut_partials(a, gridDim.x);
+    float* partials = cut_partials(a.workspace, gridDim.x);
     const int g = lane >> 2, t4 = lane & 3;
     float* join = reinterpret_cast<float*>(smem + Layout::join_at);
     float* ml = reinterpret_cast<float*>(smem + Layout::ml_at);
@@ -687,7 +695,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const bool whole = p.unit == 0 && last == p.units;
         constexpr int kRowThreads = D / 2;  // a thread two columns of a row
-        float* part = partials + ((long long)blockIdx.x * 2 + (p.unit > 0 ? 0 : 1)) * Partial<D, kRows>::floats;
+        float* part = partials + ((long long)blockIdx.x * 2 + (p.unit > 0 ? 0 : 1)) * partial_floats<D>(kRows);
         for (int row = threadIdx.x / kRowThreads; row < valid; row += 128 / kRowThreads) {
             const int d = (threadIdx.x % kRowThreads) * 2;
             float top = -INFINITY, all = 0.f;
@@ -740,6 +748,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) qf[j][k][0] = qn[j][k][0], qf[j][k][1] = qn[j][k][1];
     }
+    ends_behind();
 }
 
 // ------------------------------------------------------------------- launch
@@ -754,12 +763,21 @@ long long token_grid(const CacheAttendArgs& a, int sms) {
 }
 
 template <typename T, int S, int D, int NT>
-void launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, cudaStream_t stream) {
+CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, bool behind, cudaStream_t stream) {
     using Layout = TokenLayout<S, D, NT>;
     const int grid = (int)token_grid<Layout>(a, sms);
-    cache_tokens_kernel<T, S, D, NT><<<grid, kTokenThreads, Layout::bytes, stream>>>(a, maps);
-    CUDA_CHECK(cudaGetLastError());
-    launch_join<T, S, D, Layout::rows>(a, grid, stream);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(kTokenThreads);
+    config.dynamicSmemBytes = Layout::bytes;
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = behind ? 1 : 0;
+    CUDA_CHECK(cudaLaunchKernelEx(&config, cache_tokens_kernel<T, S, D, NT>, a, maps));
+    return {a.workspace, grid, Layout::rows};
 }
 
 }  // namespace
@@ -768,12 +786,14 @@ void launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, cud
 // its larger tiles.
 constexpr int kFewRows = 16;
 
+static size_t token_workspace(const CacheAttendShape& shape) {
+    // 3 CTAs of 8-row tiles, or 2 of 16-row tiles
+    return std::max(cut_workspace(shape.sms * 3, shape.width, 8), cut_workspace(shape.sms * 2, shape.width, 16));
+}
+
 size_t cache_attend_workspace(const CacheAttendShape& shape, int group) {
-    // 3 CTAs of 8-row tiles, or 2 of 16-row tiles; the kernels of a call, one
-    // after the other, share it
-    const size_t few = std::max(cut_workspace(shape.sms * 3, shape.width, 8), cut_workspace(shape.sms * 2, shape.width, 16));
-    const bool chunks = cache_chunk_takes(shape.storage) && (long long)shape.max_rows * group > kFewRows;
-    return chunks ? std::max(few, cache_chunk_workspace(shape)) : few;
+    const bool chunks = (long long)shape.max_rows * group > kFewRows;
+    return token_workspace(shape) + (chunks ? cache_chunk_workspace(shape) : 0);
 }
 
 void prepare_cache_attend(int storage, int width) {
@@ -794,14 +814,22 @@ void launch_cache_attend(const CacheAttendArgs& args, const CacheMaps& maps, con
     CacheAttendArgs a = args;
     const long long most = (long long)shape.max_rows * a.group;
     a.few = 0x7fffffffffffll;
-    if (most > kFewRows && cache_chunk_takes(shape.storage)) {
+    CutPart chunks{};
+    if (most > kFewRows) {
+        // Sequences of many rows first; the others' kernel fills the SMs as
+        // these leave them, and ends behind them.
         a.few = kFewRows;
-        launch_cache_chunk(a, maps, shape, stream);
+        CacheAttendArgs b = a;
+        b.workspace += token_workspace(shape);
+        chunks = launch_cache_chunk(b, maps, shape, stream);
     }
     // Tiles of 8 rows where every sequence's rows of a head fit one.
     with_cache_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
-        if (most <= 8) launch_tokens<decltype(t), s.value, d.value, 1>(a, maps, shape.sms, stream);
-        else launch_tokens<decltype(t), s.value, d.value, 2>(a, maps, shape.sms, stream);
+        using T = decltype(t);
+        constexpr int S = s.value, D = d.value;
+        const CutPart tokens = most <= 8 ? launch_tokens<T, S, D, 1>(a, maps, shape.sms, most > kFewRows, stream)
+                                         : launch_tokens<T, S, D, 2>(a, maps, shape.sms, most > kFewRows, stream);
+        launch_join<T, S, D>(a, tokens, chunks, stream);
     });
 }
 

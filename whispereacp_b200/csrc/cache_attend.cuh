@@ -40,13 +40,22 @@ struct CacheAttendShape {
     int width, max_rows, sms;
 };
 
+// What a kernel leaves to be joined: its workspace, its CTAs, and the rows of
+// its items.  The join takes a slice of an item's rows a block.
+constexpr int kJoinRows = 4, kJoinSlice = 16;
+struct CutPart {
+    unsigned char* workspace;
+    int grid, rows;
+    __host__ __device__ int slices() const { return (rows + kJoinSlice - 1) / kJoinSlice; }
+    __host__ __device__ int blocks() const { return grid > 1 ? (grid - 1) * slices() : 0; }
+};
+
 // The kernel of many rows (cache_chunk.cu): sequences of more than `few` rows
 // of a key head.
 void prepare_cache_chunk(int storage, int width);
-void launch_cache_chunk(const CacheAttendArgs& args, const CacheMaps& maps, const CacheAttendShape& shape,
-                        cudaStream_t stream);
+CutPart launch_cache_chunk(const CacheAttendArgs& args, const CacheMaps& maps, const CacheAttendShape& shape,
+                           cudaStream_t stream);
 size_t cache_chunk_workspace(const CacheAttendShape& shape);
-bool cache_chunk_takes(int storage);
 
 // Raises the kernels' limits of shared memory on the current device.
 void prepare_cache_attend(int storage, int width);

@@ -36,11 +36,7 @@ namespace wsp {
 namespace {
 
 constexpr int kBlockKeys = 128;
-constexpr int kTile = 128;          // rows of a tile
-constexpr int kPair = 2 * kTile;    // rows of an item
-constexpr int kMmaWarp = 8;
-constexpr int kCopyWarp = 9;
-constexpr int kChunkThreads = 320;
+constexpr int kTile = 128;               // rows of a tile
 constexpr int kHalfBytes = kTile * 128;  // 128 rows of 64 16-bit columns
 
 enum ChunkWait : int { kWaitBlock = 11, kWaitSlot = 12, kWaitScores = 13, kWaitP = 14, kWaitQueries = 15, kWaitO = 16,
@@ -48,13 +44,23 @@ enum ChunkWait : int { kWaitBlock = 11, kWaitSlot = 12, kWaitScores = 13, kWaitP
 
 template <int S, int D>
 struct ChunkLayout {
+    // Tiles of a CTA.  16-bit 64-wide heads: one, and two CTAs an SM, each at a
+    // point of its own (their smaller blocks may cross from L2 twice).
+    static constexpr int tiles = D == 64 && !cache_eight(S) ? 1 : 2;
+    static constexpr int ctas = 3 - tiles;
+    static constexpr int rows = tiles * kTile;  // of an item
+    static constexpr int mma_warp = 4 * tiles;
+    static constexpr int copy_warps = cache_eight(S) ? 3 : 1;
+    static constexpr int threads = 32 * (mma_warp + 1 + copy_warps);
+    static constexpr int columns = tiles == 1 ? 256 : 512;  // of tensor memory
+    static constexpr int out_column = tiles * 128;
     static constexpr int halves = D / 64;
     static constexpr int tile_bytes = halves * kHalfBytes;  // of Q_t, or of a block's keys or values
-    static constexpr int stages = D == 64 ? 8 : 5;
-    static constexpr int ring_at = 2 * tile_bytes;
+    static constexpr int stages = D == 64 && tiles == 2 ? 8 : 5;
+    static constexpr int ring_at = tiles * tile_bytes;
     static constexpr int bar_at = ring_at + stages * tile_bytes;
     // full, empty; per tile: scores, P's halves, first half, queries, O; done
-    static constexpr int bars = 2 * stages + 12 + 1;
+    static constexpr int bars = 2 * stages + 6 * tiles + 1;
     static constexpr int bytes = bar_at + bars * 8 + 16;
 };
 
@@ -63,14 +69,15 @@ struct ChunkLayout {
 struct ChunkPlace {
     int s;
     CacheSequence q;
-    int head, pair;
+    int head, item;
     int block, blocks;  // the item's first in this run; its blocks
-    int pairs;
+    int items;          // of a head
 };
 
-__device__ __forceinline__ int chunk_pairs(const CacheSequence& q, const CacheAttendArgs& a) {
+template <int kRows>
+__device__ __forceinline__ int chunk_items(const CacheSequence& q, const CacheAttendArgs& a) {
     const long long rows = (long long)q.rows * a.group;
-    return rows > a.few ? (int)((rows + kPair - 1) / kPair) : 0;
+    return rows > a.few ? (int)((rows + kRows - 1) / kRows) : 0;
 }
 
 // Keys that any of the first `rows` packed rows sees; rows * group of a call
@@ -80,36 +87,39 @@ __device__ __forceinline__ int chunk_seen(const CacheSequence& q, const CacheAtt
     const int token = min((rows - 1) / a.group, q.rows - 1);
     return max(0, min(q.length - q.rows + token + 1, q.length));
 }
-__device__ __forceinline__ int chunk_blocks(const CacheSequence& q, const CacheAttendArgs& a, int pair) {
-    return max(1, (chunk_seen(q, a, (pair + 1) * kPair) + kBlockKeys - 1) / kBlockKeys);
+template <int kRows>
+__device__ __forceinline__ int chunk_blocks(const CacheSequence& q, const CacheAttendArgs& a, int item) {
+    return max(1, (chunk_seen(q, a, (item + 1) * kRows) + kBlockKeys - 1) / kBlockKeys);
 }
-// The blocks of the first `pairs` items of one head, one lane's: whole heads'
-// items of a sequence rise from the first's blocks to the last's.
+// A sequence's blocks.
+template <int kRows>
 __device__ __forceinline__ long long chunk_units(const CacheSequence& q, const CacheAttendArgs& a) {
-    const int pairs = chunk_pairs(q, a);
-    if (pairs == 0) return 0;
+    const int items = chunk_items<kRows>(q, a);
+    if (items == 0) return 0;
     long long sum = 0;
-    if (!a.causal) sum = (long long)pairs * chunk_blocks(q, a, 0);
+    if (!a.causal) sum = (long long)items * chunk_blocks<kRows>(q, a, 0);
     else
-        for (int p = 0; p < pairs; ++p) sum += chunk_blocks(q, a, p);
+        for (int p = 0; p < items; ++p) sum += chunk_blocks<kRows>(q, a, p);
     return sum * a.cache.heads;
 }
 
+template <int kRows>
 __device__ __forceinline__ long long all_blocks(const CacheAttendArgs& a, int lane) {
     long long sum = 0;
-    for (int s = lane; s < a.batch.sequences; s += 32) sum += chunk_units(cache_sequence(a.batch, s), a);
+    for (int s = lane; s < a.batch.sequences; s += 32) sum += chunk_units<kRows>(cache_sequence(a.batch, s), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
 
+template <int kRows>
 __device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long long u, int lane) {
     ChunkPlace p{};
     for (int base = 0; base < a.batch.sequences; base += 32) {
         const int s = base + lane;
         CacheSequence q{};
         if (s < a.batch.sequences) q = cache_sequence(a.batch, s);
-        const long long mine = s < a.batch.sequences ? chunk_units(q, a) : 0;
+        const long long mine = s < a.batch.sequences ? chunk_units<kRows>(q, a) : 0;
         const long long upto = warp_scan(mine, lane);
         const unsigned holds = __ballot_sync(0xffffffffu, u < upto);
         if (holds) {
@@ -119,20 +129,20 @@ __device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long 
             p.q.first = __shfl_sync(0xffffffffu, q.first, at);
             p.q.rows = __shfl_sync(0xffffffffu, q.rows, at);
             p.q.length = __shfl_sync(0xffffffffu, q.length, at);
-            p.pairs = chunk_pairs(p.q, a);
+            p.items = chunk_items<kRows>(p.q, a);
             const long long head = __shfl_sync(0xffffffffu, mine, at) / a.cache.heads;  // blocks of a head
             p.head = (int)(inside / head);
             inside -= p.head * head;
             // 32 items at a time
-            for (;; p.pair += 32) {
-                const int blocks = p.pair + lane < p.pairs ? chunk_blocks(p.q, a, p.pair + lane) : 0;
+            for (;; p.item += 32) {
+                const int blocks = p.item + lane < p.items ? chunk_blocks<kRows>(p.q, a, p.item + lane) : 0;
                 const long long to = warp_scan(blocks, lane);
                 const unsigned in = __ballot_sync(0xffffffffu, inside < to);
                 if (in) {
                     const int i = __ffs(in) - 1;
                     p.block = (int)__shfl_sync(0xffffffffu, inside - (to - blocks), i);
                     p.blocks = __shfl_sync(0xffffffffu, blocks, i);
-                    p.pair += i;
+                    p.item += i;
                     return p;
                 }
                 inside -= __shfl_sync(0xffffffffu, to, 31);
@@ -143,25 +153,27 @@ __device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long 
     return p;
 }
 
-__device__ __forceinline__ void next_pair(ChunkPlace& p, const CacheAttendArgs& a) {
+template <int kRows>
+__device__ __forceinline__ void next_item(ChunkPlace& p, const CacheAttendArgs& a) {
     p.block = 0;
-    if (++p.pair >= p.pairs) {
-        p.pair = 0;
+    if (++p.item >= p.items) {
+        p.item = 0;
         if (++p.head >= a.cache.heads) {
             p.head = 0;
             while (++p.s < a.batch.sequences) {
                 p.q = cache_sequence(a.batch, p.s);
-                p.pairs = chunk_pairs(p.q, a);
-                if (p.pairs > 0) break;
+                p.items = chunk_items<kRows>(p.q, a);
+                if (p.items > 0) break;
             }
         }
     }
-    p.blocks = chunk_blocks(p.q, a, p.pair);
+    p.blocks = chunk_blocks<kRows>(p.q, a, p.item);
 }
 
 // The blocks of tile t of an item: 0 if it has no rows, else one at least.
+template <int kRows>
 __device__ __forceinline__ int tile_blocks(const ChunkPlace& p, const CacheAttendArgs& a, int t) {
-    const int first = p.pair * kPair + t * kTile;
+    const int first = p.item * kRows + t * kTile;
     if (first >= p.q.rows * a.group) return 0;
     return max(1, (chunk_seen(p.q, a, first + kTile) + kBlockKeys - 1) / kBlockKeys);
 }
@@ -320,7 +332,7 @@ __device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsi
     uint32_t parity = 1;
     for (long long u = begin; u < end;) {
         const int last = (int)min((long long)p.blocks, p.block + (end - u));
-        const int seen = chunk_seen(p.q, a, (p.pair + 1) * kPair);
+        const int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
         for (int j = p.block; j < last; ++j, ++u) {
             const int position = j * kBlockKeys + (min(lane, boxes - 1) << box_shift);
             const int row = position & ((1 << a.cache.page_shift) - 1);
@@ -348,7 +360,7 @@ __device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsi
             if (*abort) break;
         }
         if (*abort) break;
-        next_pair(p, a);
+        next_item<Layout::rows>(p, a);
     }
     if (*abort)  // the copies in flight land before the CTA's memory is given up
         for (int i = max(0, n - Layout::stages); i < n; ++i) {
@@ -357,6 +369,80 @@ __device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsi
                    cache_clock_ns() - start < kCacheTimeoutNs) {
             }
         }
+}
+
+// 8-bit caches: three warps read the blocks themselves and write them widened
+// to the queries' type, each value times its scale (a power of two: exact in
+// bf16, and in fp16 wherever fp16 holds the result).
+template <typename T, int S, int D>
+__device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, volatile int* abort,
+                            ChunkPlace p, long long begin, long long end, int warp, int lane) {
+    using Layout = ChunkLayout<S, D>;
+    constexpr int kThreads = 32 * Layout::copy_warps;
+    constexpr int kPieces = kBlockKeys * D / 16;  // 16 values each
+    constexpr int kMine = (kPieces + kThreads - 1) / kThreads;
+    const int me = warp * 32 + lane;
+    int stage = 0, n = 0;
+    uint32_t parity = 1;
+    for (int todo = (int)(end - begin); todo > 0;) {
+        const int last = min(p.blocks, p.block + todo);
+        const int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
+        for (int j = p.block; j < last; ++j) {
+            // A lane a page, of 16 rows at least.
+            const int pages = max(1, kBlockKeys >> a.cache.page_shift);
+            const int first = j * kBlockKeys + (min(lane, pages - 1) << a.cache.page_shift);
+            const int entry = first < seen ? cache_page(a.cache, a.batch, p.s, first) : -1;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const unsigned char* pool = v ? a.cache.values : a.cache.keys;
+                const uint8_t* scales = v ? a.cache.value_scales : a.cache.key_scales;
+                uint4 raw[kMine];
+                uint32_t scale[kMine];
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
+                    const int position = j * kBlockKeys + key;
+                    const int page = __shfl_sync(0xffffffffu, entry, min(key >> a.cache.page_shift, pages - 1));
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    scale[i] = 0;
+                    if (piece < kPieces && position < seen && page >= 0) {
+                        const int slot = position & ((1 << a.cache.page_shift) - 1);
+                        raw[i] = load_stream(pool + cache_offset(a.cache, page, p.head, slot) + c * 16);
+                        scale[i] = __ldg(scales + cache_scale_index(a.cache, page, p.head, slot));
+                    }
+                }
+                if (n >= Layout::stages) cache_wait(bar.empty + stage, parity, abort, a.status, kWaitSlot);
+                unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
+                    if (piece >= kPieces) break;
+                    const float by = cache_scale(scale[i]);
+                    const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    uint32_t out[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 f = cache_pair<S>((in[e / 2] >> (16 * (e & 1))) & 0xffffu);
+                        out[e] = Half16<T>::pack2(f.x * by, f.y * by);
+                    }
+                    unsigned char* to = tile + (c / 4) * kHalfBytes + key * 128;
+                    const int at = (c % 4) * 2;
+                    *reinterpret_cast<uint4*>(to + ((at ^ (key & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+                    *reinterpret_cast<uint4*>(to + (((at + 1) ^ (key & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+                }
+                cache_proxy_fence();
+                __syncwarp();
+                if (lane == 0) cache_arrive(bar.full + stage);
+                ++n;
+                if (++stage == Layout::stages) {
+                    stage = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+        todo -= last - p.block;
+        next_item<Layout::rows>(p, a);
+    }
 }
 
 template <typename T, int S, int D>
@@ -388,12 +474,14 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
     };
     for (int todo = uniform((int)(end - begin)); todo > 0;) {
         const int first = uniform(p.block), last = uniform(min(p.blocks, p.block + todo));
-        const int blocks[2] = {uniform(min(last, tile_blocks(p, a, 0))), uniform(min(last, tile_blocks(p, a, 1)))};
-        const int seen = uniform(chunk_seen(p.q, a, (p.pair + 1) * kPair));
+        int blocks[Layout::tiles];
+#pragma unroll
+        for (int t = 0; t < Layout::tiles; ++t) blocks[t] = uniform(min(last, tile_blocks<Layout::rows>(p, a, t)));
+        const int seen = uniform(chunk_seen(p.q, a, (p.item + 1) * Layout::rows));
         // The first block's scores.
         cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < Layout::tiles; ++t)
             if (first < blocks[t]) {
                 cache_wait(bar.queries + t, q_parity[t], abort, a.status, kWaitQueries);
                 q_parity[t] ^= 1;
@@ -407,7 +495,7 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
             const int v_stage = stage;
             cache_wait(bar.full + stage, parity, abort, a.status, kWaitBlock);
             const uint32_t values = value_desc(ring + stage * Layout::tile_bytes);
-            if ((j + 1) * kBlockKeys > seen) {
+            if (!cache_eight(S) && (j + 1) * kBlockKeys > seen) {
                 // What lies behind the last row that the item sees was not
                 // copied or may be anything, and 0 times a NaN is one.
                 unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
@@ -425,7 +513,7 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
                 advance();
             }
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < Layout::tiles; ++t) {
                 if (j >= blocks[t]) continue;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -434,7 +522,7 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
                     if (elected()) {
 #pragma unroll
                         for (int k = half * 4; k < half * 4 + 4; ++k)
-                            product_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, values + k * (2048 >> 4), out_desc,
+                            product_ts(tmem + Layout::out_column + t * D, tmem + t * 128 + k * 8, values + k * (2048 >> 4), out_desc,
                                        k != 0 ? 1u : (uint32_t)(j > first));
                         if (half == 0) umma_commit(bar.first + t);
                         else if (j + 1 >= blocks[t]) umma_commit(bar.o + t);
@@ -451,7 +539,7 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
             __syncwarp();
         }
         todo -= last - first;
-        next_pair(p, a);
+        next_item<Layout::rows>(p, a);
     }
     // Every product has completed before the tensor memory goes.
     if (elected()) {
@@ -481,35 +569,44 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
     constexpr int kComputed = 0;
     const int lane = threadIdx.x & 31, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(row & ~31) << 16;
-    const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * D + lanes;
+    const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + Layout::out_column + t * D + lanes;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // the sign goes into the queries
     const float to_log2 = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-126f);  // a masked score of -infinity stays one at scale 0
     uint32_t s_parity = 0, o_parity = 0, h_parity = 0;
-    for (long long u = begin; u < end;) {
-        const int last = (int)min((long long)p.blocks, p.block + (end - u));
-        const int blocks = min(last, tile_blocks(p, a, t));
-        const int packed = p.pair * kPair + t * kTile;
+    // The row's queries, swizzled as the copy engine does it.
+    const auto give_queries = [&](const ChunkPlace& p, const TileRow& r) {
+        const unsigned char* qp = a.queries + ((long long)p.q.first + r.token) * a.q_row + r.head * a.q_head;
+#pragma unroll
+        for (int h = 0; h < Layout::halves; ++h) {
+            uint4 v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                v[c] = make_uint4(0, 0, 0, 0);
+                if (r.valid) v[c] = *reinterpret_cast<const uint4*>(qp + h * 128 + c * 16);
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
+                *reinterpret_cast<uint4*>(smem + t * Layout::tile_bytes + h * kHalfBytes + row * 128 +
+                                          ((c ^ (row & 7)) << 4)) = v[c];
+            }
+        }
+        cache_proxy_fence();
+        __syncwarp();
+        if (lane == 0) cache_arrive(bar.queries + t);
+    };
+    int todo = (int)(end - begin);
+    int last = min(p.blocks, p.block + todo);
+    int blocks = min(last, tile_blocks<Layout::rows>(p, a, t));
+    TileRow r = tile_row(a, p.q, p.head, p.item * Layout::rows + t * kTile + row);
+    if (p.block < blocks) give_queries(p, r);
+    while (true) {
+        const int packed = p.item * Layout::rows + t * kTile;
         const bool active = p.block < blocks;
-        const TileRow r = tile_row(a, p.q, p.head, packed + row);
         const long long at = (long long)p.q.first + r.token;
         float from = 0.f, sum = 0.f;
         bool unset = true, ready = false;  // no key seen yet; every row of the warp has seen one
         if (active) {
-            // The row's queries, swizzled as the copy engine does it.
-            const unsigned char* qp = a.queries + at * a.q_row + r.head * a.q_head;
-#pragma unroll
-            for (int h = 0; h < Layout::halves; ++h)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r.valid) v = *reinterpret_cast<const uint4*>(qp + h * 128 + c * 16);
-                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                    *reinterpret_cast<uint4*>(smem + t * Layout::tile_bytes + h * kHalfBytes + row * 128 +
-                                              ((c ^ (row & 7)) << 4)) = v;
-                }
-            cache_proxy_fence();
-            __syncwarp();
-            if (lane == 0) cache_arrive(bar.queries + t);
             // Keys below `clear` are seen by every row of the tile.
             const int clear = tile_row(a, p.q, p.head, packed).seen;
             for (int j = p.block; j < blocks; ++j) {
@@ -628,6 +725,21 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                 hand_over(1);
                 h_parity ^= 1;
             }
+        }
+        // The next item's queries go out before this one's results, and its
+        // first scores are made meanwhile.
+        todo -= last - p.block;
+        ChunkPlace pn = p;
+        int last_n = 0, blocks_n = 0;
+        TileRow rn = r;
+        if (todo > 0) {
+            next_item<Layout::rows>(pn, a);
+            last_n = min(pn.blocks, pn.block + todo);
+            blocks_n = min(last_n, tile_blocks<Layout::rows>(pn, a, t));
+            rn = tile_row(a, pn.q, pn.head, pn.item * Layout::rows + t * kTile + row);
+            if (pn.block < blocks_n) give_queries(pn, rn);
+        }
+        if (active) {
             cache_wait(bar.o + t, o_parity, abort, a.status, kWaitO);
             o_parity ^= 1;
             tmem_fence_after();
@@ -635,7 +747,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         const bool whole = p.block == 0 && last == p.blocks;
         const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
         const float log_sum = unset ? -INFINITY : from;
-        float* part = cut_partials(a, gridDim.x) + ((long long)blockIdx.x * 2 + (p.block > 0 ? 0 : 1)) * Partial<D, kPair>::floats;
+        float* part = cut_partials(a.workspace, gridDim.x) + ((long long)blockIdx.x * 2 + (p.block > 0 ? 0 : 1)) * partial_floats<D>(Layout::rows);
         bool fine = true;
         unsigned char* op = a.out + at * a.o_row + r.head * a.o_head;
         if (active || !whole) {
@@ -669,11 +781,11 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         }
         if (r.valid && whole && a.lse) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (log_sum + log2f(sum)) * kLn2 : -INFINITY;
         if (r.valid && !whole) {
-            part[kPair * D + t * kTile + row] = log_sum;
-            part[kPair * (D + 1) + t * kTile + row] = sum;
+            part[Layout::rows * D + t * kTile + row] = log_sum;
+            part[Layout::rows * (D + 1) + t * kTile + row] = sum;
         }
         // Rows that a key behind them made no number.
-        unsigned again = __ballot_sync(0xffffffffu, whole && r.valid && !fine && r.seen > 0 && r.seen < p.q.length);
+        unsigned again = __ballot_sync(0xffffffffu, whole && r.valid && !fine && r.seen > 0 && (cache_eight(S) || r.seen < p.q.length));
         while (again) {
             const int i = __ffs(again) - 1;
             again &= again - 1;
@@ -682,26 +794,33 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             attend_row<T, S, D>(a, p.s, p.q.first, p.q.rows, p.q.length, token, head);
         }
         tmem_fence_before();  // this tile's reads, before the products that the next arrival lets run
-        u += last - p.block;
-        next_pair(p, a);
+        if (todo <= 0) break;
+        p = pn;
+        last = last_n;
+        blocks = blocks_n;
+        r = rn;
     }
 }
 
 template <typename T, int S, int D>
-__global__ void __launch_bounds__(kChunkThreads, 1)
+__global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>::ctas)
     cache_chunk_kernel(const __grid_constant__ CacheAttendArgs a, const __grid_constant__ CacheMaps maps) {
     using Layout = ChunkLayout<S, D>;
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Layout::bar_at);
-    const ChunkBars bar = {bars, bars + Layout::stages, bars + 2 * Layout::stages, bars + 2 * Layout::stages + 2,
-                           bars + 2 * Layout::stages + 6, bars + 2 * Layout::stages + 8, bars + 2 * Layout::stages + 10,
-                           bars + 2 * Layout::stages + 12};
+    uint64_t* tile_bars = bars + 2 * Layout::stages;
+    constexpr int kTiles = Layout::tiles;
+    const ChunkBars bar = {bars, bars + Layout::stages, tile_bars, tile_bars + kTiles, tile_bars + 3 * kTiles,
+                           tile_bars + 4 * kTiles, tile_bars + 5 * kTiles, tile_bars + 6 * kTiles};
     volatile int* abort = reinterpret_cast<volatile int*>(bars + Layout::bars);
     uint32_t* slot = reinterpret_cast<uint32_t*>(bars + Layout::bars) + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * Layout::stages; ++i) cache_barrier_init(bars + i, 1);
-        for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < Layout::stages; ++i) {
+            cache_barrier_init(bar.full + i, Layout::copy_warps);
+            cache_barrier_init(bar.empty + i, 1);
+        }
+        for (int t = 0; t < Layout::tiles; ++t) {
             cache_barrier_init(bar.scores + t, 1);
             cache_barrier_init(bar.p + 2 * t, kTile / 32);
             cache_barrier_init(bar.p + 2 * t + 1, kTile / 32);
@@ -713,79 +832,82 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) {
+    if (warp == Layout::mma_warp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(slot)),
-                     "r"(512u));
+                     "r"((uint32_t)Layout::columns));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    const long long total = all_blocks(a, lane);
+    // The few-row kernel behind this one may fill what SMs are left.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const long long total = all_blocks<Layout::rows>(a, lane);
     const long long per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
     const long long begin = min(total, blockIdx.x * per), end = min(total, begin + per);
-    const ChunkPlace p = begin < end ? find_block(a, begin, lane) : ChunkPlace{};
+    const ChunkPlace p = begin < end ? find_block<Layout::rows>(a, begin, lane) : ChunkPlace{};
     if (threadIdx.x == 0) {
         CutItem cut{};
         const long long first = begin - p.block;  // the item's
         if (begin < end && p.block > 0 && first >= begin - per)
-            cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.pair};
-        cut_items(a)[blockIdx.x] = cut;
+            cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.item};
+        cut_items(a.workspace)[blockIdx.x] = cut;
     }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = *slot;
     if (begin < end) {
-        if (warp == kCopyWarp) chunk_copy<S, D>(a, maps, smem, bar, abort, p, begin, end, lane);
-        else if (warp == kMmaWarp) chunk_products<T, S, D>(a, smem, bar, tmem, abort, p, begin, end, lane);
+        if (warp > Layout::mma_warp) {
+            if constexpr (cache_eight(S))
+                chunk_widen<T, S, D>(a, smem, bar, abort, p, begin, end, warp - Layout::mma_warp - 1, lane);
+            else chunk_copy<S, D>(a, maps, smem, bar, abort, p, begin, end, lane);
+        } else if (warp == Layout::mma_warp) chunk_products<T, S, D>(a, smem, bar, tmem, abort, p, begin, end, lane);
         else chunk_softmax<T, S, D>(a, smem, bar, tmem, abort, p, begin, end, warp >> 2);
     }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    if (warp == kMmaWarp)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    if (warp == Layout::mma_warp)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Layout::columns));
 }
 
 // ------------------------------------------------------------------- launch
 
-template <typename T, int S, int D>
-void launch_chunk(const CacheAttendArgs& a, const CacheMaps& maps, int sms, cudaStream_t stream) {
+// As many CTAs as there can be blocks, those that the SMs hold at most.
+template <int S, int D>
+int chunk_grid(const CacheAttendArgs& a, int sms) {
     using Layout = ChunkLayout<S, D>;
-    // As many CTAs as there can be blocks, one an SM at most.
-    const long long pairs = (long long)a.rows * a.group / kPair + a.batch.sequences;
+    const long long items = (long long)a.rows * a.group / Layout::rows + a.batch.sequences;
     const long long blocks = (((long long)a.batch.columns << a.cache.page_shift) + kBlockKeys - 1) / kBlockKeys;
-    const int grid = (int)std::min((double)sms, (double)pairs * a.cache.heads * std::max(1ll, blocks));
-    cache_chunk_kernel<T, S, D><<<grid, kChunkThreads, Layout::bytes, stream>>>(a, maps);
-    CUDA_CHECK(cudaGetLastError());
-    launch_join<T, S, D, kPair>(a, grid, stream);
-}
-
-template <typename F>
-void with_chunk_types(int storage, bool bf16, int width, F&& f) {
-    with_cache_types(storage, bf16, width, [&](auto t, auto s, auto d) {
-        if constexpr (!cache_eight(decltype(s)::value)) f(t, s, d);
-    });
+    return (int)std::min((double)sms * Layout::ctas, (double)items * a.cache.heads * std::max(1ll, blocks));
 }
 
 }  // namespace
 
-bool cache_chunk_takes(int storage) { return !cache_eight(storage); }
-
-size_t cache_chunk_workspace(const CacheAttendShape& shape) { return cut_workspace(shape.sms, shape.width, kPair); }
+size_t cache_chunk_workspace(const CacheAttendShape& shape) {
+    // one CTA of two tiles an SM, or two of one
+    return cut_workspace(shape.sms * 2, shape.width, kTile) + 256;
+}
 
 void prepare_cache_chunk(int storage, int width) {
     for (bool bf16 : {false, true})
-        with_chunk_types(storage, bf16, width, [&](auto t, auto s, auto d) {
+        with_cache_types(storage, bf16, width, [&](auto t, auto s, auto d) {
             CUDA_CHECK(cudaFuncSetAttribute(cache_chunk_kernel<decltype(t), s.value, d.value>,
                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             ChunkLayout<s.value, d.value>::bytes));
         });
 }
 
-void launch_cache_chunk(const CacheAttendArgs& a, const CacheMaps& maps, const CacheAttendShape& shape,
-                        cudaStream_t stream) {
-    with_chunk_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
-        launch_chunk<decltype(t), s.value, d.value>(a, maps, shape.sms, stream);
+CutPart launch_cache_chunk(const CacheAttendArgs& a, const CacheMaps& maps, const CacheAttendShape& shape,
+                           cudaStream_t stream) {
+    CutPart part{};
+    with_cache_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
+        constexpr int S = s.value, D = d.value;
+        using Layout = ChunkLayout<S, D>;
+        const int grid = chunk_grid<S, D>(a, shape.sms);
+        cache_chunk_kernel<decltype(t), S, D><<<grid, Layout::threads, Layout::bytes, stream>>>(a, maps);
+        CUDA_CHECK(cudaGetLastError());
+        part = {a.workspace, grid, Layout::rows};
     });
+    return part;
 }
 
 }  // namespace wsp

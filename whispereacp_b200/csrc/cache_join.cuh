@@ -17,16 +17,17 @@ struct CutItem {
     int parts;  // partial results of the item, if this CTA's is the second; else 0
     int sequence, head, tile;
 };
-template <int D, int kRows>
-struct Partial {
-    static constexpr int floats = kRows * (D + 2);  // o, then m, then sum
-};
-inline size_t cut_workspace(long long grid, int width, int rows) {
-    return (sizeof(CutItem) * grid + 255) / 256 * 256 + grid * 2 * rows * (width + 2) * 4;
+// A partial result: o, then m, then sum.
+template <int D>
+__host__ __device__ constexpr int partial_floats(int rows) {
+    return rows * (D + 2);
 }
-__device__ __forceinline__ CutItem* cut_items(const CacheAttendArgs& a) { return reinterpret_cast<CutItem*>(a.workspace); }
-__device__ __forceinline__ float* cut_partials(const CacheAttendArgs& a, int grid) {
-    return reinterpret_cast<float*>(a.workspace + ((sizeof(CutItem) * grid + 255) / 256) * 256);
+inline size_t cut_workspace(long long grid, int width, int rows) {
+    return (sizeof(CutItem) * grid + 255) / 256 * 256 + (grid * 2 * rows * (width + 2) * 4 + 255) / 256 * 256;
+}
+__device__ __forceinline__ CutItem* cut_items(unsigned char* workspace) { return reinterpret_cast<CutItem*>(workspace); }
+__device__ __forceinline__ float* cut_partials(unsigned char* workspace, int grid) {
+    return reinterpret_cast<float*>(workspace + ((sizeof(CutItem) * grid + 255) / 256) * 256);
 }
 
 __device__ __forceinline__ long long warp_scan(long long v, int lane) {
@@ -40,38 +41,42 @@ __device__ __forceinline__ long long warp_scan(long long v, int lane) {
 
 // ----------------------------------------------------------------- the join
 
-constexpr int kJoinRows = 4;
-
-// Block (c, y) joins rows 4 y .. of the item that the border between the runs
-// of CTAs c and c + 1 cuts, if no earlier border does.  Its warps share out
-// the rows and each row's partial results.
-template <typename T, int S, int D, int kRows, int kThreads>
-__global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_constant__ CacheAttendArgs a, int grid) {
+// Block (c, y) of a part joins rows of the item that the border between the
+// runs of CTAs c and c + 1 cuts, if no earlier border does.  Its warps share
+// out the rows and each row's partial results.
+template <typename T, int S, int D, int kThreads>
+__global__ void __launch_bounds__(kThreads)
+    cache_join_kernel(const __grid_constant__ CacheAttendArgs a, CutPart first, CutPart second) {
     constexpr int kPer = D / 32;
     constexpr int kJoinWarps = kThreads / 32;
     __shared__ float shared_o[kJoinWarps][D];
     __shared__ float shared_ml[kJoinWarps][2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool late = (int)blockIdx.x >= first.blocks();
+    const CutPart part_of = late ? second : first;
+    const int block = (int)blockIdx.x - (late ? first.blocks() : 0);
+    const int c = block / part_of.slices() + 1, slice = block % part_of.slices();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = blockIdx.x + 1;
-    const int4 record = *reinterpret_cast<const int4*>(cut_items(a) + c);
+    const int4 record = *reinterpret_cast<const int4*>(cut_items(part_of.workspace) + c);
     const CutItem cut = {record.x, record.y, record.z, record.w};
     if (cut.parts == 0) return;
-    const float* partials = cut_partials(a, grid);
+    const float* partials = cut_partials(part_of.workspace, part_of.grid);
+    const int tile_rows = part_of.rows, floats = partial_floats<D>(tile_rows);
     const CacheSequence q = cache_sequence(a.batch, cut.sequence);
-    const int all_rows = (int)min((long long)kRows, (long long)q.rows * a.group - (long long)cut.tile * kRows);
-    for (int first = (int)blockIdx.y * kJoinRows; first < all_rows; first += (int)gridDim.y * kJoinRows) {
-        const int rows = min(kJoinRows, all_rows - first);
+    const int all_rows = (int)min((long long)tile_rows, (long long)q.rows * a.group - (long long)cut.tile * tile_rows);
+    const int end = min(all_rows, (slice + 1) * kJoinSlice);
+    for (int base = slice * kJoinSlice; base < end; base += kJoinRows) {
+        const int rows = min(kJoinRows, end - base);
         int share = 1;  // warps of a row
         while (share * 2 * rows <= kJoinWarps && share < cut.parts) share *= 2;
-        const int local = warp / share, sub = warp % share, row = first + local;
+        const int local = warp / share, sub = warp % share, row = base + local;
         const bool active = local < rows;
         float m = -INFINITY, sum = 0.f, o[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) o[e] = 0.f;
         const auto add = [&](float pm, float ps, const float* v) {
-            const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
-            const float keep = exp2_fast(m - base), gain = exp2_fast(pm - base);
+            const float top = fmaxf(m, pm), from = top == -INFINITY ? 0.f : top;
+            const float keep = exp2_fast(m - from), gain = exp2_fast(pm - from);
             sum = sum * keep + ps * gain;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) o[e] = o[e] * keep + v[e] * gain;
@@ -81,11 +86,11 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_const
             const int from = (int)((long long)cut.parts * sub / share), to = (int)((long long)cut.parts * (sub + 1) / share);
 #pragma unroll 4
             for (int i = from; i < to; ++i) {
-                const float* part = partials + ((long long)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * Partial<D, kRows>::floats;
+                const float* part = partials + ((long long)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * floats;
                 float v[kPer];
 #pragma unroll
                 for (int e = 0; e < kPer; ++e) v[e] = part[row * D + lane * kPer + e];
-                add(part[kRows * D + row], part[kRows * (D + 1) + row], v);
+                add(part[tile_rows * D + row], part[tile_rows * (D + 1) + row], v);
             }
         }
         if (share > 1) {
@@ -101,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_const
                 for (int w = warp + 1; w < warp + share; ++w) add(shared_ml[w][0], shared_ml[w][1], &shared_o[w][lane * kPer]);
         }
         if (!active || sub != 0) continue;
-        const TileRow r = tile_row(a, q, cut.head, cut.tile * kRows + row);
+        const TileRow r = tile_row(a, q, cut.head, cut.tile * tile_rows + row);
         if (!r.valid) continue;
         const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
         const long long at = (long long)q.first + r.token;
@@ -114,20 +119,22 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_const
             *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(x, y);
         }
         if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
-        if (__any_sync(0xffffffffu, !fine) && r.seen < q.length && r.seen > 0)
+        if (__any_sync(0xffffffffu, !fine) && r.seen > 0 && (cache_eight(S) || r.seen < q.length))
             attend_row<T, S, D>(a, cut.sequence, q.first, q.rows, q.length, r.token, r.head);
     }
 }
 
-template <typename T, int S, int D, int kRows>
-void launch_join(const CacheAttendArgs& a, int grid, cudaStream_t stream) {
-    if (grid == 1) return;
-    // The join's launch overlaps the end of the kernel it waits for.  Where
-    // items are far fewer than CTAs, 16 warps share a row's many parts.
-    const long long items = std::max((long long)a.batch.sequences, (long long)a.rows * a.group / kRows) * a.cache.heads;
-    const bool many = grid > 8 * items;
+// Joins the items that a call's kernels cut, the last of which it was launched
+// behind: its launch overlaps that one's end.  Where items are far fewer than
+// CTAs, 16 warps share a row's many parts.
+template <typename T, int S, int D>
+void launch_join(const CacheAttendArgs& a, const CutPart& first, const CutPart& second, cudaStream_t stream) {
+    const int blocks = first.blocks() + second.blocks();
+    if (blocks == 0) return;
+    const long long items = std::max((long long)a.batch.sequences, (long long)a.rows * a.group / first.rows) * a.cache.heads;
+    const bool many = first.grid > 8 * items;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid - 1, kRows / kJoinRows);
+    config.gridDim = dim3(blocks);
     config.blockDim = dim3(many ? 512 : 128);
     config.stream = stream;
     cudaLaunchAttribute early{};
@@ -135,8 +142,8 @@ void launch_join(const CacheAttendArgs& a, int grid, cudaStream_t stream) {
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    CUDA_CHECK(cudaLaunchKernelEx(
-        &config, many ? cache_join_kernel<T, S, D, kRows, 512> : cache_join_kernel<T, S, D, kRows, 128>, a, grid));
+    CUDA_CHECK(cudaLaunchKernelEx(&config, many ? cache_join_kernel<T, S, D, 512> : cache_join_kernel<T, S, D, 128>, a,
+                                  first, second));
 }
 
 template <typename F>
