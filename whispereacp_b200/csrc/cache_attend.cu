@@ -72,6 +72,13 @@ template <int kKeys>
 __device__ __forceinline__ int item_units(int length) {
     return max(1, (length + kKeys - 1) / kKeys);
 }
+// What an item costs beside its units (its queries, the warps' meeting, its
+// results: 2500 cycles), in units (700 to 900): the list that the CTAs share
+// out counts it in front of the item's first unit.
+template <int kKeys>
+constexpr int item_cost() {
+    return kKeys == 64 ? 3 : 2;
+}
 
 // The items of a sequence of one head: tiles of its n * group rows, none where
 // those are more than this kernel is to take.
@@ -82,7 +89,7 @@ __device__ __forceinline__ int item_tiles(const CacheSequence& q, const CacheAtt
 }
 template <int kKeys, int kRows>
 __device__ __forceinline__ long long sequence_units(const CacheSequence& q, const CacheAttendArgs& a) {
-    return (long long)item_tiles<kRows>(q, a) * a.cache.heads * item_units<kKeys>(q.length);
+    return (long long)item_tiles<kRows>(q, a) * a.cache.heads * (item_units<kKeys>(q.length) + item_cost<kKeys>());
 }
 
 // Where a unit lies; every warp finds it for itself.
@@ -94,24 +101,41 @@ struct Place {
     int units, tiles; // of the item; items of a head
 };
 
+// A lane's sequence of the first 32 and its units, kept for find_unit.
+struct FirstSequences {
+    CacheSequence q;
+    long long units;
+};
+
 template <int kKeys, int kRows>
-__device__ __forceinline__ long long all_units(const CacheAttendArgs& a, int lane) {
-    long long sum = 0;
-    for (int s = lane; s < a.batch.sequences; s += 32) sum += sequence_units<kKeys, kRows>(cache_sequence(a.batch, s), a);
+__device__ __forceinline__ long long all_units(const CacheAttendArgs& a, int lane, FirstSequences& kept) {
+    kept = FirstSequences{};
+    if (lane < a.batch.sequences) {
+        kept.q = cache_sequence(a.batch, lane);
+        kept.units = sequence_units<kKeys, kRows>(kept.q, a);
+    }
+    long long sum = kept.units;
+    for (int s = lane + 32; s < a.batch.sequences; s += 32) sum += sequence_units<kKeys, kRows>(cache_sequence(a.batch, s), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
 
-// The place of unit u (below all_units); a warp.
+// The place of unit u (below all_units) of the list, and where in its item it
+// lies, the item's cost counted (below 0: in it).
 template <int kKeys, int kRows>
-__device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u, int lane) {
+__device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u, int lane, const FirstSequences& kept) {
     Place p{};
     for (int base = 0; base < a.batch.sequences; base += 32) {
-        const int s = base + lane;
-        CacheSequence q{};
-        if (s < a.batch.sequences) q = cache_sequence(a.batch, s);
-        const long long mine = s < a.batch.sequences ? sequence_units<kKeys, kRows>(q, a) : 0;
+        CacheSequence q = kept.q;
+        long long mine = kept.units;
+        if (base > 0) {
+            mine = 0;
+            if (base + lane < a.batch.sequences) {
+                q = cache_sequence(a.batch, base + lane);
+                mine = sequence_units<kKeys, kRows>(q, a);
+            }
+        }
         const long long upto = warp_scan(mine, lane);
         const unsigned holds = __ballot_sync(0xffffffffu, u < upto);
         if (holds) {
@@ -123,9 +147,11 @@ __device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u
             p.q.length = __shfl_sync(0xffffffffu, q.length, at);
             p.units = item_units<kKeys>(p.q.length);
             p.tiles = item_tiles<kRows>(p.q, a);
-            const long long item = inside / p.units;
-            p.unit = (int)(inside - item * p.units);
-            p.head = (int)(item / p.tiles);
+            const int each = p.units + item_cost<kKeys>();
+            // 32-bit division where it will do
+            const long long item = inside < 0x7fffffff ? (long long)((unsigned)inside / (unsigned)each) : inside / each;
+            p.unit = (int)(inside - item * each) - item_cost<kKeys>();
+            p.head = p.tiles == 1 ? (int)item : (int)(item / p.tiles);
             p.tile = (int)(item - (long long)p.head * p.tiles);
             return p;
         }
@@ -137,7 +163,7 @@ __device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u
 // The next item's first unit.
 template <int kKeys, int kRows>
 __device__ __forceinline__ void next_item(Place& p, const CacheAttendArgs& a) {
-    p.unit = 0;
+    p.unit = -item_cost<kKeys>();
     if (++p.tile < p.tiles) return;
     p.tile = 0;
     if (++p.head < a.cache.heads) return;
@@ -265,7 +291,7 @@ __device__ __forceinline__ void ends_behind() { asm volatile("griddepcontrol.wai
 template <int S, int D, int NT>
 __device__ __forceinline__ void token_producer(const CacheAttendArgs& a, const CacheMaps& maps, unsigned char* smem,
                                                uint64_t* full, uint64_t* empty, volatile int* abort, Place p,
-                                               long long begin, long long end, int lane) {
+                                               int left, int lane) {
     using Layout = TokenLayout<S, D, NT>;
     const int box_shift = cache_box_shift(a.cache.page_shift);
     const int box_rows = 1 << box_shift;
@@ -274,9 +300,10 @@ __device__ __forceinline__ void token_producer(const CacheAttendArgs& a, const C
     int table_s = -1, table_base = 0, entry = -1;
     int stage = 0, n = 0;
     uint32_t parity = 1;  // of the stage's previous release
-    for (long long u = begin; u < end;) {
-        const int last = (int)min((long long)p.units, p.unit + (end - u));
-        for (int t = p.unit; t < last; ++t, ++u) {
+    for (; left > 0; next_item<Layout::keys, Layout::rows>(p, a)) {
+        const int last = min(p.units, p.unit + left);
+        left -= last - p.unit;
+        for (int t = max(p.unit, 0); t < last; ++t) {
             if (n >= Layout::stages && !cache_wait(empty + stage, parity, abort, a.status, kWaitFree)) break;
             if (*abort) break;
             // 32 table entries at a time, a lane an entry
@@ -330,7 +357,6 @@ __device__ __forceinline__ void token_producer(const CacheAttendArgs& a, const C
             }
         }
         if (*abort) break;
-        next_item<Layout::keys, Layout::rows>(p, a);
     }
     if (*abort)  // the copies in flight land before the CTA's memory is given up
         for (int i = max(0, n - Layout::stages); i < n; ++i) {
@@ -368,13 +394,14 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         *redo = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const long long total = all_units<Layout::keys, kRows>(a, lane);
+    FirstSequences kept;
+    const long long total = all_units<Layout::keys, kRows>(a, lane, kept);
     const long long per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
     const long long begin = min(total, blockIdx.x * per), end = min(total, begin + per);
-    Place p = begin < end ? find_unit<Layout::keys, kRows>(a, begin, lane) : Place{};
+    Place p = begin < end ? find_unit<Layout::keys, kRows>(a, begin, lane, kept) : Place{};
     if (threadIdx.x == 0) {
         CutItem cut{};
-        const long long first = begin - p.unit;  // the item's
+        const long long first = begin - p.unit;  // the item's first unit
         if (begin < end && p.unit > 0 && first >= begin - per)
             cut = {(int)((first + p.units - 1) / per - blockIdx.x) + 2, p.s, p.head, p.tile};
         cut_items(a.workspace)[blockIdx.x] = cut;
@@ -385,7 +412,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         return;
     }
     if (warp == kWorkers) {
-        token_producer<S, D, NT>(a, maps, smem, full, empty, abort, p, begin, end, lane);
+        token_producer<S, D, NT>(a, maps, smem, full, empty, abort, p, (int)(end - begin), lane);
         ends_behind();
         return;
     }
@@ -399,8 +426,11 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     uint32_t parity = 0;
     uint32_t qf[NT][kSteps][2];
     load_queries<T, S, D, NT>(a, p, qf, lane);
-    for (long long u = begin; u < end;) {
-        const int last = (int)min((long long)p.units, p.unit + (end - u));
+    for (int left = (int)(end - begin); left > 0;) {
+        const int last = min(p.units, p.unit + left);
+        left -= last - p.unit;
+        p.unit = max(p.unit, 0);
+        if (last <= 0) break;  // the run ends in an item's cost
         const int valid = (int)min((long long)kRows, (long long)p.q.rows * a.group - (long long)p.tile * kRows);
         // A lane's rows are columns 2t and 2t + 1 of each 8.
         int seen[NT][2];
@@ -420,8 +450,8 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         const int clear = a.causal ? tile_row(a, p.q, p.head, p.tile * kRows).seen : p.q.length;
         uint32_t qn[NT][kSteps][2];  // the next item's
         Place pn = p;
-        const bool more = u + (last - p.unit) < end;
-        if (more) {
+        if (left <= item_cost<Layout::keys>()) left = 0;  // nothing behind this item but a cost
+        if (left > 0) {
             next_item<Layout::keys, kRows>(pn, a);
             load_queries<T, S, D, NT>(a, pn, qn, lane);
         }
@@ -441,7 +471,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
             for (int e = 0; e < 2; ++e) from[j][e] = sum[j][e] = 0.f, limit[j][e] = -INFINITY;
         int largest = 8;  // the value scales' largest byte so far
 
-        for (int t = p.unit; t < last; ++t, ++u) {
+        for (int t = p.unit; t < last; ++t) {
             cache_wait(full + stage, parity, abort, a.status, kWaitFull);
             unsigned char* keys = smem + stage * 2 * Layout::pool_bytes;
             unsigned char* values = keys + Layout::pool_bytes;

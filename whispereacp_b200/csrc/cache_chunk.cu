@@ -91,35 +91,59 @@ template <int kRows>
 __device__ __forceinline__ int chunk_blocks(const CacheSequence& q, const CacheAttendArgs& a, int item) {
     return max(1, (chunk_seen(q, a, (item + 1) * kRows) + kBlockKeys - 1) / kBlockKeys);
 }
+// What an item costs beside its blocks (queries, the first block's maximum,
+// results), in blocks: the list that the CTAs share out counts it in front of
+// the item's first block.
+constexpr int kItemCost = 2;
+
 // A sequence's blocks.
 template <int kRows>
 __device__ __forceinline__ long long chunk_units(const CacheSequence& q, const CacheAttendArgs& a) {
     const int items = chunk_items<kRows>(q, a);
     if (items == 0) return 0;
     long long sum = 0;
-    if (!a.causal) sum = (long long)items * chunk_blocks<kRows>(q, a, 0);
+    if (!a.causal) sum = (long long)items * (chunk_blocks<kRows>(q, a, 0) + kItemCost);
     else
-        for (int p = 0; p < items; ++p) sum += chunk_blocks<kRows>(q, a, p);
+        for (int p = 0; p < items; ++p) sum += chunk_blocks<kRows>(q, a, p) + kItemCost;
     return sum * a.cache.heads;
 }
 
+// A lane's sequence of the first 32 and its blocks, kept for find_block.
+struct FirstSequences {
+    CacheSequence q;
+    long long blocks;
+};
+
 template <int kRows>
-__device__ __forceinline__ long long all_blocks(const CacheAttendArgs& a, int lane) {
-    long long sum = 0;
-    for (int s = lane; s < a.batch.sequences; s += 32) sum += chunk_units<kRows>(cache_sequence(a.batch, s), a);
+__device__ __forceinline__ long long all_blocks(const CacheAttendArgs& a, int lane, FirstSequences& kept) {
+    kept = FirstSequences{};
+    if (lane < a.batch.sequences) {
+        kept.q = cache_sequence(a.batch, lane);
+        kept.blocks = chunk_units<kRows>(kept.q, a);
+    }
+    long long sum = kept.blocks;
+    for (int s = lane + 32; s < a.batch.sequences; s += 32) sum += chunk_units<kRows>(cache_sequence(a.batch, s), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
 
+// The place of block u (below all_blocks) of the list, and where in its item
+// it lies, the item's cost counted (below 0: in it).
 template <int kRows>
-__device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long long u, int lane) {
+__device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long long u, int lane,
+                                                 const FirstSequences& kept) {
     ChunkPlace p{};
     for (int base = 0; base < a.batch.sequences; base += 32) {
-        const int s = base + lane;
-        CacheSequence q{};
-        if (s < a.batch.sequences) q = cache_sequence(a.batch, s);
-        const long long mine = s < a.batch.sequences ? chunk_units<kRows>(q, a) : 0;
+        CacheSequence q = kept.q;
+        long long mine = kept.blocks;
+        if (base > 0) {
+            mine = 0;
+            if (base + lane < a.batch.sequences) {
+                q = cache_sequence(a.batch, base + lane);
+                mine = chunk_units<kRows>(q, a);
+            }
+        }
         const long long upto = warp_scan(mine, lane);
         const unsigned holds = __ballot_sync(0xffffffffu, u < upto);
         if (holds) {
@@ -130,18 +154,20 @@ __device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long 
             p.q.rows = __shfl_sync(0xffffffffu, q.rows, at);
             p.q.length = __shfl_sync(0xffffffffu, q.length, at);
             p.items = chunk_items<kRows>(p.q, a);
-            const long long head = __shfl_sync(0xffffffffu, mine, at) / a.cache.heads;  // blocks of a head
-            p.head = (int)(inside / head);
+            const long long all = __shfl_sync(0xffffffffu, mine, at);  // of every head
+            const long long head = all < 0x7fffffff ? (long long)((unsigned)all / (unsigned)a.cache.heads) : all / a.cache.heads;
+            // 32-bit division where it will do
+            p.head = inside < 0x7fffffff && head < 0x7fffffff ? (int)((unsigned)inside / (unsigned)head) : (int)(inside / head);
             inside -= p.head * head;
             // 32 items at a time
             for (;; p.item += 32) {
-                const int blocks = p.item + lane < p.items ? chunk_blocks<kRows>(p.q, a, p.item + lane) : 0;
+                const int blocks = p.item + lane < p.items ? chunk_blocks<kRows>(p.q, a, p.item + lane) + kItemCost : 0;
                 const long long to = warp_scan(blocks, lane);
                 const unsigned in = __ballot_sync(0xffffffffu, inside < to);
                 if (in) {
                     const int i = __ffs(in) - 1;
-                    p.block = (int)__shfl_sync(0xffffffffu, inside - (to - blocks), i);
-                    p.blocks = __shfl_sync(0xffffffffu, blocks, i);
+                    p.block = (int)__shfl_sync(0xffffffffu, inside - (to - blocks), i) - kItemCost;
+                    p.blocks = __shfl_sync(0xffffffffu, blocks, i) - kItemCost;
                     p.item += i;
                     return p;
                 }
@@ -155,7 +181,7 @@ __device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long 
 
 template <int kRows>
 __device__ __forceinline__ void next_item(ChunkPlace& p, const CacheAttendArgs& a) {
-    p.block = 0;
+    p.block = -kItemCost;
     if (++p.item >= p.items) {
         p.item = 0;
         if (++p.head >= a.cache.heads) {
@@ -168,6 +194,16 @@ __device__ __forceinline__ void next_item(ChunkPlace& p, const CacheAttendArgs& 
         }
     }
     p.blocks = chunk_blocks<kRows>(p.q, a, p.item);
+}
+
+// Takes the item at p out of the run, of which `todo` is left: returns the end
+// of the run's blocks of it (0 or less: the run ends in the item's cost).
+__device__ __forceinline__ int take_item(ChunkPlace& p, int& todo) {
+    const int last = min(p.blocks, p.block + todo);
+    todo -= last - p.block;
+    if (todo <= kItemCost) todo = 0;  // nothing behind this item but a cost
+    p.block = max(p.block, 0);
+    return last;
 }
 
 // The blocks of tile t of an item: 0 if it has no rows, else one at least.
@@ -330,10 +366,10 @@ __device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsi
     const int boxes = kBlockKeys >> box_shift;
     int stage = 0, n = 0;
     uint32_t parity = 1;
-    for (long long u = begin; u < end;) {
-        const int last = (int)min((long long)p.blocks, p.block + (end - u));
+    for (int todo = (int)(end - begin); todo > 0;) {
+        const int last = take_item(p, todo);
         const int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
-        for (int j = p.block; j < last; ++j, ++u) {
+        for (int j = p.block; j < last; ++j) {
             const int position = j * kBlockKeys + (min(lane, boxes - 1) << box_shift);
             const int row = position & ((1 << a.cache.page_shift) - 1);
             const bool mine = lane < boxes && position < seen;
@@ -385,7 +421,7 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
     int stage = 0, n = 0;
     uint32_t parity = 1;
     for (int todo = (int)(end - begin); todo > 0;) {
-        const int last = min(p.blocks, p.block + todo);
+        const int last = take_item(p, todo);
         const int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
         for (int j = p.block; j < last; ++j) {
             // A lane a page, of 16 rows at least.
@@ -440,7 +476,6 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
                 }
             }
         }
-        todo -= last - p.block;
         next_item<Layout::rows>(p, a);
     }
 }
@@ -473,7 +508,9 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
         __syncwarp();
     };
     for (int todo = uniform((int)(end - begin)); todo > 0;) {
-        const int first = uniform(p.block), last = uniform(min(p.blocks, p.block + todo));
+        const int last = uniform(take_item(p, todo)), first = uniform(p.block);
+        todo = uniform(todo);
+        if (last <= 0) break;
         int blocks[Layout::tiles];
 #pragma unroll
         for (int t = 0; t < Layout::tiles; ++t) blocks[t] = uniform(min(last, tile_blocks<Layout::rows>(p, a, t)));
@@ -538,7 +575,6 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
             }
             __syncwarp();
         }
-        todo -= last - first;
         next_item<Layout::rows>(p, a);
     }
     // Every product has completed before the tensor memory goes.
@@ -596,7 +632,8 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         if (lane == 0) cache_arrive(bar.queries + t);
     };
     int todo = (int)(end - begin);
-    int last = min(p.blocks, p.block + todo);
+    int last = take_item(p, todo);
+    if (last <= 0) return;
     int blocks = min(last, tile_blocks<Layout::rows>(p, a, t));
     TileRow r = tile_row(a, p.q, p.head, p.item * Layout::rows + t * kTile + row);
     if (p.block < blocks) give_queries(p, r);
@@ -728,13 +765,12 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         }
         // The next item's queries go out before this one's results, and its
         // first scores are made meanwhile.
-        todo -= last - p.block;
         ChunkPlace pn = p;
         int last_n = 0, blocks_n = 0;
         TileRow rn = r;
         if (todo > 0) {
             next_item<Layout::rows>(pn, a);
-            last_n = min(pn.blocks, pn.block + todo);
+            last_n = take_item(pn, todo);
             blocks_n = min(last_n, tile_blocks<Layout::rows>(pn, a, t));
             rn = tile_row(a, pn.q, pn.head, pn.item * Layout::rows + t * kTile + row);
             if (pn.block < blocks_n) give_queries(pn, rn);
@@ -794,7 +830,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             attend_row<T, S, D>(a, p.s, p.q.first, p.q.rows, p.q.length, token, head);
         }
         tmem_fence_before();  // this tile's reads, before the products that the next arrival lets run
-        if (todo <= 0) break;
+        if (last_n == 0) break;
         p = pn;
         last = last_n;
         blocks = blocks_n;
@@ -839,13 +875,14 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
     }
     // The few-row kernel behind this one may fill what SMs are left.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const long long total = all_blocks<Layout::rows>(a, lane);
+    FirstSequences kept;
+    const long long total = all_blocks<Layout::rows>(a, lane, kept);
     const long long per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
     const long long begin = min(total, blockIdx.x * per), end = min(total, begin + per);
-    const ChunkPlace p = begin < end ? find_block<Layout::rows>(a, begin, lane) : ChunkPlace{};
+    const ChunkPlace p = begin < end ? find_block<Layout::rows>(a, begin, lane, kept) : ChunkPlace{};
     if (threadIdx.x == 0) {
         CutItem cut{};
-        const long long first = begin - p.block;  // the item's
+        const long long first = begin - p.block;  // the item's first block
         if (begin < end && p.block > 0 && first >= begin - per)
             cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.item};
         cut_items(a.workspace)[blockIdx.x] = cut;
