@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 from ._native import (CCacheBatch, CCacheMemory, CCacheRows, CCacheShape, WSP_BFLOAT16, WSP_CACHE_BFLOAT16,
                       WSP_CACHE_E4M3, WSP_CACHE_FLOAT16, WSP_CACHE_INT8, WSP_FLOAT16, WSP_FLOAT32, ModelError, check,
@@ -39,11 +40,10 @@ def _name(dtype) -> str:
 
 
 def _row_type(dtype) -> int:
-    code = _codes.get(dtype)
+    code = _ROW_TYPES.get(_name(dtype))
     if code is None:
-        code = _codes[dtype] = _ROW_TYPES.get(_name(dtype), -1)
-    if code < 0:
         raise ValueError(f"rows are float32, float16 or bfloat16, not {_name(dtype)}")
+    _codes[dtype] = code
     return code
 
 
@@ -75,11 +75,12 @@ class CacheBatch:
         if max_rows is None:
             max_rows = int((starts[1:] - starts[:-1]).max()) if sequences else 0
         self.page_table, self.lengths, self.starts, self.max_rows = page_table, lengths, starts, max_rows
-        self.device = lengths.device
+        self.device, self.index = lengths.device, lengths.get_device()
         self._c = CCacheBatch(page_table.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
                               page_table.stride(0) if sequences > 1 else page_table.shape[1], page_table.shape[1],
                               sequences, max_rows)
         self._ref = ctypes.byref(self._c)
+        self.columns = page_table.shape[1]
 
 
 class PagedCache:
@@ -128,7 +129,12 @@ class PagedCache:
         check(self._lib.wsp_cache_create(ctypes.byref(shape), keys.device.index, ctypes.byref(memory),
                                          ctypes.byref(handle)))
         self._handle = handle
+        self._index = keys.device.index
+        self._scale = 1.0 / math.sqrt(width)
         self._workspace_bytes: dict = {}
+        self._workspaces: dict = {}
+        self._raw_stream = getattr(_torch()._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda index: _torch().cuda.current_stream(index).cuda_stream)
 
     @classmethod
     def allocate(cls, pages: int, heads: int, page_rows: int, head_width: int, storage: str = "float16",
@@ -179,8 +185,8 @@ class PagedCache:
                     rows = batch._rows_held = int(batch.starts[-1])
             dtype = dtype or (torch.float32 if self.eight else self.dtype)
             with self._allocating(stream):
-                keys, values = (torch.empty(rows, self.heads, self.head_width, dtype=dtype, device=self.device)
-                                for _ in range(2))
+                keys = torch.empty(rows, self.heads, self.head_width, dtype=dtype, device=self.device)
+                values = torch.empty_like(keys)
         rows = keys.shape[0]
         k, v = self._rows(keys, "keys", rows, self.heads), self._rows(values, "values", rows, self.heads)
         check(self._lib.wsp_cache_read(self._usable(batch), batch._ref, rows, ctypes.byref(k), ctypes.byref(v),
@@ -199,29 +205,33 @@ class PagedCache:
         query_heads], the log of the sum of exponentials.  A row without a key
         gets zeros and -inf.
         """
-        torch = _torch()
-        rows, heads = queries.shape[0], queries.shape[1]
+        shape = queries.shape
+        if len(shape) != 3:
+            raise ModelError(f"queries must be [rows, query_heads, {self.head_width}], not {list(shape)}")
+        rows, heads, _ = shape
         q = self._rows(queries, "queries", rows, heads)
         handle = self._usable(batch)
-        key = (heads, batch.max_rows)
+        key = (heads, batch.max_rows, batch.columns)
         needed = self._workspace_bytes.get(key)
         if needed is None:
             size = ctypes.c_size_t()
             check(self._lib.wsp_cache_attend_workspace(handle, batch._ref, rows, heads, ctypes.byref(size)))
             needed = self._workspace_bytes[key] = size.value
+        torch = _torch()
         with self._allocating(stream):
             if out is None:
-                out = torch.empty(rows, heads, self.head_width, dtype=queries.dtype, device=self.device)
-            if lse is None and return_lse:
-                lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device)
-            workspace = torch.empty(needed, dtype=torch.uint8, device=self.device) if needed else None
-        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (rows, heads) or
-                                not lse.is_contiguous() or lse.device != self.device):
-            raise ValueError(f"lse must be a contiguous float32 tensor [{rows}, {heads}] on the cache's device")
+                out = torch.empty_like(queries, memory_format=torch.contiguous_format)
+            if lse is None:
+                if return_lse:
+                    lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device)
+            elif lse.shape != (rows, heads) or lse.dtype != torch.float32 or not lse.is_contiguous() or \
+                    lse.get_device() != self._index:
+                raise ValueError(f"lse must be a contiguous float32 tensor [{rows}, {heads}] on the cache's device")
+            workspace = self._workspace(needed, stream) if needed else None
         o = self._rows(out, "out", rows, heads)
         check(self._lib.wsp_cache_attend(handle, batch._ref, rows, heads, ctypes.byref(q), ctypes.byref(o),
                                          lse.data_ptr() if lse is not None else None,
-                                         1.0 / math.sqrt(self.head_width) if scale is None else scale, causal,
+                                         self._scale if scale is None else scale, causal,
                                          workspace.data_ptr() if needed else None, needed, self._stream(stream)))
         return out if lse is None else (out, lse)
 
@@ -234,24 +244,39 @@ class PagedCache:
     def _usable(self, batch: CacheBatch):
         if self._handle is None:
             raise ValueError("the cache is closed")
-        if batch.device != self.device:
+        if batch.index != self._index:
             raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
         return self._handle
 
     def _rows(self, t, name: str, rows: int, heads: int) -> CCacheRows:
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{name} must be on {self.device}, not {t.device}")
-        if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != self.head_width:
+        if t.shape != (rows, heads, self.head_width):
             raise ModelError(f"{name} must be [{rows}, {heads}, {self.head_width}], not {list(t.shape)}")
         row_stride, head_stride, step = t.stride()
         if step != 1:
             raise ValueError(f"{name} must be contiguous in the last dimension")
-        return CCacheRows(t.data_ptr(), row_stride, head_stride, _row_type(t.dtype))
+        code = _codes.get(t.dtype)
+        return CCacheRows(t.data_ptr(), row_stride, head_stride, _row_type(t.dtype) if code is None else code)
 
     def _stream(self, stream):
         if stream is None:
-            return _torch().cuda.current_stream(self.device).cuda_stream
+            return self._raw_stream(self._index)
         return getattr(stream, "cuda_stream", stream)
+
+    def _workspace(self, needed: int, stream):
+        """A call's workspace.  Calls of one host thread on one of torch's
+        streams follow one another, so they share it; a captured call, whose
+        graph may run next to others, and a call on a given stream get their
+        own, which torch's allocator keeps for that stream's later work."""
+        torch = _torch()
+        if stream is not None or torch.cuda.is_current_stream_capturing():
+            return torch.empty(needed, dtype=torch.uint8, device=self.device)
+        key = (threading.get_ident(), self._raw_stream(self._index))
+        held = self._workspaces.get(key)
+        if held is None or held.numel() < needed:
+            held = self._workspaces[key] = torch.empty(needed, dtype=torch.uint8, device=self.device)
+        return held
 
     def _allocating(self, stream):
         """The context in which a call's tensors are allocated: its own stream,

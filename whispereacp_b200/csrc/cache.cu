@@ -341,8 +341,18 @@ CUtensorMap pool_map(const wsp_cache_shape& s, const wsp_cache_memory& m, void* 
     return map;
 }
 
-CacheAttendShape attend_shape(const wsp_cache& c, int dtype, int max_rows) {
-    return {c.shape.storage, dtype == WSP_BFLOAT16, c.shape.head_width, max_rows, c.sms};
+CacheAttendShape attend_shape(const wsp_cache& c, int dtype, const wsp_cache_batch& batch) {
+    return {c.shape.storage,    dtype == WSP_BFLOAT16,
+            c.shape.head_width, batch.max_rows,
+            (long long)batch.table_columns * c.shape.page_rows, c.sms};
+}
+
+size_t checked_workspace(const wsp_cache& c, const wsp_cache_batch* batch, int rows, int query_heads) {
+    check_batch(batch, rows);
+    if (query_heads <= 0 || query_heads % c.shape.heads)
+        throw ModelError("query_heads (" + to_string(query_heads) + ") must be a multiple of the cache's heads (" +
+                         to_string(c.shape.heads) + ")");
+    return cache_attend_workspace(attend_shape(c, WSP_FLOAT16, *batch), query_heads / c.shape.heads);
 }
 
 template <bool kWrite>
@@ -467,11 +477,7 @@ int wsp_cache_attend_workspace(const wsp_cache* cache, const wsp_cache_batch* ba
     return guarded([&] {
         const wsp_cache& c = wsp::checked(cache);
         if (!bytes) throw wsp::InvalidArgument("bytes must not be NULL");
-        wsp::check_batch(batch, rows);
-        if (query_heads <= 0 || query_heads % c.shape.heads)
-            throw wsp::ModelError("query_heads (" + std::to_string(query_heads) + ") must be a multiple of the cache's heads (" +
-                                  std::to_string(c.shape.heads) + ")");
-        *bytes = wsp::cache_attend_workspace(wsp::attend_shape(c, WSP_FLOAT16, batch->max_rows), query_heads / c.shape.heads);
+        *bytes = wsp::checked_workspace(c, batch, rows, query_heads);
     });
 }
 
@@ -481,12 +487,7 @@ int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, i
     return guarded([&] {
         using std::to_string;
         const wsp_cache& c = wsp::checked(cache);
-        size_t needed = 0;
-        if (const int status = wsp_cache_attend_workspace(cache, batch, rows, query_heads, &needed)) {
-            const std::string text = wsp::last_error_text();
-            if (status == WSP_MODEL_ERROR) throw wsp::ModelError(text);
-            throw wsp::InvalidArgument(text);
-        }
+        const size_t needed = wsp::checked_workspace(c, batch, rows, query_heads);
         const wsp::RowsView q = wsp::check_rows(queries, "queries", rows, query_heads, c.shape.head_width);
         const wsp::RowsView o = wsp::check_rows(out, "out", rows, query_heads, c.shape.head_width);
         if (queries->dtype != out->dtype || queries->dtype == WSP_FLOAT32)
@@ -519,7 +520,7 @@ int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, i
         a.status = c.status.get<int>();
         a.workspace = static_cast<unsigned char*>(workspace);
         wsp::CurrentDevice device(c.device);
-        wsp::launch_cache_attend(a, c.maps, wsp::attend_shape(c, queries->dtype, batch->max_rows),
+        wsp::launch_cache_attend(a, c.maps, wsp::attend_shape(c, queries->dtype, *batch),
                                  static_cast<cudaStream_t>(stream));
     });
 }

@@ -301,7 +301,7 @@ __device__ __forceinline__ void token_producer(const CacheAttendArgs& a, const C
     int stage = 0, n = 0;
     uint32_t parity = 1;  // of the stage's previous release
     for (; left > 0; next_item<Layout::keys, Layout::rows>(p, a)) {
-        const int last = min(p.units, p.unit + left);
+        const int last = a.uncut ? p.units : min(p.units, p.unit + left);
         left -= last - p.unit;
         for (int t = max(p.unit, 0); t < last; ++t) {
             if (n >= Layout::stages && !cache_wait(empty + stage, parity, abort, a.status, kWaitFree)) break;
@@ -399,7 +399,14 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     const long long per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
     const long long begin = min(total, blockIdx.x * per), end = min(total, begin + per);
     Place p = begin < end ? find_unit<Layout::keys, kRows>(a, begin, lane, kept) : Place{};
-    if (threadIdx.x == 0) {
+    int left = (int)(end - begin);
+    if (a.uncut) {
+        // Items that begin in the run, whole.
+        if (left > 0 && p.unit > -item_cost<Layout::keys>()) {
+            left -= p.units - p.unit;
+            if (left > 0) next_item<Layout::keys, kRows>(p, a);
+        }
+    } else if (threadIdx.x == 0) {
         CutItem cut{};
         const long long first = begin - p.unit;  // the item's first unit
         if (begin < end && p.unit > 0 && first >= begin - per)
@@ -407,12 +414,12 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         cut_items(a.workspace)[blockIdx.x] = cut;
     }
     __syncthreads();
-    if (begin >= end) {
+    if (left <= 0) {
         ends_behind();
         return;
     }
     if (warp == kWorkers) {
-        token_producer<S, D, NT>(a, maps, smem, full, empty, abort, p, (int)(end - begin), lane);
+        token_producer<S, D, NT>(a, maps, smem, full, empty, abort, p, left, lane);
         ends_behind();
         return;
     }
@@ -426,8 +433,8 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     uint32_t parity = 0;
     uint32_t qf[NT][kSteps][2];
     load_queries<T, S, D, NT>(a, p, qf, lane);
-    for (int left = (int)(end - begin); left > 0;) {
-        const int last = min(p.units, p.unit + left);
+    while (left > 0) {
+        const int last = a.uncut ? p.units : min(p.units, p.unit + left);
         left -= last - p.unit;
         p.unit = max(p.unit, 0);
         if (last <= 0) break;  // the run ends in an item's cost
@@ -450,7 +457,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         const int clear = a.causal ? tile_row(a, p.q, p.head, p.tile * kRows).seen : p.q.length;
         uint32_t qn[NT][kSteps][2];  // the next item's
         Place pn = p;
-        if (left <= item_cost<Layout::keys>()) left = 0;  // nothing behind this item but a cost
+        if (!a.uncut && left <= item_cost<Layout::keys>()) left = 0;  // nothing behind this item but a cost
         if (left > 0) {
             next_item<Layout::keys, kRows>(pn, a);
             load_queries<T, S, D, NT>(a, pn, qn, lane);
@@ -792,6 +799,15 @@ long long token_grid(const CacheAttendArgs& a, int sms) {
     return (long long)std::min((double)sms * Layout::ctas, (double)tiles * a.cache.heads * std::max(1ll, units));
 }
 
+// Where no item can be longer than this, whole items go to the CTAs instead of
+// equal runs: no partial results and no second kernel, at the price of runs
+// that end up to an item late.
+constexpr int kUncutUnits = 8;
+bool token_uncut(const CacheAttendShape& shape, int group) {
+    const int keys = shape.width * cache_bytes(shape.storage) == 64 ? 128 : 64;
+    return (long long)shape.max_rows * group <= 8 && shape.held <= (long long)kUncutUnits * keys;
+}
+
 template <typename T, int S, int D, int NT>
 CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, bool behind, cudaStream_t stream) {
     using Layout = TokenLayout<S, D, NT>;
@@ -807,7 +823,7 @@ CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, 
     config.attrs = &early;
     config.numAttrs = behind ? 1 : 0;
     CUDA_CHECK(cudaLaunchKernelEx(&config, cache_tokens_kernel<T, S, D, NT>, a, maps));
-    return {a.workspace, grid, Layout::rows};
+    return {a.workspace, a.uncut ? 0 : grid, Layout::rows};
 }
 
 }  // namespace
@@ -822,6 +838,7 @@ static size_t token_workspace(const CacheAttendShape& shape) {
 }
 
 size_t cache_attend_workspace(const CacheAttendShape& shape, int group) {
+    if (token_uncut(shape, group)) return 0;
     const bool chunks = (long long)shape.max_rows * group > kFewRows;
     return token_workspace(shape) + (chunks ? cache_chunk_workspace(shape) : 0);
 }
@@ -853,12 +870,15 @@ void launch_cache_attend(const CacheAttendArgs& args, const CacheMaps& maps, con
         b.workspace += token_workspace(shape);
         chunks = launch_cache_chunk(b, maps, shape, stream);
     }
-    // Tiles of 8 rows where every sequence's rows of a head fit one.
+    a.uncut = token_uncut(shape, a.group);
+    // Tiles of 16 rows where no sequence has more and some may have more than 8;
+    // among chunks, those that are left are mostly single tokens.
     with_cache_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
         using T = decltype(t);
         constexpr int S = s.value, D = d.value;
-        const CutPart tokens = most <= 8 ? launch_tokens<T, S, D, 1>(a, maps, shape.sms, most > kFewRows, stream)
-                                         : launch_tokens<T, S, D, 2>(a, maps, shape.sms, most > kFewRows, stream);
+        const CutPart tokens = most > 8 && most <= kFewRows
+                                   ? launch_tokens<T, S, D, 2>(a, maps, shape.sms, false, stream)
+                                   : launch_tokens<T, S, D, 1>(a, maps, shape.sms, most > kFewRows, stream);
         launch_join<T, S, D>(a, tokens, chunks, stream);
     });
 }

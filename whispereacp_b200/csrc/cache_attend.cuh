@@ -21,6 +21,7 @@ struct CacheAttendArgs {
     int rows, query_heads, group;  // group = query heads of a key head
     float scale;
     int causal;
+    int uncut;                     // the few-row kernel's CTAs take whole items
     long long few;                 // rows * group up to which a sequence is the few-row kernel's
     int* status;                   // which wait gave up, 0: none
     unsigned char* workspace;
@@ -33,11 +34,14 @@ struct CacheMaps {
 };
 
 // What a launch needs to know beside its arguments: the cache's storage, the
-// type of queries and out, the heads' width, the bound of a sequence's rows.
+// type of queries and out, the heads' width, the bounds of a sequence's new
+// and held rows.
 struct CacheAttendShape {
     int storage;
     bool bf16;
-    int width, max_rows, sms;
+    int width, max_rows;
+    long long held;
+    int sms;
 };
 
 // What a kernel leaves to be joined: its workspace, its CTAs, and the rows of

@@ -420,63 +420,84 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
     const int me = warp * 32 + lane;
     int stage = 0, n = 0;
     uint32_t parity = 1;
-    for (int todo = (int)(end - begin); todo > 0;) {
-        const int last = take_item(p, todo);
-        const int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
-        for (int j = p.block; j < last; ++j) {
-            // A lane a page, of 16 rows at least.
-            const int pages = max(1, kBlockKeys >> a.cache.page_shift);
-            const int first = j * kBlockKeys + (min(lane, pages - 1) << a.cache.page_shift);
-            const int entry = first < seen ? cache_page(a.cache, a.batch, p.s, first) : -1;
+    // A tile, keys or values of a block: this thread's pieces and their scales.
+    // The next tile's are on their way while this one's are written.
+    struct Tile {
+        uint4 raw[kMine];
+        uint8_t scale[kMine];
+    };
+    const auto fetch = [&](const ChunkPlace& p, int j, bool values, int seen, Tile& t) {
+        const unsigned char* pool = values ? a.cache.values : a.cache.keys;
+        const uint8_t* scales = values ? a.cache.value_scales : a.cache.key_scales;
+        // A lane a page, of 16 rows at least.
+        const int pages = max(1, kBlockKeys >> a.cache.page_shift);
+        const int first = j * kBlockKeys + (min(lane, pages - 1) << a.cache.page_shift);
+        const int entry = first < seen ? cache_page(a.cache, a.batch, p.s, first) : -1;
 #pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const unsigned char* pool = v ? a.cache.values : a.cache.keys;
-                const uint8_t* scales = v ? a.cache.value_scales : a.cache.key_scales;
-                uint4 raw[kMine];
-                uint32_t scale[kMine];
-#pragma unroll
-                for (int i = 0; i < kMine; ++i) {
-                    const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
-                    const int position = j * kBlockKeys + key;
-                    const int page = __shfl_sync(0xffffffffu, entry, min(key >> a.cache.page_shift, pages - 1));
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    scale[i] = 0;
-                    if (piece < kPieces && position < seen && page >= 0) {
-                        const int slot = position & ((1 << a.cache.page_shift) - 1);
-                        raw[i] = load_stream(pool + cache_offset(a.cache, page, p.head, slot) + c * 16);
-                        scale[i] = __ldg(scales + cache_scale_index(a.cache, page, p.head, slot));
-                    }
-                }
-                if (n >= Layout::stages) cache_wait(bar.empty + stage, parity, abort, a.status, kWaitSlot);
-                unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
-#pragma unroll
-                for (int i = 0; i < kMine; ++i) {
-                    const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
-                    if (piece >= kPieces) break;
-                    const float by = cache_scale(scale[i]);
-                    const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                    uint32_t out[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float2 f = cache_pair<S>((in[e / 2] >> (16 * (e & 1))) & 0xffffu);
-                        out[e] = Half16<T>::pack2(f.x * by, f.y * by);
-                    }
-                    unsigned char* to = tile + (c / 4) * kHalfBytes + key * 128;
-                    const int at = (c % 4) * 2;
-                    *reinterpret_cast<uint4*>(to + ((at ^ (key & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
-                    *reinterpret_cast<uint4*>(to + (((at + 1) ^ (key & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
-                }
-                cache_proxy_fence();
-                __syncwarp();
-                if (lane == 0) cache_arrive(bar.full + stage);
-                ++n;
-                if (++stage == Layout::stages) {
-                    stage = 0;
-                    parity ^= 1;
-                }
+        for (int i = 0; i < kMine; ++i) {
+            const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
+            const int position = j * kBlockKeys + key;
+            const int page = __shfl_sync(0xffffffffu, entry, min(key >> a.cache.page_shift, pages - 1));
+            t.raw[i] = make_uint4(0, 0, 0, 0);
+            t.scale[i] = 0;
+            if (piece < kPieces && position < seen && page >= 0) {
+                const int slot = position & ((1 << a.cache.page_shift) - 1);
+                t.raw[i] = load_stream(pool + cache_offset(a.cache, page, p.head, slot) + c * 16);
+                t.scale[i] = __ldg(scales + cache_scale_index(a.cache, page, p.head, slot));
             }
         }
-        next_item<Layout::rows>(p, a);
+    };
+    const auto write = [&](const Tile& t) {
+        if (n >= Layout::stages) cache_wait(bar.empty + stage, parity, abort, a.status, kWaitSlot);
+        unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
+            if (piece >= kPieces) break;
+            const float by = cache_scale(t.scale[i]);
+            const uint32_t in[4] = {t.raw[i].x, t.raw[i].y, t.raw[i].z, t.raw[i].w};
+            uint32_t out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 f = cache_pair<S>((in[e / 2] >> (16 * (e & 1))) & 0xffffu);
+                out[e] = Half16<T>::pack2(f.x * by, f.y * by);
+            }
+            unsigned char* to = tile + (c / 4) * kHalfBytes + key * 128;
+            const int at = (c % 4) * 2;
+            *reinterpret_cast<uint4*>(to + ((at ^ (key & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+            *reinterpret_cast<uint4*>(to + (((at + 1) ^ (key & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+        cache_proxy_fence();
+        __syncwarp();
+        if (lane == 0) cache_arrive(bar.full + stage);
+        ++n;
+        if (++stage == Layout::stages) {
+            stage = 0;
+            parity ^= 1;
+        }
+    };
+    Tile keys, values;
+    int todo = (int)(end - begin);
+    int last = take_item(p, todo);
+    if (last <= 0) return;
+    int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
+    fetch(p, p.block, false, seen, keys);
+    for (int j = p.block;;) {
+        fetch(p, j, true, seen, values);
+        write(keys);
+        bool more = true;
+        if (++j >= last) {
+            more = todo > 0;
+            if (more) {
+                next_item<Layout::rows>(p, a);
+                last = take_item(p, todo);
+                seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
+                j = p.block;
+            }
+        }
+        if (more) fetch(p, j, false, seen, keys);
+        write(values);
+        if (!more) return;
     }
 }
 
@@ -660,12 +681,11 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                 uint64_t sums[2];
                 const auto take = [&](int c) {
                     tmem_arrived(s[c & 1]);
-                    if (masked) {
-                        const int seen = r.seen - j * kBlockKeys;
+                    const int seen = r.seen - j * kBlockKeys - c * 32;
+                    if (masked && __any_sync(0xffffffffu, seen < 32))
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (c * 32 + e >= seen) s[c & 1][e] = 0xff800000u;
-                    }
+                            if (e >= seen) s[c & 1][e] = 0xff800000u;
                 };
                 const auto exponentials = [&](int c, auto computed) {
                     const uint64_t scale2 = pair_of(to_log2, to_log2), from2 = pair_of(-from, -from);
