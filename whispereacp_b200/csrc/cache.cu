@@ -14,10 +14,13 @@ namespace {
 
 // ---------------------------------------------------------- append and read
 //
-// A thread holds 8 elements of one row of one head, of the key and of the
-// value: D / 8 neighbouring lanes hold a row.  16 bytes of a 16-bit row and 8
-// of an 8-bit one are in flight per thread and side, which is what these two
-// kernels live on: they are bound by the bytes of the rows and the pages.
+// Bound by the bytes of the rows and the pages.  A block takes up to 16 rows,
+// finds each one's place once, and goes over (head, row, piece), pieces
+// fastest: a warp's lanes then cover 4 or 8 neighbouring rows of one head,
+// which lie next to one another in the page.  A thread holds a piece of 16 (8-bit
+// pages) or 8 values of the key and of the value: 16 bytes of the page each,
+// and 2 x 16 or 2 x 32 of the rows in flight.  The D / 16 lanes of an 8-bit row
+// agree on its scale.
 
 struct RowsView {
     unsigned char* data;
@@ -28,7 +31,7 @@ struct CopyArgs {
     CacheView cache;
     CacheBatchView batch;
     RowsView keys, values;
-    int rows, first_row;  // rows of the arrays; the first row of this launch
+    int rows, block_rows;  // rows of the arrays, and of a block: 2^n
 };
 
 // dtype codes of wsp_decoder.h as types
@@ -37,33 +40,45 @@ template <> struct RowType<WSP_FLOAT32> { static constexpr int bytes = 4; };
 template <> struct RowType<WSP_FLOAT16> { static constexpr int bytes = 2; using type = __half; };
 template <> struct RowType<WSP_BFLOAT16> { static constexpr int bytes = 2; using type = __nv_bfloat16; };
 
-template <int T>
-__device__ __forceinline__ void load8(const unsigned char* p, float (&x)[8]) {
+// kE values at p, of a row array or of 16-bit pages.
+template <int T, int kE>
+__device__ __forceinline__ void load_values(const unsigned char* p, float (&x)[kE]) {
     if constexpr (T == WSP_FLOAT32) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const uint4 v = load_stream(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = Half16<typename RowType<T>::type>::pair_to_float2(w[e]);
-            x[2 * e] = f.x;
-            x[2 * e + 1] = f.y;
+        for (int e = 0; e < kE; e += 4) {
+            const uint4 v = load_stream(p + e * 4);
+            x[e] = __uint_as_float(v.x), x[e + 1] = __uint_as_float(v.y);
+            x[e + 2] = __uint_as_float(v.z), x[e + 3] = __uint_as_float(v.w);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kE; e += 8) {
+            const uint4 v = load_stream(p + e * 2);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = Half16<typename RowType<T>::type>::pair_to_float2(w[i]);
+                x[e + 2 * i] = f.x;
+                x[e + 2 * i + 1] = f.y;
+            }
         }
     }
 }
 
-template <int T>
-__device__ __forceinline__ void store8(unsigned char* p, const float (&x)[8]) {
+template <int T, int kE>
+__device__ __forceinline__ void store_values(unsigned char* p, const float (&x)[kE]) {
     if constexpr (T == WSP_FLOAT32) {
-        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(p + 16) = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = Half16<typename RowType<T>::type>::pack2(x[2 * e], x[2 * e + 1]);
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int e = 0; e < kE; e += 4)
+            *reinterpret_cast<float4*>(p + e * 4) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kE; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = Half16<typename RowType<T>::type>::pack2(x[e + 2 * i], x[e + 2 * i + 1]);
+            *reinterpret_cast<uint4*>(p + e * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
 }
 
@@ -82,28 +97,29 @@ __device__ __forceinline__ uint32_t scale_byte(float top) {
     return (uint32_t)max(e, 1);
 }
 
-// Writes 8 elements of a row; the D / 8 lanes of a row agree on its scale.
-template <int S, int D>
-__device__ __forceinline__ void write8(unsigned char* p, uint8_t* scale, const float (&x)[8], bool valid) {
+// Writes a piece of a row into its page; the row's lanes agree on its scale.
+template <int S, int D, int kE>
+__device__ __forceinline__ void write_piece(unsigned char* p, uint8_t* scale, const float (&x)[kE], bool valid, int piece) {
     if constexpr (!cache_eight(S)) {
-        if (valid) store8<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
+        if (valid) store_values<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
     } else {
         // The largest magnitude through its bits, which order as the values
         // do and keep NaN on top.
         uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        for (int e = 0; e < kE; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
 #pragma unroll
-        for (int o = D / 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = D / kE / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const uint32_t byte = scale_byte<S>(__uint_as_float(top));
-        // 2^(127 - byte): exact, subnormal only for 254 (never chosen)
-        const float inverse = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
-        uint32_t w[2];
+        const bool fine = byte != 255u;
+        // 2^(127 - byte): byte is 1..249 here
+        const float inverse = __uint_as_float((254u - (fine ? byte : 127u)) << 23);
+        uint32_t w[kE / 4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kE / 4; ++h) {
             float y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = byte == 255u ? 0.f : x[4 * h + e] * inverse;
+            for (int e = 0; e < 4; ++e) y[e] = fine ? x[4 * h + e] * inverse : 0.f;
             if constexpr (S == kCacheE4m3) {
                 const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
                 const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
@@ -115,97 +131,104 @@ __device__ __forceinline__ void write8(unsigned char* p, uint8_t* scale, const f
             }
         }
         if (valid) {
-            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-            if ((threadIdx.x & (D / 8 - 1)) == 0) *scale = (uint8_t)byte;
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (piece == 0) *scale = (uint8_t)byte;
         }
     }
 }
 
-template <int S>
-__device__ __forceinline__ void read8(const unsigned char* p, const uint8_t* scale, float (&x)[8]) {
+template <int S, int kE>
+__device__ __forceinline__ void read_piece(const unsigned char* p, const uint8_t* scale, float (&x)[kE]) {
     if constexpr (!cache_eight(S)) {
-        load8<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
+        load_values<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
     } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        const float s = cache_scale(*scale);
+        const uint4 v = load_stream(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const float s = cache_scale(__ldg(scale));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = cache_pair<S>(((e < 2 ? v.x : v.y) >> (16 * (e & 1))) & 0xffffu);
+        for (int e = 0; e < 8; ++e) {
+            const float2 f = cache_pair<S>((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
             x[2 * e] = f.x * s;
             x[2 * e + 1] = f.y * s;
         }
     }
 }
 
-// The sequence that row r belongs to: the last s with starts[s] <= r, if r
-// is below starts[sequences]; -1 if none.
-__device__ __forceinline__ int sequence_of(const CacheBatchView& b, int r) {
-    int low = 0, high = b.sequences;
-    if (r < __ldg(b.starts) || r >= __ldg(b.starts + high)) return -1;
-    while (high - low > 1) {
-        const int mid = (low + high) >> 1;
-        if (__ldg(b.starts + mid) <= r) low = mid;
-        else high = mid;
-    }
-    return low;
-}
-
 constexpr int kCopyThreads = 256;
+constexpr int kCopyRows = 16;  // of a block, at most
 
 template <int S, int T, int D, bool kWrite>
-__global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const CopyArgs a) {
-    constexpr int kLanes = D / 8;  // lanes of a row
-    const long long item = ((long long)blockIdx.x * kCopyThreads + threadIdx.x) / kLanes;
-    const int piece = threadIdx.x % kLanes;
-    const long long row64 = item / a.cache.heads;
-    const int head = (int)(item - row64 * a.cache.heads);
-    const int r = (int)min(row64, (long long)a.rows);
-    int page = -1, slot = 0;
-    bool mine = r < a.rows;
-    if (mine) {
-        const int s = sequence_of(a.batch, r);
-        mine = s >= 0;
-        if (mine) {
-            const CacheSequence q = cache_sequence(a.batch, s);
-            const int position = q.length - q.rows + (r - q.first);
-            page = cache_page(a.cache, a.batch, s, position);
-            slot = position & ((1 << a.cache.page_shift) - 1);
+__global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_constant__ CopyArgs a) {
+    constexpr int kE = cache_eight(S) ? 16 : 8;  // values of a piece
+    constexpr int kLanes = D / kE;               // pieces of a row
+    __shared__ long long pool_at[kCopyRows], scale_at[kCopyRows];  // a row's place in head 0; -1: no page, -2: no row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int first = (int)blockIdx.x * a.block_rows;
+    for (int i = warp; i < a.block_rows; i += kCopyThreads / 32) {
+        const int r = first + i;
+        // The row's sequence: as many as end at or before it lie in front.
+        int s = 0;
+        for (int base = 0; base < a.batch.sequences; base += 32) {
+            const bool before = base + lane < a.batch.sequences && __ldg(a.batch.starts + base + lane + 1) <= r;
+            s += __popc(__ballot_sync(0xffffffffu, before));
+        }
+        if (lane == 0) {
+            long long at = -2, si = 0;
+            if (r < a.rows && s < a.batch.sequences) {
+                const CacheSequence q = cache_sequence(a.batch, s);
+                if (r >= q.first) {
+                    const int position = q.length - q.rows + (r - q.first);
+                    const int page = cache_page(a.cache, a.batch, s, position);
+                    const int slot = position & ((1 << a.cache.page_shift) - 1);
+                    at = page < 0 ? -1 : cache_offset(a.cache, page, 0, slot);
+                    si = page < 0 ? 0 : cache_scale_index(a.cache, page, 0, slot);
+                }
+            }
+            pool_at[i] = at;
+            scale_at[i] = si;
         }
     }
-    const long long key_at = (long long)r * a.keys.row_bytes + head * a.keys.head_bytes + piece * 8 * RowType<T>::bytes;
-    const long long value_at =
-        (long long)r * a.values.row_bytes + head * a.values.head_bytes + piece * 8 * RowType<T>::bytes;
-    const long long at = cache_offset(a.cache, page, head, slot) + piece * 8 * cache_bytes(S);
-    const long long si = cache_eight(S) ? cache_scale_index(a.cache, page, head, slot) : 0;
-    float k[8], v[8];
-    if constexpr (kWrite) {
-        // The row's lanes take the same branches; all stay for the shuffles.
-        const bool valid = page >= 0;
+    __syncthreads();
+    const int items = a.cache.heads * a.block_rows * kLanes, mask = a.block_rows - 1;
+    // Whole warps stay for the rows' shuffles.
+#pragma unroll 2
+    for (int base = warp * 32; base < items; base += kCopyThreads) {
+        const int item = min(base + lane, items - 1);
+        const int piece = item % kLanes, in_block = (item / kLanes) & mask, head = item / kLanes / a.block_rows;
+        const long long at = pool_at[in_block];
+        const bool valid = base + lane < items && at >= 0, zeros = base + lane < items && at == -1;
+        const int r = first + in_block;
+        const long long to = at + head * a.cache.head_bytes + piece * (kE * cache_bytes(S));
+        const long long si = cache_eight(S) ? scale_at[in_block] + ((long long)head << a.cache.page_shift) : 0;
+        unsigned char* key = a.keys.data + (long long)r * a.keys.row_bytes + head * a.keys.head_bytes + piece * (kE * RowType<T>::bytes);
+        unsigned char* value =
+            a.values.data + (long long)r * a.values.row_bytes + head * a.values.head_bytes + piece * (kE * RowType<T>::bytes);
+        float k[kE], v[kE];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
-        if (valid) {
-            load8<T>(a.keys.data + key_at, k);
-            load8<T>(a.values.data + value_at, v);
+        for (int e = 0; e < kE; ++e) k[e] = v[e] = 0.f;
+        if constexpr (kWrite) {
+            if (valid) {
+                load_values<T>(key, k);
+                load_values<T>(value, v);
+            }
+            write_piece<S, D>(a.cache.keys + to, a.cache.key_scales + si, k, valid, piece);
+            write_piece<S, D>(a.cache.values + to, a.cache.value_scales + si, v, valid, piece);
+        } else {
+            if (valid) {
+                read_piece<S>(a.cache.keys + to, a.cache.key_scales + si, k);
+                read_piece<S>(a.cache.values + to, a.cache.value_scales + si, v);
+            }
+            if (valid || zeros) {
+                store_values<T>(key, k);
+                store_values<T>(value, v);
+            }
         }
-        write8<S, D>(a.cache.keys + at, a.cache.key_scales + si, k, valid);
-        write8<S, D>(a.cache.values + at, a.cache.value_scales + si, v, valid);
-    } else {
-        if (!mine) return;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
-        if (page >= 0) {
-            read8<S>(a.cache.keys + at, a.cache.key_scales + si, k);
-            read8<S>(a.cache.values + at, a.cache.value_scales + si, v);
-        }
-        store8<T>(a.keys.data + key_at, k);
-        store8<T>(a.values.data + value_at, v);
     }
 }
 
 template <int S, int T, bool kWrite>
 void launch_copy(const CopyArgs& a, int width, cudaStream_t stream) {
-    const long long threads = (long long)a.rows * a.cache.heads * (width / 8);
-    const unsigned grid = (unsigned)((threads + kCopyThreads - 1) / kCopyThreads);
+    const unsigned grid = (unsigned)(((long long)a.rows + a.block_rows - 1) / a.block_rows);
     if (width == 64) cache_copy_kernel<S, T, 64, kWrite><<<grid, kCopyThreads, 0, stream>>>(a);
     else cache_copy_kernel<S, T, 128, kWrite><<<grid, kCopyThreads, 0, stream>>>(a);
 }
@@ -365,11 +388,12 @@ void copy_rows(wsp_cache* cache, const wsp_cache_batch* batch, int rows, const w
     a.values = check_rows(values, "values", rows, c.shape.heads, c.shape.head_width);
     if (keys->dtype != values->dtype) throw InvalidArgument("keys and values must have one dtype");
     if (rows == 0 || batch->sequences == 0) return;
-    if ((long long)rows * c.shape.heads * (c.shape.head_width / 8) > (long long)kCopyThreads * 0x7fffffff)
-        throw InvalidArgument("too many rows for one call: " + to_string(rows));
     a.cache = c.view;
     a.batch = batch_view(*batch);
     a.rows = rows;
+    // As many rows a block as leave every SM two blocks.
+    a.block_rows = 1;
+    while (a.block_rows < kCopyRows && rows / (2 * a.block_rows) >= 2 * c.sms) a.block_rows *= 2;
     CurrentDevice device(c.device);
     launch_copy<kWrite>(a, c.shape.storage, keys->dtype, c.shape.head_width, static_cast<cudaStream_t>(stream));
     CUDA_CHECK(cudaGetLastError());
