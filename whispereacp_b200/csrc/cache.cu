@@ -40,45 +40,57 @@ template <> struct RowType<WSP_FLOAT32> { static constexpr int bytes = 4; };
 template <> struct RowType<WSP_FLOAT16> { static constexpr int bytes = 2; using type = __half; };
 template <> struct RowType<WSP_BFLOAT16> { static constexpr int bytes = 2; using type = __nv_bfloat16; };
 
-// kE values at p, of a row array or of 16-bit pages.
-template <int T, int kE>
-__device__ __forceinline__ void load_values(const unsigned char* p, float (&x)[kE]) {
-    if constexpr (T == WSP_FLOAT32) {
+// A piece of kE values as it lies in memory, 4 bytes a word.
+template <int kWords>
+struct Piece {
+    uint32_t w[kWords];
+};
+template <int kWords>
+__device__ __forceinline__ Piece<kWords> fetch_piece(const unsigned char* p) {
+    Piece<kWords> v;
 #pragma unroll
-        for (int e = 0; e < kE; e += 4) {
-            const uint4 v = load_stream(p + e * 4);
-            x[e] = __uint_as_float(v.x), x[e + 1] = __uint_as_float(v.y);
-            x[e + 2] = __uint_as_float(v.z), x[e + 3] = __uint_as_float(v.w);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < kE; e += 8) {
-            const uint4 v = load_stream(p + e * 2);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = Half16<typename RowType<T>::type>::pair_to_float2(w[i]);
-                x[e + 2 * i] = f.x;
-                x[e + 2 * i + 1] = f.y;
-            }
-        }
+    for (int i = 0; i < kWords; i += 4) {
+        const uint4 x = load_stream(p + i * 4);
+        v.w[i] = x.x, v.w[i + 1] = x.y, v.w[i + 2] = x.z, v.w[i + 3] = x.w;
     }
+    return v;
+}
+template <int kWords>
+__device__ __forceinline__ void put_piece(unsigned char* p, const Piece<kWords>& v) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4)
+        *reinterpret_cast<uint4*>(p + i * 4) = make_uint4(v.w[i], v.w[i + 1], v.w[i + 2], v.w[i + 3]);
 }
 
-template <int T, int kE>
-__device__ __forceinline__ void store_values(unsigned char* p, const float (&x)[kE]) {
+// Values 2 i and 2 i + 1 of a piece of rows, and the way back.
+template <int T, int kWords>
+__device__ __forceinline__ float2 row_pair(const Piece<kWords>& v, int i) {
+    if constexpr (T == WSP_FLOAT32) return make_float2(__uint_as_float(v.w[2 * i]), __uint_as_float(v.w[2 * i + 1]));
+    else return Half16<typename RowType<T>::type>::pair_to_float2(v.w[i]);
+}
+template <int T, int kWords>
+__device__ __forceinline__ void set_row_pair(Piece<kWords>& v, int i, float x, float y) {
+    if constexpr (T == WSP_FLOAT32) v.w[2 * i] = __float_as_uint(x), v.w[2 * i + 1] = __float_as_uint(y);
+    else v.w[i] = Half16<typename RowType<T>::type>::pack2(x, y);
+}
+
+// The largest magnitude of a piece, through the values' bits: without the
+// sign they order as the values do, and keep a NaN on top.
+template <int T, int kWords>
+__device__ __forceinline__ float largest(const Piece<kWords>& v) {
     if constexpr (T == WSP_FLOAT32) {
+        uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < kE; e += 4)
-            *reinterpret_cast<float4*>(p + e * 4) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        for (int i = 0; i < kWords; ++i) top = max(top, v.w[i] & 0x7fffffffu);
+        return __uint_as_float(top);
     } else {
+        uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < kE; e += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = Half16<typename RowType<T>::type>::pack2(x[e + 2 * i], x[e + 2 * i + 1]);
-            *reinterpret_cast<uint4*>(p + e * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int i = 0; i < kWords; ++i)
+            asm("max.u16x2 %0, %1, %2;" : "=r"(top) : "r"(top), "r"(v.w[i] & 0x7fff7fffu));
+        const uint32_t one = max(top & 0xffffu, top >> 16);
+        if constexpr (T == WSP_BFLOAT16) return __uint_as_float(one << 16);
+        else return __half2float(__ushort_as_half((unsigned short)one));
     }
 }
 
@@ -97,59 +109,71 @@ __device__ __forceinline__ uint32_t scale_byte(float top) {
     return (uint32_t)max(e, 1);
 }
 
-// Writes a piece of a row into its page; the row's lanes agree on its scale.
-template <int S, int D, int kE>
-__device__ __forceinline__ void write_piece(unsigned char* p, uint8_t* scale, const float (&x)[kE], bool valid, int piece) {
+// A piece of rows as a piece of a page; the row's lanes agree on its scale
+// byte.  A row that holds an infinity or NaN has byte 255, and its values no
+// meaning.
+template <int S, int T, int D, int kIn, int kOut>
+__device__ __forceinline__ uint32_t narrow_piece(const Piece<kIn>& in, Piece<kOut>& out) {
     if constexpr (!cache_eight(S)) {
-        if (valid) store_values<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
-    } else {
-        // The largest magnitude through its bits, which order as the values
-        // do and keep NaN on top.
-        uint32_t top = 0;
+        constexpr int kStored = S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = D / kE / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const uint32_t byte = scale_byte<S>(__uint_as_float(top));
-        const bool fine = byte != 255u;
-        // 2^(127 - byte): byte is 1..249 here
-        const float inverse = __uint_as_float((254u - (fine ? byte : 127u)) << 23);
-        uint32_t w[kE / 4];
-#pragma unroll
-        for (int h = 0; h < kE / 4; ++h) {
-            float y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = fine ? x[4 * h + e] * inverse : 0.f;
-            if constexpr (S == kCacheE4m3) {
-                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-                w[h] = lo | (hi << 16);
+        for (int i = 0; i < kOut; ++i) {
+            if constexpr (T == kStored) {
+                out.w[i] = in.w[i];
             } else {
-                w[h] = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[h] |= ((uint32_t)__float2int_rn(y[e]) & 0xffu) << (8 * e);
+                const float2 x = row_pair<T>(in, i);
+                set_row_pair<kStored>(out, i, x.x, x.y);
             }
         }
-        if (valid) {
-            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-            if (piece == 0) *scale = (uint8_t)byte;
+        return 0;
+    } else {
+        float top = largest<T>(in);
+        // NaN above all: an order of the bits again
+        uint32_t bits = __float_as_uint(top);
+#pragma unroll
+        for (int o = D / 32; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+        const uint32_t byte = scale_byte<S>(__uint_as_float(bits));
+        // 2^(127 - byte); byte is 1..249, or 255 and then any finite factor
+        const float inverse = __uint_as_float((254u - min(byte, 253u)) << 23);
+#pragma unroll
+        for (int h = 0; h < kOut; ++h) {
+            const float2 x = row_pair<T>(in, 2 * h), y = row_pair<T>(in, 2 * h + 1);
+            if constexpr (S == kCacheE4m3) {
+                const uint32_t lo =
+                    __nv_cvt_float2_to_fp8x2(make_float2(x.x * inverse, x.y * inverse), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi =
+                    __nv_cvt_float2_to_fp8x2(make_float2(y.x * inverse, y.y * inverse), __NV_SATFINITE, __NV_E4M3);
+                out.w[h] = lo | (hi << 16);
+            } else {
+                const uint32_t a = __float2int_rn(x.x * inverse), b = __float2int_rn(x.y * inverse);
+                const uint32_t c = __float2int_rn(y.x * inverse), d = __float2int_rn(y.y * inverse);
+                out.w[h] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+            }
         }
+        return byte;
     }
 }
 
-template <int S, int kE>
-__device__ __forceinline__ void read_piece(const unsigned char* p, const uint8_t* scale, float (&x)[kE]) {
+// The way back: the values a piece of a page stands for, rounded once.
+template <int S, int T, int kIn, int kOut>
+__device__ __forceinline__ void widen_piece(const Piece<kIn>& in, uint32_t byte, Piece<kOut>& out) {
     if constexpr (!cache_eight(S)) {
-        load_values<S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16>(p, x);
-    } else {
-        const uint4 v = load_stream(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        const float s = cache_scale(__ldg(scale));
+        constexpr int kStored = S == kCacheF16 ? WSP_FLOAT16 : WSP_BFLOAT16;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float2 f = cache_pair<S>((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
-            x[2 * e] = f.x * s;
-            x[2 * e + 1] = f.y * s;
+        for (int i = 0; i < kIn; ++i) {
+            if constexpr (T == kStored) {
+                out.w[i] = in.w[i];
+            } else {
+                const float2 x = row_pair<kStored>(in, i);
+                set_row_pair<T>(out, i, x.x, x.y);
+            }
+        }
+    } else {
+        const float s = cache_scale(byte);
+#pragma unroll
+        for (int e = 0; e < 2 * kIn; ++e) {
+            const float2 f = cache_pair<S>((in.w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+            set_row_pair<T>(out, e, f.x * s, f.y * s);
         }
     }
 }
@@ -189,38 +213,67 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_c
         }
     }
     __syncthreads();
-    const int items = a.cache.heads * a.block_rows * kLanes, mask = a.block_rows - 1;
+    constexpr int kPage = kE * cache_bytes(S) / 4, kRow = kE * RowType<T>::bytes / 4;  // words of a piece
+    constexpr int kAtOnce = 2;  // pieces of the key and of the value on their way
+    const int items = a.cache.heads * a.block_rows * kLanes;
+    const int row_shift = 31 - __clz(a.block_rows);
     // Whole warps stay for the rows' shuffles.
-#pragma unroll 2
-    for (int base = warp * 32; base < items; base += kCopyThreads) {
-        const int item = min(base + lane, items - 1);
-        const int piece = item % kLanes, in_block = (item / kLanes) & mask, head = item / kLanes / a.block_rows;
-        const long long at = pool_at[in_block];
-        const bool valid = base + lane < items && at >= 0, zeros = base + lane < items && at == -1;
-        const int r = first + in_block;
-        const long long to = at + head * a.cache.head_bytes + piece * (kE * cache_bytes(S));
-        const long long si = cache_eight(S) ? scale_at[in_block] + ((long long)head << a.cache.page_shift) : 0;
-        unsigned char* key = a.keys.data + (long long)r * a.keys.row_bytes + head * a.keys.head_bytes + piece * (kE * RowType<T>::bytes);
-        unsigned char* value =
-            a.values.data + (long long)r * a.values.row_bytes + head * a.values.head_bytes + piece * (kE * RowType<T>::bytes);
-        float k[kE], v[kE];
+    for (int base = warp * 32; base < items; base += kAtOnce * kCopyThreads) {
+        Piece<kWrite ? kRow : kPage> key_in[kAtOnce], value_in[kAtOnce];
+        unsigned char *key_out[kAtOnce], *value_out[kAtOnce];
+        uint8_t *key_scale[kAtOnce], *value_scale[kAtOnce];
+        uint32_t key_byte[kAtOnce], value_byte[kAtOnce];
+        int state[kAtOnce];  // 1: a row and its page, 0: a row of no page, -1: none
 #pragma unroll
-        for (int e = 0; e < kE; ++e) k[e] = v[e] = 0.f;
-        if constexpr (kWrite) {
-            if (valid) {
-                load_values<T>(key, k);
-                load_values<T>(value, v);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int item = base + i * kCopyThreads + lane;
+            const int piece = item % kLanes, in_block = (item / kLanes) & (a.block_rows - 1);
+            const int head = (item / kLanes) >> row_shift;
+            const long long at = pool_at[in_block];
+            state[i] = item < items && at >= -1 ? (at >= 0) : -1;
+            const long long to = at + head * a.cache.head_bytes + piece * (kE * cache_bytes(S));
+            const long long r = first + in_block;
+            unsigned char* key = a.keys.data + r * a.keys.row_bytes + head * a.keys.head_bytes + piece * (kRow * 4);
+            unsigned char* value = a.values.data + r * a.values.row_bytes + head * a.values.head_bytes + piece * (kRow * 4);
+            if constexpr (cache_eight(S)) {
+                const long long si = scale_at[in_block] + ((long long)head << a.cache.page_shift);
+                key_scale[i] = a.cache.key_scales + si;
+                value_scale[i] = a.cache.value_scales + si;
+                if (piece != 0 && kWrite) key_scale[i] = nullptr;
             }
-            write_piece<S, D>(a.cache.keys + to, a.cache.key_scales + si, k, valid, piece);
-            write_piece<S, D>(a.cache.values + to, a.cache.value_scales + si, v, valid, piece);
-        } else {
-            if (valid) {
-                read_piece<S>(a.cache.keys + to, a.cache.key_scales + si, k);
-                read_piece<S>(a.cache.values + to, a.cache.value_scales + si, v);
+            key_out[i] = kWrite ? a.cache.keys + to : key;
+            value_out[i] = kWrite ? a.cache.values + to : value;
+            key_in[i] = value_in[i] = {};
+            key_byte[i] = value_byte[i] = 0;
+            if (state[i] == 1) {
+                key_in[i] = fetch_piece<kWrite ? kRow : kPage>(kWrite ? key : a.cache.keys + to);
+                value_in[i] = fetch_piece<kWrite ? kRow : kPage>(kWrite ? value : a.cache.values + to);
+                if constexpr (cache_eight(S) && !kWrite) {
+                    key_byte[i] = __ldg(key_scale[i]);
+                    value_byte[i] = __ldg(value_scale[i]);
+                }
             }
-            if (valid || zeros) {
-                store_values<T>(key, k);
-                store_values<T>(value, v);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if constexpr (kWrite) {
+                Piece<kPage> k, v;
+                const uint32_t kb = narrow_piece<S, T, D>(key_in[i], k), vb = narrow_piece<S, T, D>(value_in[i], v);
+                if (state[i] == 1) {
+                    put_piece(key_out[i], k);
+                    put_piece(value_out[i], v);
+                    if constexpr (cache_eight(S))
+                        if (key_scale[i]) {
+                            *key_scale[i] = (uint8_t)kb;
+                            *value_scale[i] = (uint8_t)vb;
+                        }
+                }
+            } else if (state[i] >= 0) {
+                Piece<kRow> k, v;
+                widen_piece<S, T>(key_in[i], key_byte[i], k);
+                widen_piece<S, T>(value_in[i], value_byte[i], v);
+                put_piece(key_out[i], k);
+                put_piece(value_out[i], v);
             }
         }
     }
