@@ -145,8 +145,11 @@ __device__ __forceinline__ uint32_t narrow_piece(const Piece<kIn>& in, Piece<kOu
                     __nv_cvt_float2_to_fp8x2(make_float2(y.x * inverse, y.y * inverse), __NV_SATFINITE, __NV_E4M3);
                 out.w[h] = lo | (hi << 16);
             } else {
-                const uint32_t a = __float2int_rn(x.x * inverse), b = __float2int_rn(x.y * inverse);
-                const uint32_t c = __float2int_rn(y.x * inverse), d = __float2int_rn(y.y * inverse);
+                // 1.5 2^23 + x rounds x to an integer, ties to even, in the low
+                // bits; the product is exact
+                const float magic = 12582912.f;
+                const uint32_t a = __float_as_uint(fmaf(x.x, inverse, magic)), b = __float_as_uint(fmaf(x.y, inverse, magic));
+                const uint32_t c = __float_as_uint(fmaf(y.x, inverse, magic)), d = __float_as_uint(fmaf(y.y, inverse, magic));
                 out.w[h] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
             }
         }

@@ -79,7 +79,11 @@ __device__ __forceinline__ float2 cache_pair(uint32_t bits) {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)bits, __NV_E4M3);
         return __half22float2(__half2(h));
     } else {
-        return make_float2((float)(int8_t)(bits & 0xff), (float)(int8_t)((bits >> 8) & 0xff));
+        // 2^23 + (x + 128) has x + 128 in its low mantissa bits: no conversion,
+        // of which an SM does 16 a cycle
+        const uint32_t u = bits ^ 0x8080u;
+        return make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7550)) - 8388736.f,
+                           __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7551)) - 8388736.f);
     }
 }
 
