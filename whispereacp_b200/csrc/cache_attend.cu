@@ -191,25 +191,6 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t address) 
                  : "memory");
 }
 
-// Bytes {i0, i1} of four held 8-bit values as two fp16, exact.
-template <int S>
-__device__ __forceinline__ void widen4(uint32_t bytes, bool interleaved, uint32_t& lo, uint32_t& hi) {
-    if constexpr (S == kCacheE4m3) {
-        const uint32_t b = interleaved ? __byte_perm(bytes, 0, 0x3120) : bytes;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)(b & 0xffffu)));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(b >> 16)));
-    } else {
-        // 1024 + (x + 128) has x + 128 in its low mantissa bits
-        const uint32_t u = bytes ^ 0x80808080u;
-        lo = __byte_perm(u, 0x64646464u, interleaved ? 0x4240 : 0x4140);
-        hi = __byte_perm(u, 0x64646464u, interleaved ? 0x4341 : 0x4342);
-        const __half2 base = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-        __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), base), b = __hsub2(*reinterpret_cast<__half2*>(&hi), base);
-        lo = *reinterpret_cast<uint32_t*>(&a);
-        hi = *reinterpret_cast<uint32_t*>(&b);
-    }
-}
-
 // The byte offset of 16-byte piece c of row r in a swizzled box of `span`
 // byte rows: the copy engine's 128- or 64-byte pattern.
 template <int kSpan>
@@ -410,7 +391,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         CutItem cut{};
         const long long first = begin - p.unit;  // the item's first unit
         if (begin < end && p.unit > 0 && first >= begin - per)
-            cut = {(int)((first + p.units - 1) / per - blockIdx.x) + 2, p.s, p.head, p.tile};
+            cut = {(int)((first + p.units - 1) / per - blockIdx.x) + 2, p.s, p.head, p.tile, p.q, 0};
         cut_items(a.workspace)[blockIdx.x] = cut;
     }
     __syncthreads();

@@ -46,7 +46,7 @@ struct CacheAttendShape {
 
 // What a kernel leaves to be joined: its workspace, its CTAs, and the rows of
 // its items.  The join takes a slice of an item's rows a block.
-constexpr int kJoinRows = 4, kJoinSlice = 16;
+constexpr int kJoinRows = 8, kJoinSlice = 8;
 struct CutPart {
     unsigned char* workspace;
     int grid, rows;

@@ -454,13 +454,29 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
         for (int i = 0; i < kMine; ++i) {
             const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
             if (piece >= kPieces) break;
-            const float by = cache_scale(t.scale[i]);
             const uint32_t in[4] = {t.raw[i].x, t.raw[i].y, t.raw[i].z, t.raw[i].w};
             uint32_t out[8];
+            if (std::is_same<T, __half>::value && t.scale[i] - 113u < 30u) {
+                // 2^-14 .. 2^15 is a number of fp16's: the product rounds as
+                // the float's way does
+                const __half2 by = __half2(__ushort_as_half((unsigned short)((t.scale[i] - 112u) << 10)),
+                                           __ushort_as_half((unsigned short)((t.scale[i] - 112u) << 10)));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float2 f = cache_pair<S>((in[e / 2] >> (16 * (e & 1))) & 0xffffu);
-                out[e] = Half16<T>::pack2(f.x * by, f.y * by);
+                for (int h = 0; h < 4; ++h) {
+                    widen4<S>(in[h], false, out[2 * h], out[2 * h + 1]);
+#pragma unroll
+                    for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                        const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&out[e]), by);
+                        out[e] = *reinterpret_cast<const uint32_t*>(&x);
+                    }
+                }
+            } else {
+                const float by = cache_scale(t.scale[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 f = cache_pair<S>((in[e / 2] >> (16 * (e & 1))) & 0xffffu);
+                    out[e] = Half16<T>::pack2(f.x * by, f.y * by);
+                }
             }
             unsigned char* to = tile + (c / 4) * kHalfBytes + key * 128;
             const int at = (c % 4) * 2;
@@ -904,7 +920,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
         CutItem cut{};
         const long long first = begin - p.block;  // the item's first block
         if (begin < end && p.block > 0 && first >= begin - per)
-            cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.item};
+            cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.item, p.q, 0};
         cut_items(a.workspace)[blockIdx.x] = cut;
     }
     tmem_fence_before();

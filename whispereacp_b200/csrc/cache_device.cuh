@@ -99,6 +99,26 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// Four held 8-bit values, unscaled, as two pairs of fp16, exact: 0 1 and 2 3, or
+// (interleaved) 0 2 and 1 3.
+template <int S>
+__device__ __forceinline__ void widen4(uint32_t bytes, bool interleaved, uint32_t& lo, uint32_t& hi) {
+    if constexpr (S == kCacheE4m3) {
+        const uint32_t b = interleaved ? __byte_perm(bytes, 0, 0x3120) : bytes;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)(b & 0xffffu)));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(b >> 16)));
+    } else {
+        // 1024 + (x + 128) has x + 128 in its low mantissa bits
+        const uint32_t u = bytes ^ 0x80808080u;
+        lo = __byte_perm(u, 0x64646464u, interleaved ? 0x4240 : 0x4140);
+        hi = __byte_perm(u, 0x64646464u, interleaved ? 0x4341 : 0x4342);
+        const __half2 base = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+        __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), base), b = __hsub2(*reinterpret_cast<__half2*>(&hi), base);
+        lo = *reinterpret_cast<uint32_t*>(&a);
+        hi = *reinterpret_cast<uint32_t*>(&b);
+    }
+}
+
 // ------------------------------------------------- a row that is done alone
 
 // One row of one query head by one warp, key by key: o = sum_j p_j v_j / sum_j

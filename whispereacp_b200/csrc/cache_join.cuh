@@ -16,6 +16,8 @@ namespace {
 struct CutItem {
     int parts;  // partial results of the item, if this CTA's is the second; else 0
     int sequence, head, tile;
+    CacheSequence q;
+    int pad;
 };
 // A partial result: o, then m, then sum.
 template <int D>
@@ -57,12 +59,13 @@ __global__ void __launch_bounds__(kThreads)
     const int block = (int)blockIdx.x - (late ? first.blocks() : 0);
     const int c = block / part_of.slices() + 1, slice = block % part_of.slices();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 record = *reinterpret_cast<const int4*>(cut_items(part_of.workspace) + c);
-    const CutItem cut = {record.x, record.y, record.z, record.w};
+    const CutItem* record = cut_items(part_of.workspace) + c;
+    const int4 head_of = *reinterpret_cast<const int4*>(record), rest = *(reinterpret_cast<const int4*>(record) + 1);
+    const CutItem cut = {head_of.x, head_of.y, head_of.z, head_of.w, {rest.x, rest.y, rest.z}, 0};
     if (cut.parts == 0) return;
     const float* partials = cut_partials(part_of.workspace, part_of.grid);
     const int tile_rows = part_of.rows, floats = partial_floats<D>(tile_rows);
-    const CacheSequence q = cache_sequence(a.batch, cut.sequence);
+    const CacheSequence q = cut.q;
     const int all_rows = (int)min((long long)tile_rows, (long long)q.rows * a.group - (long long)cut.tile * tile_rows);
     const int end = min(all_rows, (slice + 1) * kJoinSlice);
     for (int base = slice * kJoinSlice; base < end; base += kJoinRows) {
@@ -135,14 +138,14 @@ void launch_join(const CacheAttendArgs& a, const CutPart& first, const CutPart& 
     const bool many = first.grid > 8 * items;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(blocks);
-    config.blockDim = dim3(many ? 512 : 128);
+    config.blockDim = dim3(many ? 512 : 256);
     config.stream = stream;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, many ? cache_join_kernel<T, S, D, 512> : cache_join_kernel<T, S, D, 128>, a,
+    CUDA_CHECK(cudaLaunchKernelEx(&config, many ? cache_join_kernel<T, S, D, 512> : cache_join_kernel<T, S, D, 256>, a,
                                   first, second));
 }
 
