@@ -56,9 +56,13 @@ struct ChunkLayout {
     static constexpr int out_column = tiles * 128;
     static constexpr int halves = D / 64;
     static constexpr int tile_bytes = halves * kHalfBytes;  // of Q_t, or of a block's keys or values
-    static constexpr int stages = D == 64 && tiles == 2 ? 8 : 5;
+    static constexpr int stages = D == 64 && tiles == 2 ? 8 : cache_eight(S) ? 3 : 5;
     static constexpr int ring_at = tiles * tile_bytes;
-    static constexpr int bar_at = ring_at + stages * tile_bytes;
+    // 8-bit storage: blocks as they are held, and their scale bytes.
+    static constexpr int depth = cache_eight(S) ? 4 : 0;
+    static constexpr int held_bytes = kBlockKeys * (D + 1) + 16;  // and how many of the keys are seen
+    static constexpr int held_at = ring_at + stages * tile_bytes;
+    static constexpr int bar_at = held_at + depth * held_bytes;
     // full, empty; per tile: scores, P's halves, first half, queries, O; done
     static constexpr int bars = 2 * stages + 6 * tiles + 1;
     static constexpr int bytes = bar_at + bars * 8 + 16;
@@ -407,77 +411,118 @@ __device__ void chunk_copy(const CacheAttendArgs& a, const CacheMaps& maps, unsi
         }
 }
 
-// 8-bit caches: three warps read the blocks themselves and write them widened
-// to the queries' type, each value times its scale (a power of two: exact in
-// bf16, and in fp16 wherever fp16 holds the result).
+// 16 held 8-bit values times their scale (byte `scale`), as 16-bit values.
+template <typename T, int S>
+__device__ __forceinline__ void widen_piece(const uint4& raw, uint32_t scale, uint32_t (&out)[8]) {
+    const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+    if (std::is_same<T, __half>::value && scale - 113u < 30u) {
+        // 2^-14 .. 2^15 is a number of fp16's: the product rounds as the
+        // float's way does
+        const unsigned short bits = (unsigned short)((scale - 112u) << 10);
+        const __half2 by = __half2(__ushort_as_half(bits), __ushort_as_half(bits));
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            widen4<S>(in[h], false, out[2 * h], out[2 * h + 1]);
+#pragma unroll
+            for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&out[e]), by);
+                out[e] = *reinterpret_cast<const uint32_t*>(&x);
+            }
+        }
+    } else {
+        const float by = cache_scale(scale);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float2 f = cache_pair<S>((in[e / 2] >> (16 * (e & 1))) & 0xffffu);
+            out[e] = Half16<T>::pack2(f.x * by, f.y * by);
+        }
+    }
+}
+
+// 8-bit caches: three warps bring the blocks in as they are held, four tiles
+// (keys or values of a block) deep, and write them into the ring widened to the
+// queries' type, each value times its scale (a power of two: exact in bf16, and
+// in fp16 wherever fp16 holds the result).
 template <typename T, int S, int D>
 __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, volatile int* abort,
                             ChunkPlace p, long long begin, long long end, int warp, int lane) {
     using Layout = ChunkLayout<S, D>;
     constexpr int kThreads = 32 * Layout::copy_warps;
     constexpr int kPieces = kBlockKeys * D / 16;  // 16 values each
-    constexpr int kMine = (kPieces + kThreads - 1) / kThreads;
+    constexpr int kDepth = Layout::depth;
     const int me = warp * 32 + lane;
-    int stage = 0, n = 0;
-    uint32_t parity = 1;
-    // A tile, keys or values of a block: this thread's pieces and their scales.
-    // The next tile's are on their way while this one's are written.
-    struct Tile {
-        uint4 raw[kMine];
-        uint8_t scale[kMine];
-    };
-    const auto fetch = [&](const ChunkPlace& p, int j, bool values, int seen, Tile& t) {
-        const unsigned char* pool = values ? a.cache.values : a.cache.keys;
-        const uint8_t* scales = values ? a.cache.value_scales : a.cache.key_scales;
-        // A lane a page, of 16 rows at least.
-        const int pages = max(1, kBlockKeys >> a.cache.page_shift);
-        const int first = j * kBlockKeys + (min(lane, pages - 1) << a.cache.page_shift);
-        const int entry = first < seen ? cache_page(a.cache, a.batch, p.s, first) : -1;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
-            const int position = j * kBlockKeys + key;
-            const int page = __shfl_sync(0xffffffffu, entry, min(key >> a.cache.page_shift, pages - 1));
-            t.raw[i] = make_uint4(0, 0, 0, 0);
-            t.scale[i] = 0;
-            if (piece < kPieces && position < seen && page >= 0) {
+    int todo = (int)(end - begin);
+    int last = take_item(p, todo);
+    if (last <= 0) return;
+    int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows), j = p.block;
+    bool values = false, more = true;  // of the tile to ask for; there is one
+    int asked = 0;
+    // Asks for the next tile; what is not there, or not seen, comes as zeros.
+    const auto ask = [&] {
+        if (more) {
+            unsigned char* held = smem + Layout::held_at + (asked % kDepth) * Layout::held_bytes;
+            const unsigned char* pool = values ? a.cache.values : a.cache.keys;
+            const uint8_t* scales = values ? a.cache.value_scales : a.cache.key_scales;
+            // A lane a page, of 16 rows at least.
+            const int pages = max(1, kBlockKeys >> a.cache.page_shift);
+            const int first = j * kBlockKeys + (min(lane, pages - 1) << a.cache.page_shift);
+            const int entry = first < seen ? cache_page(a.cache, a.batch, p.s, first) : -1;
+            const auto copy16 = [&](unsigned char* to, const void* from, bool there) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_address(to)), "l"(from),
+                             "r"(there ? 16 : 0)
+                             : "memory");
+            };
+            if (me == 0) *reinterpret_cast<int*>(held + kPieces * 16 + kBlockKeys) = seen - j * kBlockKeys;
+#pragma unroll 2
+            for (int i = 0; i < (kPieces + 8 + kThreads - 1) / kThreads; ++i) {
+                const int piece = me + i * kThreads;
+                const bool scale = piece >= kPieces;  // 16 keys' scale bytes
+                const int key = min(scale ? (piece - kPieces) * 16 : piece / (D / 16), kBlockKeys - 1);
+                const int position = j * kBlockKeys + key;
+                const int page = __shfl_sync(0xffffffffu, entry, min(key >> a.cache.page_shift, pages - 1));
+                if (piece >= kPieces + 8) continue;
+                const bool there = position < seen && page >= 0;
                 const int slot = position & ((1 << a.cache.page_shift) - 1);
-                t.raw[i] = load_stream(pool + cache_offset(a.cache, page, p.head, slot) + c * 16);
-                t.scale[i] = __ldg(scales + cache_scale_index(a.cache, page, p.head, slot));
+                if (scale)
+                    copy16(held + kPieces * 16 + key,
+                           there ? scales + cache_scale_index(a.cache, page, p.head, slot) : scales, there);
+                else
+                    copy16(held + piece * 16,
+                           there ? pool + cache_offset(a.cache, page, p.head, slot) + (piece % (D / 16)) * 16 : pool, there);
+            }
+            ++asked;
+            // keys of block 0, its values, keys of block 1, ...
+            values = !values;
+            if (!values && ++j >= last) {
+                more = todo > 0;
+                if (more) {
+                    next_item<Layout::rows>(p, a);
+                    last = take_item(p, todo);
+                    seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
+                    j = p.block;
+                }
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const auto write = [&](const Tile& t) {
+    for (int i = 0; i < kDepth - 1; ++i) ask();
+    int stage = 0;
+    uint32_t parity = 1;
+    for (int n = 0; n < asked; ++n) {
+        // This tile's copies are in, everybody's, and the last tile's place is
+        // read.
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+        ask();
         if (n >= Layout::stages) cache_wait(bar.empty + stage, parity, abort, a.status, kWaitSlot);
+        const unsigned char* held = smem + Layout::held_at + (n % kDepth) * Layout::held_bytes;
+        const int keys = *reinterpret_cast<const int*>(held + kPieces * 16 + kBlockKeys);  // seen; the others are zeros
         unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const int piece = me + i * kThreads, key = piece / (D / 16), c = piece % (D / 16);
-            if (piece >= kPieces) break;
-            const uint32_t in[4] = {t.raw[i].x, t.raw[i].y, t.raw[i].z, t.raw[i].w};
+#pragma unroll 2
+        for (int piece = me; piece < kPieces; piece += kThreads) {
+            const int key = piece / (D / 16), c = piece % (D / 16);
             uint32_t out[8];
-            if (std::is_same<T, __half>::value && t.scale[i] - 113u < 30u) {
-                // 2^-14 .. 2^15 is a number of fp16's: the product rounds as
-                // the float's way does
-                const __half2 by = __half2(__ushort_as_half((unsigned short)((t.scale[i] - 112u) << 10)),
-                                           __ushort_as_half((unsigned short)((t.scale[i] - 112u) << 10)));
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    widen4<S>(in[h], false, out[2 * h], out[2 * h + 1]);
-#pragma unroll
-                    for (int e = 2 * h; e < 2 * h + 2; ++e) {
-                        const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&out[e]), by);
-                        out[e] = *reinterpret_cast<const uint32_t*>(&x);
-                    }
-                }
-            } else {
-                const float by = cache_scale(t.scale[i]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float2 f = cache_pair<S>((in[e / 2] >> (16 * (e & 1))) & 0xffffu);
-                    out[e] = Half16<T>::pack2(f.x * by, f.y * by);
-                }
-            }
+            widen_piece<T, S>(*reinterpret_cast<const uint4*>(held + piece * 16), key < keys ? held[kPieces * 16 + key] : 0u, out);
             unsigned char* to = tile + (c / 4) * kHalfBytes + key * 128;
             const int at = (c % 4) * 2;
             *reinterpret_cast<uint4*>(to + ((at ^ (key & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
@@ -486,34 +531,10 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
         cache_proxy_fence();
         __syncwarp();
         if (lane == 0) cache_arrive(bar.full + stage);
-        ++n;
         if (++stage == Layout::stages) {
             stage = 0;
             parity ^= 1;
         }
-    };
-    Tile keys, values;
-    int todo = (int)(end - begin);
-    int last = take_item(p, todo);
-    if (last <= 0) return;
-    int seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
-    fetch(p, p.block, false, seen, keys);
-    for (int j = p.block;;) {
-        fetch(p, j, true, seen, values);
-        write(keys);
-        bool more = true;
-        if (++j >= last) {
-            more = todo > 0;
-            if (more) {
-                next_item<Layout::rows>(p, a);
-                last = take_item(p, todo);
-                seen = chunk_seen(p.q, a, (p.item + 1) * Layout::rows);
-                j = p.block;
-            }
-        }
-        if (more) fetch(p, j, false, seen, keys);
-        write(values);
-        if (!more) return;
     }
 }
 
