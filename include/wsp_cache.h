@@ -91,8 +91,11 @@ int wsp_cache_get_memory(const wsp_cache* cache, wsp_cache_memory* memory);
  * starts must not decrease, starts[0] may be any row, and rows before
  * starts[0] or from starts[sequences] on belong to no sequence and are left
  * alone.  A page id outside the pool, and a position outside the table, is
- * no page: appending there does nothing, and its rows read as zeros.
- * max_rows is a bound of n, the same or larger; it chooses kernels only.
+ * no page: appending there does nothing, and its rows read as zeros.  In the
+ * attention rows of such pages take part as zeros, positions outside the
+ * table do not take part, and a sequence whose rows lie outside the call's
+ * arrays has none.  max_rows is a bound of n, the same or larger; it chooses
+ * kernels only.
  */
 typedef struct wsp_cache_batch {
     const int32_t* table;

@@ -50,8 +50,10 @@ def quantised(x, storage):
 
 
 def held_rows(cache, table_row, length):
-    """[length, heads, width] of one sequence in 64 bits; rows of no page are zeros."""
+    """[length, heads, width] of one sequence in 64 bits, no more than its table
+    has places for; rows of no page are zeros."""
     import torch
+    length = min(length, len(table_row) * cache.page_rows)
     out = torch.zeros(length, cache.heads, cache.head_width, dtype=torch.float64, device="cuda")
     k, v = out, out.clone()
     columns = table_row.tolist()
@@ -409,9 +411,10 @@ def test_large_scores_and_large_values(storage, dtype):
         check_attend(cache, batch, starts, q, out, lse, 0.125, causal)
 
 
-def test_rows_of_no_page_take_part_as_zeros():
+def test_rows_of_no_page_take_part_as_zeros_and_those_outside_the_table_do_not():
     cache = make_cache("float16", 20, 2, 16, 64, 47)
     for new in ([1, 1], [140, 2]):
+        # 150 rows, of which the table has places for 144
         batch, starts = make_batch([150, 70], new, 16, 20, 48, columns=9)
         batch.page_table[0, 3] = -1
         batch.page_table[1, 1] = 20
@@ -630,3 +633,132 @@ def test_windows_at_their_own_tokens_follow_the_decoder():
         assert np.isfinite(mine).all()
         assert float(np.abs(mine - np.asarray(truth)).max()) <= 2e-2
         assert float(np.abs(mine - lockstep).max()) <= 4e-2
+
+
+# ------------------------------------------------------- more of the range
+
+@pytest.mark.parametrize("storage,dtype,width", [("float16", "float16", 64), ("int8", "bfloat16", 64), ("bfloat16", "bfloat16", 128)])
+def test_many_sequences_of_every_kind(storage, dtype, width):
+    """90 sequences -- more than one round of a warp's lanes -- with no rows,
+    single ones, 2 to 16 (tiles of 8 and of 16), and chunks, in one batch."""
+    rng = np.random.default_rng(5)
+    for most in (1, 3, 16, 150):
+        new = [int(rng.integers(0, most + 1)) for _ in range(90)]
+        new[17], new[88] = most, most
+        lengths = [n + int(rng.integers(0, 300)) for n in new]
+        lengths[3], new[3] = 0, 0
+        pages = sum(-(-n // 32) for n in lengths) + 3
+        cache = make_cache(storage, pages, 2, 32, width, 6)
+        batch, starts = make_batch(lengths, new, 32, pages, 7)
+        q = queries(int(starts[-1]), 4, width, dtype, 8)
+        for causal in (True, False):
+            out, lse = cache.attend(batch, q, causal=causal, return_lse=True)
+            check_attend(cache, batch, starts, q, out, lse, 1 / math.sqrt(width), causal)
+
+
+@pytest.mark.parametrize("storage,source", [("float16", "float16"), ("bfloat16", "float32"), ("int8", "bfloat16"), ("float8_e4m3fn", "float16")])
+def test_append_and_read_of_many_rows(storage, source):
+    """Thousands of rows: blocks of several rows, ragged."""
+    import torch
+    rng = np.random.default_rng(11)
+    lengths = [int(n) for n in rng.integers(1, 260, 60)]
+    pages = sum(-(-n // 16) for n in lengths) + 2
+    cache = make_cache(storage, pages, 3, 16, 64, 12)
+    batch, starts = make_batch(lengths, lengths, 16, pages, 13)
+    k, v = (queries(int(starts[-1]), 3, 64, source, 14 + i) for i in range(2))
+    cache.append(batch, k, v)
+    a, b = cache.read(batch, dtype=torch.float32)
+    for x, got in ((k, a), (v, b)):
+        want = quantised(x, storage)[0] if storage in EIGHT else x.to(dt(storage)).double()
+        assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("storage,dtype", PAIRS)
+@pytest.mark.parametrize("rows", [([33, 200, 5], [1, 1, 1]), ([200, 300], [90, 130])])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_a_scale_below_or_at_zero(storage, dtype, rows, scale):
+    """At scale 0 every seen key weighs the same."""
+    lengths, new = rows
+    pages = sum(-(-n // 16) for n in lengths) + 2
+    cache = make_cache(storage, pages, 2, 16, 64, 21)
+    batch, starts = make_batch(lengths, new, 16, pages, 22)
+    q = queries(int(starts[-1]), 2, 64, dtype, 23)
+    out, lse = cache.attend(batch, q, scale=scale, return_lse=True)
+    check_attend(cache, batch, starts, q, out, lse, float(np.float32(scale)), True)
+
+
+def test_batches_that_ask_for_nothing_or_for_the_impossible():
+    """No sequences, no rows, no columns, and rows outside the arrays."""
+    import torch
+    from whispereacp_b200 import CacheBatch
+    cache = make_cache("float16", 8, 2, 16, 64, 31)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q = queries(6, 2, 64, "float16", 32)
+    target = torch.full_like(q, 9.0)
+    none = CacheBatch(torch.zeros(0, 4, **i32), torch.zeros(0, **i32), torch.zeros(1, **i32), max_rows=0)
+    cache.append(none, q, q)
+    cache.attend(none, q, out=target)
+    cache.read(none, target, target.clone())
+    assert bool((target == 9).all())
+    # a table without columns: no keys at all
+    bare = CacheBatch(torch.zeros(2, 0, **i32), torch.tensor([30, 4], **i32), torch.tensor([0, 1, 6], **i32), max_rows=5)
+    cache.append(bare, q, q)
+    out, lse = cache.attend(bare, q, return_lse=True)
+    assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
+    # starts past the arrays' rows: the sequences inside are done, that one is not
+    table = torch.tensor([[0, 1], [2, 3]], **i32)
+    past = CacheBatch(table, torch.tensor([20, 30], **i32), torch.tensor([0, 4, 90], **i32), max_rows=86)
+    target.fill_(9.0)
+    cache.attend(past, q, out=target)
+    k, v = held_rows(cache, table[0], 20)
+    o, _, tol, _ = expected(q[:4], k, v, 0.125, True, 16)
+    assert bool(((target[:4].double() - o).abs() <= tol).all()) and bool((target[4:] == 9).all())
+    with pytest.raises(ValueError, match="a batch of 1 sequences"):
+        CacheBatch(table, torch.tensor([20], **i32), torch.tensor([0, 4], **i32))
+
+
+def test_refusals_of_the_binding():
+    import torch
+    from whispereacp_b200 import CacheBatch, ModelError, PagedCache
+    cache = make_cache("float16", 8, 2, 16, 64, 41)
+    batch, _ = make_batch([20], [2], 16, 8, 42)
+    q = queries(2, 4, 64, "float16", 43)
+    with pytest.raises(ModelError, match="queries must be"):
+        cache.attend(batch, q[0])
+    with pytest.raises(ModelError, match="queries must be"):
+        cache.attend(batch, queries(2, 4, 128, "float16", 43))
+    with pytest.raises(ModelError, match="multiple"):
+        cache.attend(batch, q[:, :3])
+    with pytest.raises(ModelError, match="have its type"):
+        cache.attend(batch, q.bfloat16())
+    with pytest.raises(ModelError, match="16-bit"):
+        cache.attend(batch, q.float())
+    with pytest.raises(ValueError, match="contiguous in the last"):
+        cache.attend(batch, q.transpose(1, 2).contiguous().transpose(1, 2))
+    with pytest.raises(ValueError, match="16-byte"):
+        cache.attend(batch, torch.zeros(2 * 4 * 64 + 1, dtype=torch.float16, device="cuda")[1:].view(2, 4, 64))
+    with pytest.raises(ValueError, match="must be on"):
+        cache.attend(batch, q.cpu())
+    with pytest.raises(ValueError, match="lse"):
+        cache.attend(batch, q, lse=torch.zeros(2, 3, device="cuda"))
+    with pytest.raises(ValueError, match="finite"):
+        cache.attend(batch, q, scale=float("nan"))
+    with pytest.raises(ValueError, match="together"):
+        cache.read(batch, keys=q)
+    with pytest.raises(ValueError, match="rows are"):
+        cache.append(batch, q[:, :2].double(), q[:, :2].double())
+    with pytest.raises(ValueError, match="one dtype"):
+        cache.append(batch, q[:, :2], q[:, :2].float())
+    with pytest.raises(ValueError, match="alike"):
+        PagedCache(cache.keys, cache.values.float())
+    with pytest.raises(ValueError, match="no scales"):
+        PagedCache(cache.keys, cache.values, torch.zeros(8, 2, 16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(ValueError, match="scale bytes"):
+        PagedCache(cache.keys.to(torch.int8), cache.values.to(torch.int8))
+    with pytest.raises(ModelError, match="64 or 128"):
+        PagedCache.allocate(4, 2, 16, 96)
+    with pytest.raises(ModelError, match="a page has"):
+        PagedCache.allocate(4, 2, 24, 64)
+    cache.close()
+    with pytest.raises(ValueError, match="closed"):
+        cache.attend(batch, q)

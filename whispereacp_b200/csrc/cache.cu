@@ -202,9 +202,9 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_c
         if (lane == 0) {
             long long at = -2, si = 0;
             if (r < a.rows && s < a.batch.sequences) {
-                const CacheSequence q = cache_sequence(a.batch, s);
+                const CacheSequence q = cache_sequence(a.cache, a.batch, s);
                 if (r >= q.first) {
-                    const int position = q.length - q.rows + (r - q.first);
+                    const int position = q.before + (r - q.first);
                     const int page = cache_page(a.cache, a.batch, s, position);
                     const int slot = position & ((1 << a.cache.page_shift) - 1);
                     at = page < 0 ? -1 : cache_offset(a.cache, page, 0, slot);

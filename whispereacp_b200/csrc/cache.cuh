@@ -30,16 +30,18 @@ struct CacheBatchView {
     int columns, sequences;
 };
 
-// One sequence of a batch: its first new row, how many it has, and how many
-// rows it holds.
+// One sequence of a batch: its first new row and how many it has, the position
+// of the first, and the rows it holds that the table has places for.
 struct CacheSequence {
-    int first, rows, length;
+    int first, rows, before, length;
 };
-__device__ __forceinline__ CacheSequence cache_sequence(const CacheBatchView& b, int s) {
+__device__ __forceinline__ CacheSequence cache_sequence(const CacheView& c, const CacheBatchView& b, int s) {
     CacheSequence q;
     q.first = b.starts[s];
     q.rows = b.starts[s + 1] - q.first;
-    q.length = b.lengths[s];
+    const int length = b.lengths[s];
+    q.before = length - q.rows;
+    q.length = (int)max(0ll, min((long long)length, (long long)b.columns << c.page_shift));
     return q;
 }
 

@@ -111,11 +111,11 @@ template <int kKeys, int kRows>
 __device__ __forceinline__ long long all_units(const CacheAttendArgs& a, int lane, FirstSequences& kept) {
     kept = FirstSequences{};
     if (lane < a.batch.sequences) {
-        kept.q = cache_sequence(a.batch, lane);
+        kept.q = attend_sequence(a, lane);
         kept.units = sequence_units<kKeys, kRows>(kept.q, a);
     }
     long long sum = kept.units;
-    for (int s = lane + 32; s < a.batch.sequences; s += 32) sum += sequence_units<kKeys, kRows>(cache_sequence(a.batch, s), a);
+    for (int s = lane + 32; s < a.batch.sequences; s += 32) sum += sequence_units<kKeys, kRows>(attend_sequence(a, s), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
@@ -132,7 +132,7 @@ __device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u
         if (base > 0) {
             mine = 0;
             if (base + lane < a.batch.sequences) {
-                q = cache_sequence(a.batch, base + lane);
+                q = attend_sequence(a, base + lane);
                 mine = sequence_units<kKeys, kRows>(q, a);
             }
         }
@@ -144,6 +144,7 @@ __device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u
             p.s = base + at;
             p.q.first = __shfl_sync(0xffffffffu, q.first, at);
             p.q.rows = __shfl_sync(0xffffffffu, q.rows, at);
+            p.q.before = __shfl_sync(0xffffffffu, q.before, at);
             p.q.length = __shfl_sync(0xffffffffu, q.length, at);
             p.units = item_units<kKeys>(p.q.length);
             p.tiles = item_tiles<kRows>(p.q, a);
@@ -169,7 +170,7 @@ __device__ __forceinline__ void next_item(Place& p, const CacheAttendArgs& a) {
     if (++p.head < a.cache.heads) return;
     p.head = 0;
     while (++p.s < a.batch.sequences) {
-        p.q = cache_sequence(a.batch, p.s);
+        p.q = attend_sequence(a, p.s);
         p.tiles = item_tiles<kRows>(p.q, a);
         if (p.tiles > 0) break;
     }
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         CutItem cut{};
         const long long first = begin - p.unit;  // the item's first unit
         if (begin < end && p.unit > 0 && first >= begin - per)
-            cut = {(int)((first + p.units - 1) / per - blockIdx.x) + 2, p.s, p.head, p.tile, p.q, 0};
+            cut = {(int)((first + p.units - 1) / per - blockIdx.x) + 2, p.s, p.head, p.tile, p.q};
         cut_items(a.workspace)[blockIdx.x] = cut;
     }
     __syncthreads();
@@ -754,7 +755,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                 for (int row = warp; row < kRows; row += kWorkers)
                     if (again >> row & 1) {
                         const TileRow r = tile_row(a, p.q, p.head, p.tile * kRows + row);
-                        attend_row<T, S, D>(a, p.s, p.q.first, p.q.rows, p.q.length, r.token, r.head);
+                        attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, r.token, r.head);
                     }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (threadIdx.x == 0) *redo = 0;

@@ -87,9 +87,9 @@ __device__ __forceinline__ int chunk_items(const CacheSequence& q, const CacheAt
 // Keys that any of the first `rows` packed rows sees; rows * group of a call
 // fit 31 bits.
 __device__ __forceinline__ int chunk_seen(const CacheSequence& q, const CacheAttendArgs& a, int rows) {
-    if (!a.causal) return max(q.length, 0);
+    if (!a.causal) return q.length;
     const int token = min((rows - 1) / a.group, q.rows - 1);
-    return max(0, min(q.length - q.rows + token + 1, q.length));
+    return max(0, min(q.before + token + 1, q.length));
 }
 template <int kRows>
 __device__ __forceinline__ int chunk_blocks(const CacheSequence& q, const CacheAttendArgs& a, int item) {
@@ -122,11 +122,11 @@ template <int kRows>
 __device__ __forceinline__ long long all_blocks(const CacheAttendArgs& a, int lane, FirstSequences& kept) {
     kept = FirstSequences{};
     if (lane < a.batch.sequences) {
-        kept.q = cache_sequence(a.batch, lane);
+        kept.q = attend_sequence(a, lane);
         kept.blocks = chunk_units<kRows>(kept.q, a);
     }
     long long sum = kept.blocks;
-    for (int s = lane + 32; s < a.batch.sequences; s += 32) sum += chunk_units<kRows>(cache_sequence(a.batch, s), a);
+    for (int s = lane + 32; s < a.batch.sequences; s += 32) sum += chunk_units<kRows>(attend_sequence(a, s), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
@@ -144,7 +144,7 @@ __device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long 
         if (base > 0) {
             mine = 0;
             if (base + lane < a.batch.sequences) {
-                q = cache_sequence(a.batch, base + lane);
+                q = attend_sequence(a, base + lane);
                 mine = chunk_units<kRows>(q, a);
             }
         }
@@ -156,6 +156,7 @@ __device__ __forceinline__ ChunkPlace find_block(const CacheAttendArgs& a, long 
             p.s = base + at;
             p.q.first = __shfl_sync(0xffffffffu, q.first, at);
             p.q.rows = __shfl_sync(0xffffffffu, q.rows, at);
+            p.q.before = __shfl_sync(0xffffffffu, q.before, at);
             p.q.length = __shfl_sync(0xffffffffu, q.length, at);
             p.items = chunk_items<kRows>(p.q, a);
             const long long all = __shfl_sync(0xffffffffu, mine, at);  // of every head
@@ -191,7 +192,7 @@ __device__ __forceinline__ void next_item(ChunkPlace& p, const CacheAttendArgs& 
         if (++p.head >= a.cache.heads) {
             p.head = 0;
             while (++p.s < a.batch.sequences) {
-                p.q = cache_sequence(a.batch, p.s);
+                p.q = attend_sequence(a, p.s);
                 p.items = chunk_items<kRows>(p.q, a);
                 if (p.items > 0) break;
             }
@@ -884,7 +885,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             again &= again - 1;
             const int token = __shfl_sync(0xffffffffu, r.token, i), head = __shfl_sync(0xffffffffu, r.head, i);
             __syncwarp();
-            attend_row<T, S, D>(a, p.s, p.q.first, p.q.rows, p.q.length, token, head);
+            attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, token, head);
         }
         tmem_fence_before();  // this tile's reads, before the products that the next arrival lets run
         if (last_n == 0) break;
@@ -941,7 +942,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
         CutItem cut{};
         const long long first = begin - p.block;  // the item's first block
         if (begin < end && p.block > 0 && first >= begin - per)
-            cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.item, p.q, 0};
+            cut = {(int)((first + p.blocks - 1) / per - blockIdx.x) + 2, p.s, p.head, p.item, p.q};
         cut_items(a.workspace)[blockIdx.x] = cut;
     }
     tmem_fence_before();

@@ -128,11 +128,11 @@ __device__ __forceinline__ void widen4(uint32_t bytes, bool interleaved, uint32_
 // the row NaN; such rows, which see fewer keys than the sequence holds, come
 // here.
 template <typename T, int S, int D>
-__device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int first, int rows, int length, int i,
+__device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int first, int before, int length, int i,
                                         int head) {
     constexpr int kPer = D / 32;  // a lane's elements
     const int lane = threadIdx.x & 31;
-    const int keys = a.causal ? min(length - rows + i + 1, length) : length;
+    const int keys = a.causal ? min(before + i + 1, length) : length;
     const long long row = (long long)first + i;
     const int kv = head / a.group;
     float qv[kPer], o[kPer];
@@ -188,6 +188,14 @@ __device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int fir
 
 // ------------------------------------------------------------ a tile's rows
 
+// A sequence as the attention takes it: none of its rows if any lies outside
+// the call's arrays.
+__device__ __forceinline__ CacheSequence attend_sequence(const CacheAttendArgs& a, int s) {
+    CacheSequence q = cache_sequence(a.cache, a.batch, s);
+    if (q.first < 0 || (long long)q.first + q.rows > a.rows) q.rows = 0;
+    return q;
+}
+
 // Packed row R of a sequence's n * group rows of one key head is token R /
 // group of query head R % group.
 struct TileRow {
@@ -198,9 +206,8 @@ __device__ __forceinline__ TileRow tile_row(const CacheAttendArgs& a, const Cach
     TileRow r;
     r.token = a.group == 1 ? packed : packed / a.group;
     r.head = kv * a.group + packed - r.token * a.group;
-    const long long row = (long long)q.first + r.token;
-    r.valid = r.token < q.rows && row >= 0 && row < a.rows;
-    r.seen = a.causal ? max(0, min(q.length - q.rows + r.token + 1, q.length)) : max(q.length, 0);
+    r.valid = r.token < q.rows;
+    r.seen = a.causal ? max(0, min(q.before + r.token + 1, q.length)) : q.length;
     return r;
 }
 

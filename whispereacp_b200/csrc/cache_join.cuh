@@ -17,7 +17,6 @@ struct CutItem {
     int parts;  // partial results of the item, if this CTA's is the second; else 0
     int sequence, head, tile;
     CacheSequence q;
-    int pad;
 };
 // A partial result: o, then m, then sum.
 template <int D>
@@ -61,7 +60,7 @@ __global__ void __launch_bounds__(kThreads)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const CutItem* record = cut_items(part_of.workspace) + c;
     const int4 head_of = *reinterpret_cast<const int4*>(record), rest = *(reinterpret_cast<const int4*>(record) + 1);
-    const CutItem cut = {head_of.x, head_of.y, head_of.z, head_of.w, {rest.x, rest.y, rest.z}, 0};
+    const CutItem cut = {head_of.x, head_of.y, head_of.z, head_of.w, {rest.x, rest.y, rest.z, rest.w}};
     if (cut.parts == 0) return;
     const float* partials = cut_partials(part_of.workspace, part_of.grid);
     const int tile_rows = part_of.rows, floats = partial_floats<D>(tile_rows);
@@ -123,7 +122,7 @@ __global__ void __launch_bounds__(kThreads)
         }
         if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
         if (__any_sync(0xffffffffu, !fine) && r.seen > 0 && (cache_eight(S) || r.seen < q.length))
-            attend_row<T, S, D>(a, cut.sequence, q.first, q.rows, q.length, r.token, r.head);
+            attend_row<T, S, D>(a, cut.sequence, q.first, q.before, q.length, r.token, r.head);
     }
 }
 
