@@ -81,6 +81,13 @@ class CacheBatch:
                               sequences, max_rows)
         self._ref = ctypes.byref(self._c)
         self.columns = page_table.shape[1]
+        self._rows = None
+
+    def rows(self) -> int:
+        """The rows of the calls' arrays, starts[-1]: asked of the device once."""
+        if self._rows is None:
+            self._rows = int(self.starts[-1])
+        return self._rows
 
 
 class PagedCache:
@@ -177,20 +184,24 @@ class PagedCache:
         starts, once, which waits for the device)."""
         if (keys is None) != (values is None):
             raise ValueError("keys and values to fill are given together")
+        handle = self._usable(batch)
         if keys is None:
             torch = _torch()
             if rows is None:
-                rows = getattr(batch, "_rows_held", None)
-                if rows is None:
-                    rows = batch._rows_held = int(batch.starts[-1])
-            dtype = dtype or (torch.float32 if self.eight else self.dtype)
+                rows = batch.rows()
+            if dtype is None:
+                dtype = torch.float32 if self.eight else self.dtype
+            code = _codes.get(dtype)
+            if code is None:
+                code = _row_type(dtype)
             with self._allocating(stream):
                 keys = torch.empty(rows, self.heads, self.head_width, dtype=dtype, device=self.device)
                 values = torch.empty_like(keys)
-        rows = keys.shape[0]
-        k, v = self._rows(keys, "keys", rows, self.heads), self._rows(values, "values", rows, self.heads)
-        check(self._lib.wsp_cache_read(self._usable(batch), batch._ref, rows, ctypes.byref(k), ctypes.byref(v),
-                                       self._stream(stream)))
+            k, v = self._plain(keys, self.heads, code), self._plain(values, self.heads, code)
+        else:
+            rows = keys.shape[0]
+            k, v = self._rows(keys, "keys", rows, self.heads), self._rows(values, "values", rows, self.heads)
+        check(self._lib.wsp_cache_read(handle, batch._ref, rows, ctypes.byref(k), ctypes.byref(v), self._stream(stream)))
         return keys, values
 
     def attend(self, batch: CacheBatch, queries, out=None, lse=None, scale: float | None = None, causal: bool = True,
@@ -221,6 +232,9 @@ class PagedCache:
         with self._allocating(stream):
             if out is None:
                 out = torch.empty_like(queries, memory_format=torch.contiguous_format)
+                o = self._plain(out, heads, q.dtype)
+            else:
+                o = self._rows(out, "out", rows, heads)
             if lse is None:
                 if return_lse:
                     lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device)
@@ -228,7 +242,6 @@ class PagedCache:
                     lse.get_device() != self._index:
                 raise ValueError(f"lse must be a contiguous float32 tensor [{rows}, {heads}] on the cache's device")
             workspace = self._workspace(needed, stream) if needed else None
-        o = self._rows(out, "out", rows, heads)
         check(self._lib.wsp_cache_attend(handle, batch._ref, rows, heads, ctypes.byref(q), ctypes.byref(o),
                                          lse.data_ptr() if lse is not None else None,
                                          self._scale if scale is None else scale, causal,
@@ -258,6 +271,10 @@ class PagedCache:
             raise ValueError(f"{name} must be contiguous in the last dimension")
         code = _codes.get(t.dtype)
         return CCacheRows(t.data_ptr(), row_stride, head_stride, _row_type(t.dtype) if code is None else code)
+
+    def _plain(self, t, heads: int, code: int) -> CCacheRows:
+        """A new, contiguous row array."""
+        return CCacheRows(t.data_ptr(), heads * self.head_width, self.head_width, code)
 
     def _stream(self, stream):
         if stream is None:

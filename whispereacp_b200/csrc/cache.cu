@@ -7,6 +7,7 @@
 #include "host.h"
 
 #include <algorithm>
+#include <atomic>
 #include <memory>
 
 namespace wsp {
@@ -338,7 +339,7 @@ struct wsp_cache {
     int device = 0;
     int sms = 0;
     wsp::DeviceBuffer owned[4];
-    wsp::DeviceBuffer status;  // which wait of a kernel gave up
+    int* status = nullptr;  // which wait of a kernel gave up
 };
 
 namespace wsp {
@@ -382,6 +383,19 @@ RowsView check_rows(const wsp_cache_rows* r, const char* name, int rows, int hea
 
 CacheBatchView batch_view(const wsp_cache_batch& b) {
     return {b.table, b.lengths, b.starts, b.table_stride, b.table_columns, b.sequences};
+}
+
+// The caches' status words: static device memory, one after another, so that
+// making a cache allocates and waits for nothing.  A word is 0 unless a wait
+// gave up and nobody has asked since; caches 1024 apart share one.
+constexpr int kStatusWords = 1024;
+__device__ int status_words[kStatusWords];
+
+int* status_word() {
+    static std::atomic<unsigned> made{0};
+    void* words = nullptr;
+    CUDA_CHECK(cudaGetSymbolAddress(&words, status_words));
+    return static_cast<int*>(words) + made++ % kStatusWords;
 }
 
 using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
@@ -522,7 +536,7 @@ int wsp_cache_create(const wsp_cache_shape* shape, int device, const wsp_cache_m
         c->maps.keys = wsp::pool_map(s, m, m.keys);
         c->maps.values = wsp::pool_map(s, m, m.values);
         wsp::prepare_cache_attend(s.storage, s.head_width);
-        c->status.allocate(sizeof(int));
+        c->status = wsp::status_word();
         *out = c.release();
     });
 }
@@ -597,7 +611,7 @@ int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, i
         a.group = query_heads / c.shape.heads;
         a.scale = scale;
         a.causal = causal != 0;
-        a.status = c.status.get<int>();
+        a.status = c.status;
         a.workspace = static_cast<unsigned char*>(workspace);
         wsp::CurrentDevice device(c.device);
         wsp::launch_cache_attend(a, c.maps, wsp::attend_shape(c, queries->dtype, *batch),
@@ -611,8 +625,10 @@ int wsp_cache_check(wsp_cache* cache) {
         wsp::CurrentDevice device(c.device);
         wsp::cuda_check(cudaDeviceSynchronize(), "wsp_cache_check");
         int status = 0;
-        wsp::cuda_check(cudaMemcpy(&status, c.status.get(), sizeof status, cudaMemcpyDeviceToHost), "wsp_cache_check");
-        if (status) throw wsp::CudaFailure("a wait of the cache's attention gave up (" + std::to_string(status) + ")", false);
+        wsp::cuda_check(cudaMemcpy(&status, c.status, sizeof status, cudaMemcpyDeviceToHost), "wsp_cache_check");
+        if (!status) return;
+        wsp::cuda_check(cudaMemset(c.status, 0, sizeof status), "wsp_cache_check");
+        throw wsp::CudaFailure("a wait of the cache's attention gave up (" + std::to_string(status) + ")", false);
     });
 }
 
