@@ -1,8 +1,9 @@
 """The paged cache without a device: every entry point include/wsp_cache.h
-declares is exported and has a ctypes signature, the header compiles as C,
-the package's names are there, and every refusal of the entry points comes
-back before anything is launched (tests/cpp/cache_test.cu, compiled with the
-cache's host code)."""
+declares is exported and has a ctypes signature, the structures are laid out
+as the header has them, the C++ header compiles against the library, and every
+refusal of the entry points comes back before anything is launched
+(tests/cpp/cache_test.cu, compiled with the cache's host code).  On the GPU, the
+program over the C++ header runs."""
 import os
 import re
 import shutil
@@ -52,6 +53,30 @@ def test_every_refusal_comes_before_any_launch(tmp_path):
     if build.returncode != 0:
         pytest.fail(build.stderr)
     run = subprocess.run([program], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
+
+
+def compile_binding(out_dir) -> str:
+    cuda = "/usr/local/cuda"
+    library = os.path.join(ROOT, "whispereacp_b200")
+    program = os.path.join(str(out_dir), "cache_binding_test")
+    build = subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "include"),
+                            "-I", os.path.join(cuda, "include"), os.path.join(ROOT, "tests", "cpp", "cache_binding_test.cpp"),
+                            "-L", library, "-lwsp_b200", f"-Wl,-rpath,{library}", "-L", os.path.join(cuda, "lib64"),
+                            "-lcudart", f"-Wl,-rpath,{os.path.join(cuda, 'lib64')}", "-o", program],
+                           capture_output=True, text=True)
+    if build.returncode != 0:
+        pytest.fail(build.stderr)
+    return program
+
+
+def test_the_cpp_header_compiles_against_the_library(tmp_path):
+    compile_binding(tmp_path)
+
+
+@pytest.mark.gpu
+def test_the_cache_through_the_cpp_header(tmp_path):
+    run = subprocess.run([compile_binding(tmp_path)], capture_output=True, text=True, timeout=120)
     assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
 
 
