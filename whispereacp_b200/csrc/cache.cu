@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_c
     __shared__ long long pool_at[kCopyRows], scale_at[kCopyRows];  // a row's place in head 0; -1: no page, -2: no row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int first = (int)blockIdx.x * a.block_rows;
+    wait_for_kernel_before();
     for (int i = warp; i < a.block_rows; i += kCopyThreads / 32) {
         const int r = first + i;
         // The row's sequence: as many as end at or before it lie in front.
@@ -286,8 +287,8 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_c
 template <int S, int T, bool kWrite>
 void launch_copy(const CopyArgs& a, int width, cudaStream_t stream) {
     const unsigned grid = (unsigned)(((long long)a.rows + a.block_rows - 1) / a.block_rows);
-    if (width == 64) cache_copy_kernel<S, T, 64, kWrite><<<grid, kCopyThreads, 0, stream>>>(a);
-    else cache_copy_kernel<S, T, 128, kWrite><<<grid, kCopyThreads, 0, stream>>>(a);
+    CUDA_CHECK(launch_early(width == 64 ? cache_copy_kernel<S, T, 64, kWrite> : cache_copy_kernel<S, T, 128, kWrite>,
+                            dim3(grid), kCopyThreads, 0, stream, a));
 }
 
 template <int S, bool kWrite>
@@ -466,7 +467,6 @@ void copy_rows(wsp_cache* cache, const wsp_cache_batch* batch, int rows, const w
     while (a.block_rows < kCopyRows && rows / (2 * a.block_rows) >= 2 * c.sms) a.block_rows *= 2;
     CurrentDevice device(c.device);
     launch_copy<kWrite>(a, c.shape.storage, keys->dtype, c.shape.head_width, static_cast<cudaStream_t>(stream));
-    CUDA_CHECK(cudaGetLastError());
 }
 
 }  // namespace

@@ -27,8 +27,8 @@
 // 8-bit keys and values become fp16 exactly (both types fit) and are
 // multiplied unscaled.  A key's scale multiplies its score; a value's scale
 // multiplies its probability, relative to the warp's largest so far, so that
-// the product stays in fp16's range whatever the scales are.  bf16 queries
-// become fp16 after a power of two a row brings them near 1.
+// the product stays in fp16's range whatever the scales are; P is one fp16
+// here, whose 2^-12 is below what 8 bits leave of a value.  bf16 queries become fp16 after a power of two a row brings them near 1.
 #include "cache_join.cuh"
 
 #include <algorithm>
@@ -101,21 +101,23 @@ struct Place {
     int units, tiles; // of the item; items of a head
 };
 
-// A lane's sequence of the first 32 and its units, kept for find_unit.
+// A lane's sequences of the first 64 and their units, kept for find_unit.
 struct FirstSequences {
-    CacheSequence q;
-    long long units;
+    CacheSequence q[2];
+    long long units[2];
 };
 
 template <int kKeys, int kRows>
 __device__ __forceinline__ long long all_units(const CacheAttendArgs& a, int lane, FirstSequences& kept) {
     kept = FirstSequences{};
-    if (lane < a.batch.sequences) {
-        kept.q = attend_sequence(a, lane);
-        kept.units = sequence_units<kKeys, kRows>(kept.q, a);
-    }
-    long long sum = kept.units;
-    for (int s = lane + 32; s < a.batch.sequences; s += 32) sum += sequence_units<kKeys, kRows>(attend_sequence(a, s), a);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (32 * i + lane < a.batch.sequences) kept.q[i] = attend_sequence(a, 32 * i + lane);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (32 * i + lane < a.batch.sequences) kept.units[i] = sequence_units<kKeys, kRows>(kept.q[i], a);
+    long long sum = kept.units[0] + kept.units[1];
+    for (int s = lane + 64; s < a.batch.sequences; s += 32) sum += sequence_units<kKeys, kRows>(attend_sequence(a, s), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
@@ -127,9 +129,9 @@ template <int kKeys, int kRows>
 __device__ __forceinline__ Place find_unit(const CacheAttendArgs& a, long long u, int lane, const FirstSequences& kept) {
     Place p{};
     for (int base = 0; base < a.batch.sequences; base += 32) {
-        CacheSequence q = kept.q;
-        long long mine = kept.units;
-        if (base > 0) {
+        CacheSequence q = base == 0 ? kept.q[0] : kept.q[1];
+        long long mine = base == 0 ? kept.units[0] : kept.units[1];
+        if (base > 32) {
             mine = 0;
             if (base + lane < a.batch.sequences) {
                 q = attend_sequence(a, base + lane);
@@ -267,7 +269,7 @@ __device__ __forceinline__ float narrow_queries(uint32_t (&qf)[D / 16][2]) {
 
 // A grid that was launched behind another, whose results it does not read,
 // ends behind it all the same: who waits for this one waits for both.
-__device__ __forceinline__ void ends_behind() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void ends_behind() { wait_for_kernel_before(); }
 
 // The producer warp: every unit of the run into the ring.
 template <int S, int D, int NT>
@@ -376,6 +378,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         *redo = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (!a.behind) wait_for_kernel_before();
     FirstSequences kept;
     const long long total = all_units<Layout::keys, kRows>(a, lane, kept);
     const long long per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
@@ -636,9 +639,13 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            split_pair<MT>(x[i][j][2 * h], x[i][j][2 * h + 1], hi[j][h], lo[j][h]);
-                            hi[j][h] = transposed(hi[j][h]);
-                            lo[j][h] = transposed(lo[j][h]);
+                            if constexpr (kEight) {
+                                hi[j][h] = transposed(Half16<MT>::pack2(x[i][j][2 * h], x[i][j][2 * h + 1]));
+                            } else {
+                                split_pair<MT>(x[i][j][2 * h], x[i][j][2 * h + 1], hi[j][h], lo[j][h]);
+                                hi[j][h] = transposed(hi[j][h]);
+                                lo[j][h] = transposed(lo[j][h]);
+                            }
                         }
                     const uint32_t base = smem_address(values);
                     if constexpr (!kEight) {
@@ -669,7 +676,6 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
 #pragma unroll
                                 for (int j = 0; j < NT; ++j) {
                                     mma_16816<MT>(o[k + h][j], f, hi[j]);
-                                    mma_16816<MT>(o[k + h][j], f, lo[j]);
                                 }
                             }
                         }
@@ -791,20 +797,10 @@ bool token_uncut(const CacheAttendShape& shape, int group) {
 }
 
 template <typename T, int S, int D, int NT>
-CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, bool behind, cudaStream_t stream) {
+CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, cudaStream_t stream) {
     using Layout = TokenLayout<S, D, NT>;
     const int grid = (int)token_grid<Layout>(a, sms);
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid);
-    config.blockDim = dim3(kTokenThreads);
-    config.dynamicSmemBytes = Layout::bytes;
-    config.stream = stream;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = behind ? 1 : 0;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, cache_tokens_kernel<T, S, D, NT>, a, maps));
+    CUDA_CHECK(launch_early(cache_tokens_kernel<T, S, D, NT>, dim3(grid), kTokenThreads, Layout::bytes, stream, a, maps));
     return {a.workspace, a.uncut ? 0 : grid, Layout::rows};
 }
 
@@ -851,6 +847,7 @@ void launch_cache_attend(const CacheAttendArgs& args, const CacheMaps& maps, con
         CacheAttendArgs b = a;
         b.workspace += token_workspace(shape);
         chunks = launch_cache_chunk(b, maps, shape, stream);
+        a.behind = 1;
     }
     a.uncut = token_uncut(shape, a.group);
     // Tiles of 16 rows where no sequence has more and some may have more than 8;
@@ -859,8 +856,8 @@ void launch_cache_attend(const CacheAttendArgs& args, const CacheMaps& maps, con
         using T = decltype(t);
         constexpr int S = s.value, D = d.value;
         const CutPart tokens = most > 8 && most <= kFewRows
-                                   ? launch_tokens<T, S, D, 2>(a, maps, shape.sms, false, stream)
-                                   : launch_tokens<T, S, D, 1>(a, maps, shape.sms, most > kFewRows, stream);
+                                   ? launch_tokens<T, S, D, 2>(a, maps, shape.sms, stream)
+                                   : launch_tokens<T, S, D, 1>(a, maps, shape.sms, stream);
         launch_join<T, S, D>(a, tokens, chunks, stream);
     });
 }

@@ -22,6 +22,7 @@ struct CacheAttendArgs {
     float scale;
     int causal;
     int uncut;                     // the few-row kernel's CTAs take whole items
+    int behind;                    // the few-row kernel runs behind the chunks', which waited for what is before
     long long few;                 // rows * group up to which a sequence is the few-row kernel's
     int* status;                   // which wait gave up, 0: none
     unsigned char* workspace;
@@ -60,6 +61,26 @@ void prepare_cache_chunk(int storage, int width);
 CutPart launch_cache_chunk(const CacheAttendArgs& args, const CacheMaps& maps, const CacheAttendShape& shape,
                            cudaStream_t stream);
 size_t cache_chunk_workspace(const CacheAttendShape& shape);
+
+// A launch that may begin while the kernel before it ends: the kernel's first
+// act is to wait for that (griddepcontrol.wait), so that only its launch and
+// what comes before the wait overlap.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t shared, cudaStream_t stream,
+                         const Args&... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Raises the kernels' limits of shared memory on the current device.
 void prepare_cache_attend(int storage, int width);

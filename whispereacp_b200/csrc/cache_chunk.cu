@@ -931,6 +931,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
                      "r"((uint32_t)Layout::columns));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    wait_for_kernel_before();
     // The few-row kernel behind this one may fill what SMs are left.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     FirstSequences kept;
@@ -998,8 +999,8 @@ CutPart launch_cache_chunk(const CacheAttendArgs& a, const CacheMaps& maps, cons
         constexpr int S = s.value, D = d.value;
         using Layout = ChunkLayout<S, D>;
         const int grid = chunk_grid<S, D>(a, shape.sms);
-        cache_chunk_kernel<decltype(t), S, D><<<grid, Layout::threads, Layout::bytes, stream>>>(a, maps);
-        CUDA_CHECK(cudaGetLastError());
+        CUDA_CHECK(launch_early(cache_chunk_kernel<decltype(t), S, D>, dim3(grid), Layout::threads, Layout::bytes, stream,
+                                a, maps));
         part = {a.workspace, grid, Layout::rows};
     });
     return part;

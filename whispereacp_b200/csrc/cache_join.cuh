@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kThreads)
     const CutPart part_of = late ? second : first;
     const int block = (int)blockIdx.x - (late ? first.blocks() : 0);
     const int c = block / part_of.slices() + 1, slice = block % part_of.slices();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_kernel_before();
     const CutItem* record = cut_items(part_of.workspace) + c;
     const int4 head_of = *reinterpret_cast<const int4*>(record), rest = *(reinterpret_cast<const int4*>(record) + 1);
     const CutItem cut = {head_of.x, head_of.y, head_of.z, head_of.w, {rest.x, rest.y, rest.z, rest.w}};
@@ -135,17 +135,8 @@ void launch_join(const CacheAttendArgs& a, const CutPart& first, const CutPart& 
     if (blocks == 0) return;
     const long long items = std::max((long long)a.batch.sequences, (long long)a.rows * a.group / first.rows) * a.cache.heads;
     const bool many = first.grid > 8 * items;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(blocks);
-    config.blockDim = dim3(many ? 512 : 256);
-    config.stream = stream;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, many ? cache_join_kernel<T, S, D, 512> : cache_join_kernel<T, S, D, 256>, a,
-                                  first, second));
+    CUDA_CHECK(launch_early(many ? cache_join_kernel<T, S, D, 512> : cache_join_kernel<T, S, D, 256>, dim3(blocks),
+                            many ? 512 : 256, 0, stream, a, first, second));
 }
 
 template <typename F>
