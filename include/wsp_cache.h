@@ -94,7 +94,8 @@ int wsp_cache_get_memory(const wsp_cache* cache, wsp_cache_memory* memory);
  * no page: appending there does nothing, and its rows read as zeros.  In the
  * attention rows of such pages take part as zeros, positions outside the
  * table do not take part, and a sequence whose rows lie outside the call's
- * arrays has none.  max_rows is a bound of n, the same or larger; it chooses
+ * arrays has none.  table_columns * page_rows is at most 2^31 - 256.  max_rows
+ * is a bound of n, the same or larger; it chooses
  * kernels only.
  */
 typedef struct wsp_cache_batch {
@@ -137,7 +138,8 @@ int wsp_cache_read(wsp_cache* cache, const wsp_cache_batch* batch, int rows, con
  * to the row's own (causal) or over every held row.  queries and out are
  * [rows, query_heads, head_width] of one 16-bit type, which a 16-bit cache
  * shares; query_heads is a multiple of the cache's heads, and query head h
- * reads head h / (query_heads / heads).  lse (NULL: none), [rows,
+ * reads head h / (query_heads / heads); out overlaps neither queries nor the
+ * pools.  lse (NULL: none), [rows,
  * query_heads] contiguous, gets the natural logarithm of the sum of
  * exponentials.  A row that sees no key gets zeros and -infinity.  Keys and
  * values a row does not see cannot change its result, whatever they hold.

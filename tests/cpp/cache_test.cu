@@ -146,6 +146,19 @@ int main() {
         EXPECT(wsp_cache_attend(&cache, &batch, 6, 4, &rows, &rows, nullptr, 1.f, 1, at(4104), bytes, nullptr),
                WSP_INVALID_ARGUMENT, "workspace");
     }
+    EXPECT(wsp_cache_attend(&cache, &batch, 6, 4, &rows, &rows, nullptr, 1.f, 1, at(4096), bytes, nullptr),
+           WSP_INVALID_ARGUMENT, "one memory");
+    {
+        // The rows of a sequence: 2^31 - 256 are the most.
+        wsp_cache_batch b = batch;
+        b.table_stride = b.table_columns = (0x7fffff00 >> 4) + 1;
+        EXPECT(wsp_cache_attend(&cache, &b, 6, 4, &rows, &rows, nullptr, 1.f, 1, at(4096), bytes, nullptr),
+               WSP_INVALID_ARGUMENT, "at most 2147483392 rows");
+        EXPECT(wsp_cache_append(&cache, &b, 6, &rows, &rows, nullptr), WSP_INVALID_ARGUMENT, "at most 2147483392 rows");
+        EXPECT(wsp_cache_read(&cache, &b, 6, &rows, &rows, nullptr), WSP_INVALID_ARGUMENT, "at most 2147483392 rows");
+        b.table_stride = --b.table_columns;
+        EXPECT(wsp_cache_attend_workspace(&cache, &b, 6, 4, &bytes), WSP_OK, "");
+    }
     EXPECT(wsp_cache_get_memory(&cache, nullptr), WSP_INVALID_ARGUMENT, "NULL");
     wsp_cache_memory got{};
     EXPECT(wsp_cache_get_memory(&cache, &got), WSP_OK, "");

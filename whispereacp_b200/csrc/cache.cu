@@ -353,11 +353,18 @@ const wsp_cache& checked(const wsp_cache* cache) {
     return *cache;
 }
 
-void check_batch(const wsp_cache_batch* b, int rows) {
+// Positions and what a kernel adds to them (a block of 128 keys, the copies'
+// boxes) stay in 31 bits.
+constexpr long long kMostHeld = 0x7fffff00ll;
+
+void check_batch(const wsp_cache& c, const wsp_cache_batch* b, int rows) {
     if (!b) throw InvalidArgument("batch must not be NULL");
     if (rows < 0) throw InvalidArgument("rows must not be negative, got " + to_string(rows));
     if (b->sequences < 0 || b->table_columns < 0 || b->max_rows < 0)
         throw InvalidArgument("a batch's sequences, table_columns and max_rows must not be negative");
+    if ((long long)b->table_columns * c.shape.page_rows > kMostHeld)
+        throw InvalidArgument("a table's columns hold at most " + to_string(kMostHeld) + " rows of a sequence, not " +
+                              to_string((long long)b->table_columns * c.shape.page_rows));
     if (b->sequences == 0) return;
     if (!b->lengths || !b->starts || (!b->table && b->table_columns > 0))
         throw InvalidArgument("a batch's table, lengths and starts must not be NULL");
@@ -442,7 +449,7 @@ CacheAttendShape attend_shape(const wsp_cache& c, int dtype, const wsp_cache_bat
 }
 
 size_t checked_workspace(const wsp_cache& c, const wsp_cache_batch* batch, int rows, int query_heads) {
-    check_batch(batch, rows);
+    check_batch(c, batch, rows);
     if (query_heads <= 0 || query_heads % c.shape.heads)
         throw ModelError("query_heads (" + to_string(query_heads) + ") must be a multiple of the cache's heads (" +
                          to_string(c.shape.heads) + ")");
@@ -453,7 +460,7 @@ template <bool kWrite>
 void copy_rows(wsp_cache* cache, const wsp_cache_batch* batch, int rows, const wsp_cache_rows* keys,
                const wsp_cache_rows* values, void* stream) {
     const wsp_cache& c = checked(cache);
-    check_batch(batch, rows);
+    check_batch(c, batch, rows);
     CopyArgs a{};
     a.keys = check_rows(keys, "keys", rows, c.shape.heads, c.shape.head_width);
     a.values = check_rows(values, "values", rows, c.shape.heads, c.shape.head_width);
@@ -596,6 +603,7 @@ int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, i
         if (needed && (!workspace || !wsp::aligned(workspace) || workspace_bytes < needed))
             throw wsp::InvalidArgument("the workspace must be 16-byte aligned and hold " + to_string(needed) + " bytes, not " +
                                        to_string(workspace ? workspace_bytes : 0));
+        if (q.data == o.data) throw wsp::InvalidArgument("queries and out must not be one memory");
         wsp::CacheAttendArgs a{};
         a.cache = c.view;
         a.batch = wsp::batch_view(*batch);
