@@ -386,6 +386,32 @@ def test_what_a_row_does_not_see_cannot_change_it(storage, dtype, rows):
             assert bool(((lse[a:b - 1].double() - l).abs() <= lse_tol)[~torch.isnan(l) & ~torch.isinf(l)].all())
 
 
+@pytest.mark.parametrize("storage,dtype", [("bfloat16", "bfloat16"), ("int8", "float16")])
+def test_chunks_of_a_long_context_whose_last_key_is_no_number(storage, dtype):
+    """Whole items of many heads: every row that shares the last key's block is
+    computed again, alone, while the CTA's other warps wait for its next item."""
+    import torch
+    length, new, heads = 6000, 300, 160
+    cache = make_cache(storage, 400, heads, 16, 128, 217)
+    batch, starts = make_batch([length], [new], 16, 400, 218)
+    page, row = int(batch.page_table[0, (length - 1) // 16]), (length - 1) % 16
+    for pool, scale in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales)):
+        if scale is not None:
+            scale[page, :, row] = 255
+        else:
+            pool[page, :, row] = math.nan
+    q = queries(int(starts[-1]), heads, 128, dtype, 219)
+    out, lse = cache.attend(batch, q, return_lse=True)
+    cache.check()
+    a, b = int(starts[0]), int(starts[-1])
+    assert bool(torch.isnan(out[b - 1]).all()) and bool(torch.isnan(lse[b - 1]).all())
+    for h in range(0, heads, 53):
+        k, v = (x[:-1, h:h + 1].contiguous() for x in held_rows(cache, batch.page_table[0], length))
+        o, l, tol, lse_tol = expected(q[a:b - 1, h:h + 1], k, v, 128 ** -0.5, True, length - new)
+        assert bool(((out[a:b - 1, h:h + 1].double() - o).abs() <= tol).all())
+        assert bool(((lse[a:b - 1, h:h + 1].double() - l).abs() <= lse_tol).all())
+
+
 @pytest.mark.parametrize("storage,dtype", [("float16", "float16"), ("bfloat16", "bfloat16"), ("int8", "float16")])
 def test_large_scores_and_large_values(storage, dtype):
     """Scores in the hundreds, a maximum that grows tile by tile, and values
@@ -506,6 +532,42 @@ def test_a_step_captured_and_replayed_with_other_contents():
     torch.cuda.synchronize()
     for _, q, k, v, out, lse in graphs:
         check_attend(cache, batch, starts, q, out, lse, 0.125, True)
+
+
+def test_a_mixed_batch_captured_and_replayed():
+    """Chunks, tokens and the join of both in one graph, an append before and a
+    read behind them; the contents change between the replays."""
+    import torch
+    lengths, new = [700, 100, 300, 64], [150, 1, 20, 0]
+    cache = make_cache("int8", 128, 2, 32, 128, 177)
+    batch, starts = make_batch([n + 51 for n in lengths], new, 32, 128, 178, columns=40)
+    batch.lengths -= 51  # pages for every replay's rows
+    rows = int(starts[-1])
+    q = queries(rows, 6, 128, "bfloat16", 179)
+    k, v = queries(rows, 2, 128, "bfloat16", 180), queries(rows, 2, 128, "bfloat16", 181)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.attend(batch, q, return_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(batch, k, v)
+        out, lse = cache.attend(batch, q, return_lse=True)
+        again, all_lse = cache.attend(batch, q, causal=False, return_lse=True)
+        kr, vr = cache.read(batch, dtype=torch.float32, rows=rows)
+    for step in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attend(cache, batch, starts, q, out, lse, 128 ** -0.5, True)
+        check_attend(cache, batch, starts, q, again, all_lse, 128 ** -0.5, False)
+        first, last = int(starts[0]), int(starts[-1])
+        assert torch.equal(kr[first:last].double(), quantised(k[first:last], "int8")[0])
+        assert torch.equal(vr[first:last].double(), quantised(v[first:last], "int8")[0])
+        batch.lengths += 17
+        q.copy_(queries(rows, 6, 128, "bfloat16", 190 + step))
+        k.copy_(queries(rows, 2, 128, "bfloat16", 195 + step))
+    cache.check()
 
 
 def test_two_streams_at_once():

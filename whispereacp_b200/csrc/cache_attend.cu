@@ -40,7 +40,7 @@ constexpr int kWorkers = 4;  // consumer warps
 constexpr int kTokenThreads = 32 * (kWorkers + 1);
 constexpr float kLazy = 8.f;  // how far a score may pass the running maximum, in log2
 
-enum CacheWait : int { kWaitFull = 1, kWaitFree = 2, kWaitDrain = 3 };
+enum CacheWait : int { kWaitFull = 1, kWaitFree = 2 };
 
 // Shared memory: the stages, the item join's rows, the warps' softmax rows,
 // barriers and the abort flag.  A stage is 16 KB (32 KB for 128-wide 16-bit
@@ -64,7 +64,7 @@ struct TokenLayout {
     static constexpr int join_at = scale_at + stages * scale_bytes;
     static constexpr int ml_at = join_at + join_bytes;
     static constexpr int bar_at = ml_at + kWorkers * rows * 2 * 4;
-    static constexpr int bytes = bar_at + 2 * stages * 8 + 16;
+    static constexpr int bytes = bar_at + 2 * stages * 8 + kBarrierWords * 4;
     static_assert(stages >= 2 && stages <= 14, "a ring");
 };
 
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + Layout::bar_at);
     uint64_t* empty = full + Layout::stages;
     volatile int* abort = reinterpret_cast<volatile int*>(empty + Layout::stages);
-    int* redo = reinterpret_cast<int*>(empty + Layout::stages) + 1;
+    int* redo = reinterpret_cast<int*>(empty + Layout::stages) + kOwnWord;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
             cache_barrier_init(full + i, 1);
             cache_barrier_init(empty + i, kWorkers);
         }
-        *abort = 0;
+        *abort = abort[kBeatWord] = 0;
         *redo = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                 for (int row = warp; row < kRows; row += kWorkers)
                     if (again >> row & 1) {
                         const TileRow r = tile_row(a, p.q, p.head, p.tile * kRows + row);
-                        attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, r.token, r.head);
+                        attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, r.token, r.head, abort + kBeatWord);
                     }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (threadIdx.x == 0) *redo = 0;

@@ -65,7 +65,7 @@ struct ChunkLayout {
     static constexpr int bar_at = held_at + depth * held_bytes;
     // full, empty; per tile: scores, P's halves, first half, queries, O; done
     static constexpr int bars = 2 * stages + 6 * tiles + 1;
-    static constexpr int bytes = bar_at + bars * 8 + 16;
+    static constexpr int bytes = bar_at + bars * 8 + kBarrierWords * 4;
 };
 
 // ------------------------------------------------------------ the block list
@@ -885,7 +885,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             again &= again - 1;
             const int token = __shfl_sync(0xffffffffu, r.token, i), head = __shfl_sync(0xffffffffu, r.head, i);
             __syncwarp();
-            attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, token, head);
+            attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, token, head, abort + kBeatWord);
         }
         tmem_fence_before();  // this tile's reads, before the products that the next arrival lets run
         if (last_n == 0) break;
@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
     const ChunkBars bar = {bars, bars + Layout::stages, tile_bars, tile_bars + kTiles, tile_bars + 3 * kTiles,
                            tile_bars + 4 * kTiles, tile_bars + 5 * kTiles, tile_bars + 6 * kTiles};
     volatile int* abort = reinterpret_cast<volatile int*>(bars + Layout::bars);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + Layout::bars) + 1;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + Layout::bars) + kOwnWord;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < Layout::stages; ++i) {
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
             cache_barrier_init(bar.o + t, 1);
         }
         cache_barrier_init(bar.done, 1);
-        *abort = 0;
+        *abort = abort[kBeatWord] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == Layout::mma_warp) {

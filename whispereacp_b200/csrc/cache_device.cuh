@@ -34,18 +34,31 @@ __device__ __forceinline__ bool cache_phase_done(uint64_t* bar, uint32_t parity)
     return done != 0;
 }
 
+// The words behind a CTA's barriers: whether a wait has given up, a word of
+// the kernel's own, and one that changes while a warp does a row alone.
+constexpr int kAbortWord = 0, kOwnWord = 1, kBeatWord = 2, kBarrierWords = 4;
+
 // Waits for the phase of `parity`.  After 2 s, or once another wait of the CTA
 // has given up, it records `kind` and returns false, and so does every later
 // wait at once: the roles then run through their loops without waiting, so
-// all meet at the barriers between them, and the results are void.
+// all meet at the barriers between them, and the results are void.  A warp of
+// the CTA that does rows alone may take longer over a long context; the 2 s
+// count from its last sign (its loops end by themselves).
 static __device__ __noinline__ bool cache_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
                                                     int kind) {
-    const unsigned long long start = cache_clock_ns();
+    unsigned long long start = cache_clock_ns();
+    int beat = abort[kBeatWord];
     for (unsigned spin = 1;; ++spin) {
         if (cache_phase_done(bar, parity)) return true;
         if ((spin & 15) != 0) continue;
         if (*abort) return false;
         if (cache_clock_ns() - start > kCacheTimeoutNs) {
+            const int now = abort[kBeatWord];
+            if (now != beat) {
+                beat = now;
+                start = cache_clock_ns();
+                continue;
+            }
             atomicCAS(status, 0, kind);
             *abort = 1;
             return false;
@@ -126,11 +139,13 @@ __device__ __forceinline__ void widen4(uint32_t bytes, bool interleaved, uint32_
 // the row sees are read.  The tiled kernels multiply whole tiles, where an
 // infinity or NaN among the values of a key behind the row (0 times it) makes
 // the row NaN; such rows, which see fewer keys than the sequence holds, come
-// here.
+// here.  16 keys share a page, and 4 of them are on their way at once.  `beat`
+// (null: nobody waits) changes every 16 keys.
 template <typename T, int S, int D>
 __device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int first, int before, int length, int i,
-                                        int head) {
+                                        int head, volatile int* beat) {
     constexpr int kPer = D / 32;  // a lane's elements
+    using Pair = typename std::conditional<cache_eight(S), uint16_t, uint32_t>::type;
     const int lane = threadIdx.x & 31;
     const int keys = a.causal ? min(before + i + 1, length) : length;
     const long long row = (long long)first + i;
@@ -145,38 +160,57 @@ __device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int fir
         o[e] = o[e + 1] = 0.f;
     }
     float top = -INFINITY, total = 0.f;
-    for (int j = 0; j < keys; ++j) {
-        const int page = cache_page(a.cache, a.batch, s, j);
-        float k[kPer], v[kPer], ks = 1.f, vs = 1.f;
+    for (int j16 = 0; j16 < keys; j16 += 16) {
+        const int page = cache_page(a.cache, a.batch, s, j16);
+        if (beat && lane == 0) *beat = *beat + 1;
+        for (int j = j16; j < min(j16 + 16, keys); j += 4) {
+            Pair k[4][kPer / 2], v[4][kPer / 2];
+            uint8_t ks[4], vs[4];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) k[e] = v[e] = 0.f;
-        if (page >= 0) {
-            const int slot = j & ((1 << a.cache.page_shift) - 1);
-            const long long at = cache_offset(a.cache, page, kv, slot) + lane * kPer * cache_bytes(S);
+            for (int n = 0; n < 4; ++n) {
+                ks[n] = vs[n] = 0;
 #pragma unroll
-            for (int e = 0; e < kPer; e += 2) {
-                using Pair = typename std::conditional<cache_eight(S), uint16_t, uint32_t>::type;
-                const float2 fk = cache_pair<S>(*reinterpret_cast<const Pair*>(a.cache.keys + at + e * cache_bytes(S)));
-                const float2 fv = cache_pair<S>(*reinterpret_cast<const Pair*>(a.cache.values + at + e * cache_bytes(S)));
-                k[e] = fk.x, k[e + 1] = fk.y, v[e] = fv.x, v[e + 1] = fv.y;
+                for (int e = 0; e < kPer / 2; ++e) k[n][e] = v[n][e] = 0;
+                if (page < 0 || j + n >= keys) continue;
+                const int slot = (j + n) & ((1 << a.cache.page_shift) - 1);
+                const long long at = cache_offset(a.cache, page, kv, slot) + lane * kPer * cache_bytes(S);
+#pragma unroll
+                for (int e = 0; e < kPer / 2; ++e) {
+                    k[n][e] = *reinterpret_cast<const Pair*>(a.cache.keys + at + 2 * e * cache_bytes(S));
+                    v[n][e] = *reinterpret_cast<const Pair*>(a.cache.values + at + 2 * e * cache_bytes(S));
+                }
+                if constexpr (cache_eight(S)) {
+                    const long long si = cache_scale_index(a.cache, page, kv, slot);
+                    ks[n] = a.cache.key_scales[si];
+                    vs[n] = a.cache.value_scales[si];
+                }
             }
-            if (cache_eight(S)) {
-                const long long si = cache_scale_index(a.cache, page, kv, slot);
-                ks = cache_scale(a.cache.key_scales[si]);
-                vs = cache_scale(a.cache.value_scales[si]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                if (j + n >= keys) break;
+                float dot = 0.f;
+#pragma unroll
+                for (int e = 0; e < kPer / 2; ++e) {
+                    const float2 f = cache_pair<S>(k[n][e]);
+                    dot += qv[2 * e] * f.x;
+                    dot += qv[2 * e + 1] * f.y;
+                }
+                const float score = warp_sum(dot) * (cache_eight(S) ? cache_scale(ks[n]) : 1.f) * a.scale;
+                const float higher = fmaxf(top, score);
+                const float from = higher == -INFINITY ? 0.f : higher;
+                const float keep = expf(top - from), p = expf(score - from);
+                const float by = cache_eight(S) ? cache_scale(vs[n]) : 1.f;
+                total = total * keep + p;
+#pragma unroll
+                for (int e = 0; e < kPer / 2; ++e) {
+                    const float2 f = cache_pair<S>(v[n][e]);
+                    o[2 * e] = o[2 * e] * keep + p * (f.x * by);
+                    o[2 * e + 1] = o[2 * e + 1] * keep + p * (f.y * by);
+                }
+                top = higher;
             }
         }
-        float dot = 0.f;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) dot += qv[e] * k[e];
-        const float score = warp_sum(dot) * ks * a.scale;
-        const float higher = fmaxf(top, score);
-        const float from = higher == -INFINITY ? 0.f : higher;
-        const float keep = expf(top - from), p = expf(score - from);
-        total = total * keep + p;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) o[e] = o[e] * keep + p * (v[e] * vs);
-        top = higher;
+        if (!(total == total)) break;  // and so it stays, and every sum of it
     }
     const float inverse = keys > 0 ? 1.f / total : 0.f;
     unsigned char* op = a.out + row * a.o_row + head * a.o_head + lane * (kPer * 2);

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads)
         }
         if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
         if (__any_sync(0xffffffffu, !fine) && r.seen > 0 && (cache_eight(S) || r.seen < q.length))
-            attend_row<T, S, D>(a, cut.sequence, q.first, q.before, q.length, r.token, r.head);
+            attend_row<T, S, D>(a, cut.sequence, q.first, q.before, q.length, r.token, r.head, nullptr);
     }
 }
 
