@@ -488,6 +488,70 @@ def test_pools_whose_offsets_pass_32_bits():
         check_attend(cache, batch, starts.tolist(), q, out, lse, 0.125, True)
 
 
+# Calls of little work are one kernel's whatever their rows; what a table has
+# places for bounds the work, so the same sequences in a wide table are another's.
+
+def wide_batches(monkeypatch):
+    import sys
+    here = sys.modules[__name__]
+    plain = here.make_batch
+
+    def wide(lengths, new, page_rows, pages, seed, columns=None, lead=0):
+        return plain(lengths, new, page_rows, pages, seed, columns=(64 * 2400) // page_rows, lead=lead)
+
+    monkeypatch.setattr(here, "make_batch", wide)
+
+
+@pytest.mark.parametrize("storage,dtype", PAIRS)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("width,heads,group,page_rows,rows", [
+    (64, 2, 1, 16, CHUNKS), (128, 1, 3, 256, CHUNKS), (64, 1, 7, 64, CHUNKS), (128, 2, 1, 16, CHUNKS),
+    (64, 2, 3, 32, FEW), (128, 1, 8, 128, FEW)])
+def test_attention_under_a_wide_table(monkeypatch, storage, dtype, causal, width, heads, group, page_rows, rows):
+    wide_batches(monkeypatch)
+    test_attention_is_the_definition(storage, dtype, causal, width, heads, group, page_rows, rows)
+
+
+@pytest.mark.parametrize("storage,dtype", PAIRS)
+def test_unseen_keys_under_a_wide_table(monkeypatch, storage, dtype):
+    wide_batches(monkeypatch)
+    test_what_a_row_does_not_see_cannot_change_it(storage, dtype, CHUNKS)
+
+
+@pytest.mark.parametrize("storage,dtype", [("float16", "float16"), ("bfloat16", "bfloat16"), ("int8", "float16")])
+def test_large_scores_under_a_wide_table(monkeypatch, storage, dtype):
+    wide_batches(monkeypatch)
+    test_large_scores_and_large_values(storage, dtype)
+
+
+@pytest.mark.parametrize("storage,dtype", [("float16", "float16"), ("int8", "bfloat16")])
+def test_scales_under_a_wide_table(monkeypatch, storage, dtype):
+    wide_batches(monkeypatch)
+    for scale in (0.0, -0.3):
+        test_a_scale_below_or_at_zero(storage, dtype, ([200, 300], [90, 130]), scale)
+
+
+def test_two_streams_under_a_wide_table(monkeypatch):
+    wide_batches(monkeypatch)
+    test_two_streams_at_once()
+
+
+@pytest.mark.parametrize("storage,dtype", PAIRS)
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("most", [9, 16, 17, 31, 33, 63, 65])
+def test_chunks_around_the_kernels_limits(storage, dtype, width, most):
+    """The row counts where one kernel ends and the other begins, of a group of
+    one, alone and beside single tokens and an empty sequence."""
+    cache = make_cache(storage, 400, 2, 16, width, 301)
+    for new in ([most], [most, 1, 0, most - 1]):
+        lengths = [max(n, 1) + 40 * i for i, n in enumerate(new)]
+        for columns in (20, 9600):
+            batch, starts = make_batch(lengths, new, 16, 400, 302, columns=columns)
+            q = queries(sum(new), 2, width, dtype, 303)
+            out, lse = cache.attend(batch, q, return_lse=True)
+            check_attend(cache, batch, starts, q, out, lse, width ** -0.5, True)
+
+
 # ------------------------------------------------------- streams and graphs
 
 def test_a_step_captured_and_replayed_with_other_contents():
@@ -534,13 +598,14 @@ def test_a_step_captured_and_replayed_with_other_contents():
         check_attend(cache, batch, starts, q, out, lse, 0.125, True)
 
 
-def test_a_mixed_batch_captured_and_replayed():
+@pytest.mark.parametrize("columns", [40, 400])
+def test_a_mixed_batch_captured_and_replayed(columns):
     """Chunks, tokens and the join of both in one graph, an append before and a
     read behind them; the contents change between the replays."""
     import torch
     lengths, new = [700, 100, 300, 64], [150, 1, 20, 0]
     cache = make_cache("int8", 128, 2, 32, 128, 177)
-    batch, starts = make_batch([n + 51 for n in lengths], new, 32, 128, 178, columns=40)
+    batch, starts = make_batch([n + 51 for n in lengths], new, 32, 128, 178, columns=columns)
     batch.lengths -= 51  # pages for every replay's rows
     rows = int(starts[-1])
     q = queries(rows, 6, 128, "bfloat16", 179)

@@ -787,13 +787,16 @@ long long token_grid(const CacheAttendArgs& a, int sms) {
     return (long long)std::min((double)sms * Layout::ctas, (double)tiles * a.cache.heads * std::max(1ll, units));
 }
 
-// Where no item can be longer than this, whole items go to the CTAs instead of
-// equal runs: no partial results and no second kernel, at the price of runs
-// that end up to an item late.
-constexpr int kUncutUnits = 8;
+// Where no item can hold more keys than this, whole items go to the CTAs
+// instead of equal runs: no partial results and no second kernel, at the price
+// of runs that end up to an item late.  Single tokens over fp16 64-wide heads,
+// equal runs and whole items: 1 window x 16 heads of 512 keys 6.9 and 5.6 us,
+// 64 windows 17.3 and 15.2; of 1024 keys 7.6 and 7.2, 64 windows 35.9 and 33.2,
+// but 8-bit ones of 1024 keys 7.9 and 9.3 us, and 128-wide ones of 1536 keys in
+// 8 windows 11.4 and 17.2.
+constexpr long long kUncutKeys = 512;
 bool token_uncut(const CacheAttendShape& shape, int group) {
-    const int keys = shape.width * cache_bytes(shape.storage) == 64 ? 128 : 64;
-    return (long long)shape.max_rows * group <= 8 && shape.held <= (long long)kUncutUnits * keys;
+    return (long long)shape.max_rows * group <= 8 && shape.held <= kUncutKeys;
 }
 
 template <typename T, int S, int D, int NT>
@@ -806,9 +809,33 @@ CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, 
 
 }  // namespace
 
-// Rows of a key head up to which a sequence is the few-row kernel's: one of
-// its larger tiles.
-constexpr int kFewRows = 16;
+// Rows of a key head up to which a call is the few-row kernel's alone, in tiles
+// of 16: the chunk kernel's 128-row tiles cost the same for fewer, and its
+// 8-bit blocks the widening besides.  16 x 1500 keys x 8 heads, few-row and
+// chunk kernel: 32 fp16 rows 22 and 28 us (64 wide), 39 and 46 (128 wide, where
+// 4 x 8192 keys take 57 and 51, and 4 x 32768 171 and 113); 48 rows 28.5 and 28.8
+// (4 x 8192 31.6 and 31.3); 64 int8 rows 34 and 60, 57 and 97; 96 bf16 rows over
+// 64 x 450 int8 keys 82 and 79, 163 and 120.
+static long long few_rows(const CacheAttendShape& shape) {
+    return cache_eight(shape.storage) ? 64 : shape.width == 64 ? 32 : 16;
+}
+// And up to which a sequence is the few-row kernel's, in tiles of 8, beside
+// sequences of more: 12 of 48 sequences of up to 1200 keys x 8 heads with 32
+// rows, one with 200, taken by the few-row and by the chunk kernel: int8 43.5
+// and 48.8 us (64 wide), 59 and 72 (128 wide), fp16 36.0 and 31.9, 57 and 53.
+static long long few_rows_beside(const CacheAttendShape& shape) { return cache_eight(shape.storage) ? 32 : 16; }
+// Calls whose units, 16 rows each, come to this many for each of two CTAs an SM
+// at most are the few-row kernel's too, whatever their rows: it starts sooner.
+// One window's 224 rows over 450 keys x 20 heads, few-row and chunk kernel: fp16
+// 11.5 and 18.2 us, int8 11.5 and 24.8; with 12 to 15 units a CTA 21 and 23 us
+// (64 wide) but 37 and 29 (128 wide), with 30 34 and 27.
+constexpr int kSmallUnits = 8;
+static bool few_alone(const CacheAttendArgs& a, const CacheAttendShape& shape) {
+    if ((long long)shape.max_rows * a.group <= few_rows(shape)) return true;
+    const int keys = shape.width * cache_bytes(shape.storage) == 64 ? 128 : 64;
+    const double tiles = (double)((long long)a.rows * a.group / 16 + a.batch.sequences);
+    return tiles * a.cache.heads * (double)((shape.held + keys - 1) / keys) <= (double)kSmallUnits * 2 * shape.sms;
+}
 
 static size_t token_workspace(const CacheAttendShape& shape) {
     // 3 CTAs of 8-row tiles, or 2 of 16-row tiles
@@ -817,7 +844,7 @@ static size_t token_workspace(const CacheAttendShape& shape) {
 
 size_t cache_attend_workspace(const CacheAttendShape& shape, int group) {
     if (token_uncut(shape, group)) return 0;
-    const bool chunks = (long long)shape.max_rows * group > kFewRows;
+    const bool chunks = (long long)shape.max_rows * group > few_rows(shape);
     return token_workspace(shape) + (chunks ? cache_chunk_workspace(shape) : 0);
 }
 
@@ -840,22 +867,23 @@ void launch_cache_attend(const CacheAttendArgs& args, const CacheMaps& maps, con
     const long long most = (long long)shape.max_rows * a.group;
     a.few = 0x7fffffffffffll;
     CutPart chunks{};
-    if (most > kFewRows) {
+    const bool alone = few_alone(a, shape);
+    if (!alone) {
         // Sequences of many rows first; the others' kernel fills the SMs as
         // these leave them, and ends behind them.
-        a.few = kFewRows;
+        a.few = few_rows_beside(shape);
         CacheAttendArgs b = a;
         b.workspace += token_workspace(shape);
         chunks = launch_cache_chunk(b, maps, shape, stream);
         a.behind = 1;
     }
     a.uncut = token_uncut(shape, a.group);
-    // Tiles of 16 rows where no sequence has more and some may have more than 8;
-    // among chunks, those that are left are mostly single tokens.
+    // Tiles of 16 rows where some sequence may have more than 8; beside chunks,
+    // those that are left are mostly single tokens.
     with_cache_types(shape.storage, shape.bf16, shape.width, [&](auto t, auto s, auto d) {
         using T = decltype(t);
         constexpr int S = s.value, D = d.value;
-        const CutPart tokens = most > 8 && most <= kFewRows
+        const CutPart tokens = alone && most > 8
                                    ? launch_tokens<T, S, D, 2>(a, maps, shape.sms, stream)
                                    : launch_tokens<T, S, D, 1>(a, maps, shape.sms, stream);
         launch_join<T, S, D>(a, tokens, chunks, stream);

@@ -46,12 +46,12 @@ struct CacheAttendShape {
 };
 
 // What a kernel leaves to be joined: its workspace, its CTAs, and the rows of
-// its items.  The join takes a slice of an item's rows a block.
-constexpr int kJoinRows = 8, kJoinSlice = 8;
+// its items.  The join takes 8 of an item's rows a block.
+constexpr int kJoinRows = 8;
 struct CutPart {
     unsigned char* workspace;
     int grid, rows;
-    __host__ __device__ int slices() const { return (rows + kJoinSlice - 1) / kJoinSlice; }
+    __host__ __device__ int slices() const { return rows / kJoinRows; }
     __host__ __device__ int blocks() const { return grid > 1 ? (grid - 1) * slices() : 0; }
 };
 

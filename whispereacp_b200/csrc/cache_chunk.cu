@@ -325,33 +325,6 @@ __device__ __forceinline__ float2 exp2_pair(uint64_t v) {
     const float2 x = pair_values(v);
     return make_float2(exp2_fast(x.x), exp2_fast(x.y));
 }
-// 2^x by arithmetic, for some of the elements, since the 16 exponentials a
-// cycle of an SM are what a softmax waits for: x = n + f with n the nearest
-// integer (adding 1.5 2^23 rounds to it and leaves it in the low bits), 2^f by
-// the polynomial of degree 4 whose largest relative error on [-1/2, 1/2] is the
-// smallest, 2^-18.5 (found by Remez's exchange), and n added to the exponent.
-// What is no number, or above 2^127, becomes 2^127 or more: the caller's check
-// of the sum finds it.
-__device__ __forceinline__ float2 exp2_computed(uint64_t v) {
-    const float2 y = pair_values(v);
-    const auto clamped = [](float z) {
-        float r;  // a NaN stays one, and its bits plus n's are a huge number's
-        asm("{\n\t.reg .f32 m;\n\tmax.NaN.f32 m, %1, 0fC2FC0000;\n\tmin.NaN.f32 %0, m, 0f42FE0000;\n\t}" : "=f"(r) : "f"(z));
-        return r;
-    };
-    const uint64_t x = pair_of(clamped(y.x), clamped(y.y));
-    const uint64_t t = add_pair(x, pair_of(12582912.f, 12582912.f));
-    const uint64_t n = add_pair(t, pair_of(-12582912.f, -12582912.f));
-    const uint64_t f = fma_pair(n, pair_of(-1.f, -1.f), x);
-    uint64_t p = fma_pair(f, pair_of(0x1.3997d6p-7f, 0x1.3997d6p-7f), pair_of(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    p = fma_pair(f, p, pair_of(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    p = fma_pair(f, p, pair_of(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    p = fma_pair(f, p, pair_of(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    const float2 a = pair_values(p), b = pair_values(t);
-    return make_float2(__uint_as_float(__float_as_uint(a.x) + (__float_as_uint(b.x) << 23)),
-                       __uint_as_float(__float_as_uint(a.y) + (__float_as_uint(b.y) << 23)));
-}
-
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -660,8 +633,6 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr float kShift = kHalf ? 4.f : 0.f;
     constexpr float kMost = kHalf ? 32768.f : 0x1p60f;
-    // Of 8 pairs of exponentials, those that the multipliers take.
-    constexpr int kComputed = 0;
     const int lane = threadIdx.x & 31, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(row & ~31) << 16;
     const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + Layout::out_column + t * D + lanes;
@@ -725,14 +696,14 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                         for (int e = 0; e < 32; ++e)
                             if (e >= seen) s[c & 1][e] = 0xff800000u;
                 };
-                const auto exponentials = [&](int c, auto computed) {
+                const auto exponentials = [&](int c) {
                     const uint64_t scale2 = pair_of(to_log2, to_log2), from2 = pair_of(-from, -from);
                     if ((c & 1) == 0) sums[0] = sums[1] = 0;
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         const uint64_t x = fma_pair(
                             pair_of(__uint_as_float(s[c & 1][e]), __uint_as_float(s[c & 1][e + 1])), scale2, from2);
-                        const float2 p = (e / 2) % 8 < decltype(computed)::value ? exp2_computed(x) : exp2_pair(x);
+                        const float2 p = exp2_pair(x);
                         sums[(e >> 1) & 1] = add_pair(sums[(e >> 1) & 1], pair_of(p.x, p.y));
                         w[c & 1][e / 2] = Half16<T>::pack2(p.x, p.y);
                     }
@@ -778,8 +749,8 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                             tmem_store32(o_at + c * 32, o);
                         }
                     }
-                    exponentials(2 * half, std::integral_constant<int, 0>{});
-                    exponentials(2 * half + 1, std::integral_constant<int, 0>{});
+                    exponentials(2 * half);
+                    exponentials(2 * half + 1);
                 };
                 const auto store = [&](int half) {
                     sum += part[half];
@@ -792,15 +763,14 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                     __syncwarp();
                     if (lane == 0) cache_arrive(bar.p + 2 * t + half);
                 };
-                const std::integral_constant<int, kComputed> computed;
                 tmem_load32_begin(s_at, s[0]);
                 take(0);
                 tmem_load32_begin(s_at + 32, s[1]);
                 if (ready) {
-                    exponentials(0, computed);
+                    exponentials(0);
                     take(1);
                     tmem_load32_begin(s_at + 64, s[0]);
-                    exponentials(1, computed);
+                    exponentials(1);
                 } else {
                     part[0] = INFINITY;
                 }
@@ -811,10 +781,10 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                 store(0);
                 take(2);
                 tmem_load32_begin(s_at + 96, s[1]);
-                exponentials(2, computed);
+                exponentials(2);
                 hand_over(0);
                 take(3);
-                exponentials(3, computed);
+                exponentials(3);
                 if (__any_sync(0xffffffffu, !(part[1] <= kMost))) refer(1);
                 store(1);
                 hand_over(1);

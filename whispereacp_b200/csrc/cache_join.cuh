@@ -66,64 +66,61 @@ __global__ void __launch_bounds__(kThreads)
     const int tile_rows = part_of.rows, floats = partial_floats<D>(tile_rows);
     const CacheSequence q = cut.q;
     const int all_rows = (int)min((long long)tile_rows, (long long)q.rows * a.group - (long long)cut.tile * tile_rows);
-    const int end = min(all_rows, (slice + 1) * kJoinSlice);
-    for (int base = slice * kJoinSlice; base < end; base += kJoinRows) {
-        const int rows = min(kJoinRows, end - base);
-        int share = 1;  // warps of a row
-        while (share * 2 * rows <= kJoinWarps && share < cut.parts) share *= 2;
-        const int local = warp / share, sub = warp % share, row = base + local;
-        const bool active = local < rows;
-        float m = -INFINITY, sum = 0.f, o[kPer];
+    const int base = slice * kJoinRows, rows = min(kJoinRows, all_rows - base);
+    if (rows <= 0) return;
+    int share = 1;  // warps of a row
+    while (share * 2 * rows <= kJoinWarps && share < cut.parts) share *= 2;
+    const int local = warp / share, sub = warp % share, row = base + local;
+    const bool active = local < rows;
+    float m = -INFINITY, sum = 0.f, o[kPer];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-        const auto add = [&](float pm, float ps, const float* v) {
-            const float top = fmaxf(m, pm), from = top == -INFINITY ? 0.f : top;
-            const float keep = exp2_fast(m - from), gain = exp2_fast(pm - from);
-            sum = sum * keep + ps * gain;
+    for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+    const auto add = [&](float pm, float ps, const float* v) {
+        const float top = fmaxf(m, pm), from = top == -INFINITY ? 0.f : top;
+        const float keep = exp2_fast(m - from), gain = exp2_fast(pm - from);
+        sum = sum * keep + ps * gain;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) o[e] = o[e] * keep + v[e] * gain;
-            m = top;
-        };
-        if (active) {
-            const int from = (int)((long long)cut.parts * sub / share), to = (int)((long long)cut.parts * (sub + 1) / share);
+        for (int e = 0; e < kPer; ++e) o[e] = o[e] * keep + v[e] * gain;
+        m = top;
+    };
+    if (active) {
+        const int from = (int)((long long)cut.parts * sub / share), to = (int)((long long)cut.parts * (sub + 1) / share);
 #pragma unroll 4
-            for (int i = from; i < to; ++i) {
-                const float* part = partials + ((long long)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * floats;
-                float v[kPer];
+        for (int i = from; i < to; ++i) {
+            const float* part = partials + ((long long)(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * floats;
+            float v[kPer];
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) v[e] = part[row * D + lane * kPer + e];
-                add(part[tile_rows * D + row], part[tile_rows * (D + 1) + row], v);
-            }
+            for (int e = 0; e < kPer; ++e) v[e] = part[row * D + lane * kPer + e];
+            add(part[tile_rows * D + row], part[tile_rows * (D + 1) + row], v);
         }
-        if (share > 1) {
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) shared_o[warp][lane * kPer + e] = o[e];
-            if (lane == 0) {
-                shared_ml[warp][0] = m;
-                shared_ml[warp][1] = sum;
-            }
-            __syncthreads();
-            if (sub == 0)
-                for (int w = warp + 1; w < warp + share; ++w) add(shared_ml[w][0], shared_ml[w][1], &shared_o[w][lane * kPer]);
-        }
-        if (!active || sub != 0) continue;
-        const TileRow r = tile_row(a, q, cut.head, cut.tile * tile_rows + row);
-        if (!r.valid) continue;
-        const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
-        const long long at = (long long)q.first + r.token;
-        unsigned char* op = a.out + at * a.o_row + r.head * a.o_head + lane * (kPer * 2);
-        bool fine = true;
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) {
-            const float x = o[e] * inverse, y = o[e + 1] * inverse;
-            fine = fine && fabsf(x) + fabsf(y) < INFINITY;
-            *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(x, y);
-        }
-        if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
-        if (__any_sync(0xffffffffu, !fine) && r.seen > 0 && (cache_eight(S) || r.seen < q.length))
-            attend_row<T, S, D>(a, cut.sequence, q.first, q.before, q.length, r.token, r.head, nullptr);
     }
+    if (share > 1) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) shared_o[warp][lane * kPer + e] = o[e];
+        if (lane == 0) {
+            shared_ml[warp][0] = m;
+            shared_ml[warp][1] = sum;
+        }
+        __syncthreads();
+        if (sub == 0)
+            for (int w = warp + 1; w < warp + share; ++w) add(shared_ml[w][0], shared_ml[w][1], &shared_o[w][lane * kPer]);
+    }
+    if (!active || sub != 0) return;
+    const TileRow r = tile_row(a, q, cut.head, cut.tile * tile_rows + row);
+    if (!r.valid) return;
+    const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
+    const long long at = (long long)q.first + r.token;
+    unsigned char* op = a.out + at * a.o_row + r.head * a.o_head + lane * (kPer * 2);
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+        const float x = o[e] * inverse, y = o[e + 1] * inverse;
+        fine = fine && fabsf(x) + fabsf(y) < INFINITY;
+        *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(x, y);
+    }
+    if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
+    if (__any_sync(0xffffffffu, !fine) && r.seen > 0 && (cache_eight(S) || r.seen < q.length))
+        attend_row<T, S, D>(a, cut.sequence, q.first, q.before, q.length, r.token, r.head, nullptr);
 }
 
 // Joins the items that a call's kernels cut, the last of which it was launched
