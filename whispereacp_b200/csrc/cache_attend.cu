@@ -829,7 +829,7 @@ static long long few_rows_beside(const CacheAttendShape& shape) { return cache_e
 // One window's 224 rows over 450 keys x 20 heads, few-row and chunk kernel: fp16
 // 11.5 and 18.2 us, int8 11.5 and 24.8; with 12 to 15 units a CTA 21 and 23 us
 // (64 wide) but 37 and 29 (128 wide), with 30 34 and 27.
-constexpr int kSmallUnits = 8;
+constexpr int kSmallUnits = 10;
 static bool few_alone(const CacheAttendArgs& a, const CacheAttendShape& shape) {
     if ((long long)shape.max_rows * a.group <= few_rows(shape)) return true;
     const int keys = shape.width * cache_bytes(shape.storage) == 64 ? 128 : 64;
