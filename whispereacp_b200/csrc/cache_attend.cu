@@ -12,7 +12,8 @@
 // wherever items (sequence, head, tile) begin and end: ragged lengths cannot
 // unbalance it.  An item cut by a run's border leaves partial results (m, sum,
 // o) in the workspace, which cache_join_kernel adds in an order that the sizes
-// fix, so the result has the same bits every time.
+// fix, so the result has the same bits every time.  Short items go whole to a
+// CTA, and nothing is joined.
 //
 // In a CTA a producer warp copies units' keys and values into a ring of
 // shared-memory stages (bulk tensor copies, a box a page), and four warps take
@@ -28,7 +29,16 @@
 // multiplied unscaled.  A key's scale multiplies its score; a value's scale
 // multiplies its probability, relative to the warp's largest so far, so that
 // the product stays in fp16's range whatever the scales are; P is one fp16
-// here, whose 2^-12 is below what 8 bits leave of a value.  bf16 queries become fp16 after a power of two a row brings them near 1.
+// here, whose 2^-11 is below what 8 bits leave of a value.  bf16 queries
+// become fp16 after a power of two a row brings them near 1.
+//
+// Measured (6.54 TB/s is a copy's rate): one token of 12 sequences of up to
+// 32768 bf16 rows, 128 wide, 148 us for 967 MB, 6.5 TB/s; of 64 windows x 20
+// heads over 1500 int8 rows 53 us for 250 MB, 4.7 TB/s, where the widening's
+// instructions fill the issue slots beside the copies (57 % of them, 3 CTAs an
+// SM); of 64 windows over up to 448 bf16 rows 18 us for 66 MB, of which the
+// launch, the search of the list and an item's 2500 cycles are the most; of
+// one window 5.6 us, all latency.
 #include "cache_join.cuh"
 
 #include <algorithm>
@@ -74,7 +84,8 @@ __device__ __forceinline__ int item_units(int length) {
 }
 // What an item costs beside its units (its queries, the warps' meeting, its
 // results: 2500 cycles), in units (700 to 900): the list that the CTAs share
-// out counts it in front of the item's first unit.
+// out counts it in front of the item's first unit (64 ragged windows: 26.3 us
+// without, 20.5 with).
 template <int kKeys>
 constexpr int item_cost() {
     return kKeys == 64 ? 3 : 2;
@@ -813,22 +824,25 @@ CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, 
 // of 16: the chunk kernel's 128-row tiles cost the same for fewer, and its
 // 8-bit blocks the widening besides.  16 x 1500 keys x 8 heads, few-row and
 // chunk kernel: 32 fp16 rows 22 and 28 us (64 wide), 39 and 46 (128 wide, where
-// 4 x 8192 keys take 57 and 51, and 4 x 32768 171 and 113); 48 rows 28.5 and 28.8
-// (4 x 8192 31.6 and 31.3); 64 int8 rows 34 and 60, 57 and 97; 96 bf16 rows over
-// 64 x 450 int8 keys 82 and 79, 163 and 120.
+// 4 x 8192 keys take 57 and 51, and 4 x 32768 171 and 113); 48 fp16 rows 28.5 and
+// 28.8 (4 x 8192 31.6 and 31.3); 64 int8 rows 34 and 46 (64 x 450 keys 50 and
+// 59); 128 wide 48 int8 rows 46 and 64 (64 x 450 78 and 82), 64 of them 57 and
+// 65 but 94 and 84.
 static long long few_rows(const CacheAttendShape& shape) {
-    return cache_eight(shape.storage) ? 64 : shape.width == 64 ? 32 : 16;
+    if (cache_eight(shape.storage)) return shape.width == 64 ? 64 : 48;
+    return shape.width == 64 ? 32 : 16;
 }
 // And up to which a sequence is the few-row kernel's, in tiles of 8, beside
-// sequences of more: 12 of 48 sequences of up to 1200 keys x 8 heads with 32
-// rows, one with 200, taken by the few-row and by the chunk kernel: int8 43.5
-// and 48.8 us (64 wide), 59 and 72 (128 wide), fp16 36.0 and 31.9, 57 and 53.
-static long long few_rows_beside(const CacheAttendShape& shape) { return cache_eight(shape.storage) ? 32 : 16; }
+// sequences of more.  One of 48 sequences of up to 1200 keys x 8 heads has 200
+// rows, 11 have these, the others one, taken by the few-row and by the chunk
+// kernel: 20 int8 rows 35.0 and 40.3 us (64 wide), 53 and 54.5 (128 wide), 32 of
+// them 42.2 and 40.6, 56 and 55; 20 fp16 rows 34.6 and 31.1, 55 and 51.
+static long long few_rows_beside(const CacheAttendShape& shape) { return cache_eight(shape.storage) ? 24 : 16; }
 // Calls whose units, 16 rows each, come to this many for each of two CTAs an SM
 // at most are the few-row kernel's too, whatever their rows: it starts sooner.
 // One window's 224 rows over 450 keys x 20 heads, few-row and chunk kernel: fp16
-// 11.5 and 18.2 us, int8 11.5 and 24.8; with 12 to 15 units a CTA 21 and 23 us
-// (64 wide) but 37 and 29 (128 wide), with 30 34 and 27.
+// 11.5 and 17.9 us; with 15 units a CTA 21 and 23 us (64 wide) but 37 and 29
+// (128 wide), with 30 34 and 27.
 constexpr int kSmallUnits = 10;
 static bool few_alone(const CacheAttendArgs& a, const CacheAttendShape& shape) {
     if ((long long)shape.max_rows * a.group <= few_rows(shape)) return true;

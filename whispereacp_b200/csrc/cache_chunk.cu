@@ -10,16 +10,28 @@
 //
 //   warps 0-3, 4-7  the softmax of tile 0 and of tile 1, a thread a row: read
 //                   the scores from tensor memory, p = 2^(s - m), P as 16-bit
-//                   values back into the scores' columns (rounded once: what
-//                   the products take), the sum of p in a register.  The
-//                   maximum moves only when it grows by more than 2^8; then
-//                   the thread rescales its row of o in tensor memory.
+//                   values back into the scores' columns, half a block at a
+//                   time (rounded once to the queries' type, which the
+//                   products take: 2^-8 or 2^-11 of a probability, as much as
+//                   the output's own rounding, and of either sign), the
+//                   sum of p in a register.  m comes from the first block that
+//                   the row sees; it moves, and the row of o in tensor memory
+//                   is rescaled, only when a block's sum of P says so.
 //   warp 8          issues the products: S_t = Q_t K^T (both from shared
 //                   memory) and O_t += P_t V (P from tensor memory), those of
 //                   one tile while the other's softmax runs.
 //   warp 9          copies the blocks' keys and values into a ring, a box a
 //                   page, as the 128-byte-swizzled tiles the products read:
 //                   keys K-major, values MN-major, as they lie in the cache.
+//   warps 9-15      over 8-bit caches instead: bring the blocks in as they are
+//                   held and widen them into the ring.  A warp issues them at
+//                   its own latency, so their number counts: 8 sequences of
+//                   8192 int8 keys, 128 wide, 256 rows, took 231 us with three
+//                   warps, 198 with four, 151 with seven (at 128 registers a
+//                   thread, where the softmax has no scores on their way).
+//
+// 16-bit 64-wide heads have items of one tile, and an SM two CTAs, which then
+// are the two that take turns: ragged prompts of 32 windows 42 us against 47.
 //
 // Tensor memory: S_0, S_1 (128 columns each, P in the first 64), O_0, O_1 (D
 // columns each).  The order of products on one issuing thread is the order of
@@ -27,7 +39,17 @@
 // and the commit behind S_t also says that O_t stands still.
 //
 // The blocks of all items form one list, dealt evenly over the SMs as in
-// cache_attend.cu; cut items leave partial results for the join.
+// cache_attend.cu; cut items leave partial results for the join.  What an item
+// passes once (its queries, results, a rescaling) is kept in loops, not
+// unrolled: the code then stays in the instruction caches, and the widening's
+// loops likewise (64 x 450 int8 keys, 256 rows, 86 -> 71 us in all).
+//
+// Measured: two chunks of up to 1500 bf16 rows x 32 heads over up to 15.5k keys
+// of 8 heads, 128 wide, 0.66 ms for 664 GFLOP, 1.0 PFLOP/s of a matrix product's 1.63: a
+// block's scores, softmax and product follow one another, and two tiles in
+// turn do not hide all of that.  Ragged prompts of 32 windows (fp16, 64 wide,
+// 450 keys) 34.6 us, nearly all of it what an item and a launch cost; a mixed
+// batch of 48 sequences over e4m3, the few-row kernel's share behind it, 72 us.
 #include "cache_join.cuh"
 
 #include <algorithm>
@@ -50,7 +72,7 @@ struct ChunkLayout {
     static constexpr int ctas = 3 - tiles;
     static constexpr int rows = tiles * kTile;  // of an item
     static constexpr int mma_warp = 4 * tiles;
-    static constexpr int copy_warps = cache_eight(S) ? 3 : 1;
+    static constexpr int copy_warps = cache_eight(S) ? 7 : 1;
     static constexpr int threads = 32 * (mma_warp + 1 + copy_warps);
     static constexpr int columns = tiles == 1 ? 256 : 512;  // of tensor memory
     static constexpr int out_column = tiles * 128;
@@ -97,7 +119,7 @@ __device__ __forceinline__ int chunk_blocks(const CacheSequence& q, const CacheA
 }
 // What an item costs beside its blocks (queries, the first block's maximum,
 // results), in blocks: the list that the CTAs share out counts it in front of
-// the item's first block.
+// the item's first block (ragged prompts of 32 windows: 42 us without, 35 with).
 constexpr int kItemCost = 2;
 
 // A sequence's blocks.
@@ -413,7 +435,7 @@ __device__ __forceinline__ void widen_piece(const uint4& raw, uint32_t scale, ui
     }
 }
 
-// 8-bit caches: three warps bring the blocks in as they are held, four tiles
+// 8-bit caches: the warps bring the blocks in as they are held, four tiles
 // (keys or values of a block) deep, and write them into the ring widened to the
 // queries' type, each value times its scale (a power of two: exact in bf16, and
 // in fp16 wherever fp16 holds the result).
@@ -447,7 +469,7 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
                              : "memory");
             };
             if (me == 0) *reinterpret_cast<int*>(held + kPieces * 16 + kBlockKeys) = seen - j * kBlockKeys;
-#pragma unroll 2
+#pragma unroll 1
             for (int i = 0; i < (kPieces + 8 + kThreads - 1) / kThreads; ++i) {
                 const int piece = me + i * kThreads;
                 const bool scale = piece >= kPieces;  // 16 keys' scale bytes
@@ -492,7 +514,7 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
         const unsigned char* held = smem + Layout::held_at + (n % kDepth) * Layout::held_bytes;
         const int keys = *reinterpret_cast<const int*>(held + kPieces * 16 + kBlockKeys);  // seen; the others are zeros
         unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
-#pragma unroll 2
+#pragma unroll 1
         for (int piece = me; piece < kPieces; piece += kThreads) {
             const int key = piece / (D / 16), c = piece % (D / 16);
             uint32_t out[8];
@@ -633,6 +655,9 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr float kShift = kHalf ? 4.f : 0.f;
     constexpr float kMost = kHalf ? 32768.f : 0x1p60f;
+    // The next 32 scores on their way while 32 are worked on, where the
+    // registers reach for it; 8-bit caches' 512 threads have 128 each.
+    constexpr bool kAhead = !cache_eight(S);
     const int lane = threadIdx.x & 31, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(row & ~31) << 16;
     const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + Layout::out_column + t * D + lanes;
@@ -642,7 +667,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
     // The row's queries, swizzled as the copy engine does it.
     const auto give_queries = [&](const ChunkPlace& p, const TileRow& r) {
         const unsigned char* qp = a.queries + ((long long)p.q.first + r.token) * a.q_row + r.head * a.q_head;
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < Layout::halves; ++h) {
             uint4 v[8];
 #pragma unroll
@@ -718,7 +743,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int c = 2 * half; c < 2 * half + 2; ++c) {
-                        tmem_arrived(s[c & 1]);  // whatever is on its way
+                        if (kAhead) tmem_arrived(s[c & 1]);  // whatever is on its way
                         tmem_load32_begin(s_at + c * 32, s[c & 1]);
                         take(c);
 #pragma unroll
@@ -740,7 +765,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                             cache_wait(bar.first + t, h_parity, abort, a.status, kWaitFirst);
                             tmem_fence_after();
                         }
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             uint32_t o[32];
                             tmem_load32(o_at + c * 32, o);
@@ -765,24 +790,27 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                 };
                 tmem_load32_begin(s_at, s[0]);
                 take(0);
-                tmem_load32_begin(s_at + 32, s[1]);
+                if (kAhead) tmem_load32_begin(s_at + 32, s[1]);
                 if (ready) {
                     exponentials(0);
+                    if (!kAhead) tmem_load32_begin(s_at + 32, s[1]);
                     take(1);
-                    tmem_load32_begin(s_at + 64, s[0]);
+                    if (kAhead) tmem_load32_begin(s_at + 64, s[0]);
                     exponentials(1);
                 } else {
                     part[0] = INFINITY;
                 }
                 if (__any_sync(0xffffffffu, !(part[0] <= kMost))) {
                     refer(0);
-                    tmem_load32_begin(s_at + 64, s[0]);
+                    if (kAhead) tmem_load32_begin(s_at + 64, s[0]);
                 }
                 store(0);
+                if (!kAhead) tmem_load32_begin(s_at + 64, s[0]);
                 take(2);
-                tmem_load32_begin(s_at + 96, s[1]);
+                if (kAhead) tmem_load32_begin(s_at + 96, s[1]);
                 exponentials(2);
                 hand_over(0);
+                if (!kAhead) tmem_load32_begin(s_at + 96, s[1]);
                 take(3);
                 exponentials(3);
                 if (__any_sync(0xffffffffu, !(part[1] <= kMost))) refer(1);
@@ -815,7 +843,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         bool fine = true;
         unsigned char* op = a.out + at * a.o_row + r.head * a.o_head;
         if (active || !whole) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
                 if (active) tmem_load32(o_at + c * 32, o);

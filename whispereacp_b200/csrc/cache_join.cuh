@@ -125,7 +125,9 @@ __global__ void __launch_bounds__(kThreads)
 
 // Joins the items that a call's kernels cut, the last of which it was launched
 // behind: its launch overlaps that one's end.  Where items are far fewer than
-// CTAs, 16 warps share a row's many parts.
+// CTAs, 16 warps share a row's many parts: 32768 bf16 keys of one sequence, 8
+// heads, 31.4 us against 36.9 with 8; 64 sequences of 1500 int8 keys, 16 heads,
+// 46.7 against 43.5 (the rule's side).
 template <typename T, int S, int D>
 void launch_join(const CacheAttendArgs& a, const CutPart& first, const CutPart& second, cudaStream_t stream) {
     const int blocks = first.blocks() + second.blocks();
