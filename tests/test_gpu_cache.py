@@ -531,6 +531,25 @@ def test_scales_under_a_wide_table(monkeypatch, storage, dtype):
         test_a_scale_below_or_at_zero(storage, dtype, ([200, 300], [90, 130]), scale)
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("columns", [20, 9600])
+def test_first_keys_of_score_minus_infinity(dtype, width, columns):
+    """The first 70 keys weigh nothing: the row's first numbers come in the
+    middle of a block."""
+    import torch
+    cache = make_cache(dtype, 40, 2, 16, width, 401)
+    batch, starts = make_batch([300], [130], 16, 40, 402, columns=columns)
+    for p in range(70):
+        cache.keys[int(batch.page_table[0, p // 16]), :, p % 16] = -math.inf
+    q = queries(130, 2, width, dtype, 403).abs() + 0.01
+    out, lse = cache.attend(batch, q, return_lse=True)
+    k, v = held_rows(cache, batch.page_table[0], 300)
+    o, l, tol, lse_tol = expected(q, k[70:], v[70:], width ** -0.5, True, 100)
+    assert bool(((out.double() - o).abs() <= tol).all())
+    assert bool(((lse.double() - l).abs() <= lse_tol).all())
+
+
 def test_two_streams_under_a_wide_table(monkeypatch):
     wide_batches(monkeypatch)
     test_two_streams_at_once()

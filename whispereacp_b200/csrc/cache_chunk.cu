@@ -813,7 +813,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                 if (!kAhead) tmem_load32_begin(s_at + 96, s[1]);
                 take(3);
                 exponentials(3);
-                if (__any_sync(0xffffffffu, !(part[1] <= kMost))) refer(1);
+                if (!ready || __any_sync(0xffffffffu, !(part[1] <= kMost))) refer(1);
                 store(1);
                 hand_over(1);
                 h_parity ^= 1;
