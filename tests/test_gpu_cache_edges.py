@@ -1,0 +1,108 @@
+"""The paged cache's attention where held numbers leave the usual range:
+infinities and NaN, scales far apart, rows that see nothing, and what a call
+keeps, against the definition in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+
+from tests.test_gpu_cache import CHUNKS, EIGHT, FEW, PAIRS, TOKENS, dt, held_rows, make_batch, make_cache, queries
+
+pytestmark = pytest.mark.gpu
+
+EIGHT_PAIRS = [p for p in PAIRS if p[0] in EIGHT]
+
+
+def place(cache, batch, s, position):
+    """(page, row) of a position of sequence s."""
+    return int(batch.page_table[s, position // cache.page_rows]), position % cache.page_rows
+
+
+def definition(q, k, v, scale, causal, first):
+    """(out, lse, tolerance of out, of lse) of one sequence's rows, in 64 bits,
+    with the tolerances of tests/test_gpu_cache.py's `expected`, all rows at
+    once.  Values that are no numbers count where a row sees them only."""
+    import torch
+    n, heads, width = q.shape
+    length, group = k.shape[0], heads // k.shape[1]
+    u = torch.finfo(q.dtype).eps / 2
+    tiny = torch.finfo(q.dtype).tiny
+    if length == 0:
+        zeros = torch.zeros(n, heads, width, dtype=torch.float64, device=q.device)
+        lse = torch.full((n, heads), -math.inf, dtype=torch.float64, device=q.device)
+        return zeros, lse, zeros + tiny, torch.zeros_like(lse)
+    q64 = q.double().transpose(0, 1)                                               # [heads, n, width]
+    k, v = (x.repeat_interleave(group, 1).permute(1, 2, 0) for x in (k, v))        # [heads, width, length]
+    seen = torch.arange(length, device=q.device)[None] <= first + torch.arange(n, device=q.device)[:, None]
+    if not causal:
+        seen = torch.ones_like(seen)
+    some = seen.any(1)
+    s = ((q64 @ k) * scale).masked_fill(~seen, -math.inf)
+    big = ((q64.abs() @ k.abs()) * abs(scale)).masked_fill(~seen, 0).amax(2)       # [heads, n]
+    lse = torch.logsumexp(s, 2)
+    p = torch.exp(s - torch.where(some, lse, torch.zeros_like(lse))[..., None])
+    finite = torch.where(torch.isfinite(v), v, torch.zeros_like(v)).transpose(1, 2)
+    out, a = p @ finite, p @ finite.abs()
+    of = seen.double()[None].expand(heads, -1, -1)
+    held = [(of @ x.double().transpose(1, 2)) > 0 for x in (torch.isnan(v), torch.isposinf(v), torch.isneginf(v))]
+    out = torch.where(held[1], out + math.inf, out)
+    out = torch.where(held[2], out - math.inf, out)
+    out = torch.where(held[0], torch.full_like(out, math.nan), out)
+    each = (width + 3) * 2.0 ** -24 * big + 2.0 ** -18
+    count = seen.sum(1).double()
+    tol = u * out.abs() + (u + 2 * each + count * 2.0 ** -24)[..., None] * a + tiny
+    lse_tol = each + count * 2.0 ** -24 + 2.0 ** -23 * lse.abs()
+    return out.transpose(0, 1), lse.T, tol.transpose(0, 1), lse_tol.T
+
+
+def check(cache, batch, starts, q, out, lse, scale, causal=True):
+    """The sequences' rows against the definition; a result that is above the
+    type's largest, by its tolerance too, has to be an infinity."""
+    import torch
+    got, got_lse = out.double(), lse.double()
+    for s in range(len(starts) - 1):
+        a, b = int(starts[s]), int(starts[s + 1])
+        if a == b:
+            continue
+        length = int(batch.lengths[s])
+        k, v = held_rows(cache, batch.page_table[s], length)
+        o, l, tol, lse_tol = definition(q[a:b], k, v, scale, causal, length - (b - a))
+        at, largest = (s, length, b - a), torch.finfo(q.dtype).max
+        assert torch.equal(torch.isnan(got[a:b]), torch.isnan(o)), at
+        infinite = torch.isinf(o) | (o.abs() - tol > largest)
+        assert torch.equal(got[a:b][infinite], torch.sign(o[infinite]) * math.inf), at
+        fine = torch.isfinite(o) & (o.abs() + tol < largest)
+        off = (got[a:b] - o).abs()
+        assert bool((off <= tol)[fine].all()), (*at, float((off / tol)[fine].max()))
+        assert torch.equal(torch.isnan(got_lse[a:b]), torch.isnan(l)), at
+        assert torch.equal(torch.isneginf(got_lse[a:b]), torch.isneginf(l)), at
+        fine = torch.isfinite(l)
+        off = (got_lse[a:b] - l).abs()
+        assert bool((off <= lse_tol)[fine].all()), (*at, float((off / lse_tol)[fine].max()))
+
+
+def pages_of(lengths, page_rows):
+    return sum(-(-n // page_rows) for n in lengths) + 2
+
+
+# The rows a call brings, and a table's columns: what a table has places for
+# decides which kernel takes a call, and whether items are cut.
+SHAPES = [(TOKENS, None), (FEW, None), (FEW, 600), (CHUNKS, None), (CHUNKS, 9600)]
+
+
+@pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_a_value_row_that_was_no_number_makes_those_that_see_it_none(storage, dtype, width, rows, columns):
+    """Scale byte 255 of a value row reads as NaN, and so does what sees it."""
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, width, 511)
+    batch, starts = make_batch(lengths, new, 16, pages, 512, columns=columns)
+    for s, n in enumerate(lengths):
+        if n > 2:
+            page, row = place(cache, batch, s, n // 2)
+            cache.value_scales[page, 0, row] = 255
+    q = queries(int(starts[-1]), 4, width, dtype, 513)
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, width ** -0.5)

@@ -572,8 +572,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                             const int at = warp * kWarpKeys + i * 16 + g + 8 * h;
                             int byte = scales[Layout::keys + at];
                             if (masked && key0 + i * 16 + g + 8 * h >= p.q.length) byte = 0;
-                            // 2^(byte - 127), infinity for 255: its hi + lo is a NaN
-                            factor[i][h] = __uint_as_float((uint32_t)byte << 23);
+                            factor[i][h] = cache_scale(byte);  // a NaN for 255, and so is what meets it
                             above |= byte > largest && byte < 255;
                         }
                 }
