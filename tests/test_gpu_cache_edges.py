@@ -106,3 +106,23 @@ def test_a_value_row_that_was_no_number_makes_those_that_see_it_none(storage, dt
     q = queries(int(starts[-1]), 4, width, dtype, 513)
     out, lse = cache.attend(batch, q, return_lse=True)
     check(cache, batch, starts, q, out, lse, width ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_an_infinity_among_the_values_stays_one(dtype, width, rows, columns):
+    """A seen value of infinity makes its column infinite, not NaN, and no
+    other column anything else."""
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(dtype, pages, 2, 16, width, 521)
+    batch, starts = make_batch(lengths, new, 16, pages, 522, columns=columns)
+    for s, n in enumerate(lengths):
+        if n:
+            page, row = place(cache, batch, s, n // 2)
+            cache.values[page, 0, row, 5] = -math.inf
+            cache.values[page, 1, row, 40] = math.inf
+    q = queries(int(starts[-1]), 4, width, dtype, 523)
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, width ** -0.5)

@@ -278,6 +278,17 @@ __device__ __forceinline__ float narrow_queries(uint32_t (&qf)[D / 16][2]) {
     return fine ? __uint_as_float((uint32_t)(e - 8) << 23) : 1.f;  // 2^(e - 135)
 }
 
+// The consumer warps' barrier; whether any of their threads says so.
+__device__ __forceinline__ bool workers_any(bool v) {
+    int any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.s32 %0, 1, 0, q;\n\t}\n"
+        : "=r"(any)
+        : "r"((int)v)
+        : "memory");
+    return any != 0;
+}
+
 // A grid that was launched behind another, whose results it does not read,
 // ends behind it all the same: who waits for this one waits for both.
 __device__ __forceinline__ void ends_behind() { wait_for_kernel_before(); }
@@ -730,6 +741,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const bool whole = p.unit == 0 && last == p.units;
         constexpr int kRowThreads = D / 2;  // a thread two columns of a row
+        bool broken = false;                // a result of this thread's is not finite
         float* part = partials + ((long long)blockIdx.x * 2 + (p.unit > 0 ? 0 : 1)) * partial_floats<D>(kRows);
         for (int row = threadIdx.x / kRowThreads; row < valid; row += 128 / kRowThreads) {
             const int d = (threadIdx.x % kRowThreads) * 2;
@@ -762,20 +774,20 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
             v.y *= inverse;
             *reinterpret_cast<uint32_t*>(a.out + at * a.o_row + r.head * a.o_head + d * 2) = Half16<T>::pack2(v.x, v.y);
             if (a.lse && d == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (top + log2f(all)) * kLn2 : -INFINITY;
-            if (!(fabsf(v.x) + fabsf(v.y) < INFINITY) && r.seen < p.q.length && r.seen > 0) atomicOr(redo, 1 << row);
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (a.causal && p.q.rows > 1 && whole) {
-            const int again = *reinterpret_cast<volatile int*>(redo);
-            if (again) {
-                for (int row = warp; row < kRows; row += kWorkers)
-                    if (again >> row & 1) {
-                        const TileRow r = tile_row(a, p.q, p.head, p.tile * kRows + row);
-                        attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, r.token, r.head, abort + kBeatWord);
-                    }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (threadIdx.x == 0) *redo = 0;
+            if (!(fabsf(v.x) + fabsf(v.y) < INFINITY) && r.seen > 0) {
+                atomicOr(redo, 1 << row);
+                broken = true;
             }
+        }
+        if (workers_any(broken)) {
+            const int again = *reinterpret_cast<volatile int*>(redo);
+            for (int row = warp; row < kRows; row += kWorkers)
+                if (again >> row & 1) {
+                    const TileRow r = tile_row(a, p.q, p.head, p.tile * kRows + row);
+                    attend_row<T, S, D>(a, p.s, p.q.first, p.q.before, p.q.length, r.token, r.head, abort + kBeatWord);
+                }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (threadIdx.x == 0) *redo = 0;
         }
         p = pn;
 #pragma unroll

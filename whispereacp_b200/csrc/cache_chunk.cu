@@ -876,8 +876,8 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             part[Layout::rows * D + t * kTile + row] = log_sum;
             part[Layout::rows * (D + 1) + t * kTile + row] = sum;
         }
-        // Rows that a key behind them made no number.
-        unsigned again = __ballot_sync(0xffffffffu, whole && r.valid && !fine && r.seen > 0 && (cache_eight(S) || r.seen < p.q.length));
+        // Rows that are no numbers (attend_row).
+        unsigned again = __ballot_sync(0xffffffffu, whole && r.valid && !fine && r.seen > 0);
         while (again) {
             const int i = __ffs(again) - 1;
             again &= again - 1;

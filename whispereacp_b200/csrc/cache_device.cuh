@@ -136,11 +136,12 @@ __device__ __forceinline__ void widen4(uint32_t bytes, bool interleaved, uint32_
 
 // One row of one query head by one warp, key by key: o = sum_j p_j v_j / sum_j
 // p_j with p_j = exp(s_j - max), the maximum and both sums running.  Only keys
-// the row sees are read.  The tiled kernels multiply whole tiles, where an
-// infinity or NaN among the values of a key behind the row (0 times it) makes
-// the row NaN; such rows, which see fewer keys than the sequence holds, come
-// here.  16 keys share a page, and 4 of them are on their way at once.  `beat`
-// (null: nobody waits) changes every 16 keys.
+// the row sees are read.  The tiled kernels multiply whole tiles by P of 16
+// bits, or of two: an infinity or NaN among the values of a key behind the row
+// (0 times it) makes the row NaN there, and so may a seen infinity (P's lower
+// half is 0 or negative).  Rows whose results are not finite come here, and
+// have here what the definition says.  16 keys share a page, and 4 of them are
+// on their way at once.  `beat` (null: nobody waits) changes every 16 keys.
 template <typename T, int S, int D>
 __device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int first, int before, int length, int i,
                                         int head, volatile int* beat) {

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads)
         *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(x, y);
     }
     if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
-    if (__any_sync(0xffffffffu, !fine) && r.seen > 0 && (cache_eight(S) || r.seen < q.length))
+    if (__any_sync(0xffffffffu, !fine) && r.seen > 0)
         attend_row<T, S, D>(a, cut.sequence, q.first, q.before, q.length, r.token, r.head, nullptr);
 }
 
