@@ -126,3 +126,31 @@ def test_an_infinity_among_the_values_stays_one(dtype, width, rows, columns):
     q = queries(int(starts[-1]), 4, width, dtype, 523)
     out, lse = cache.attend(batch, q, return_lse=True)
     check(cache, batch, starts, q, out, lse, width ** -0.5)
+
+
+@pytest.mark.parametrize("storage,dtype", PAIRS)
+@pytest.mark.parametrize("columns", [None, 40, 9600])
+def test_rows_that_see_nothing_beside_values_that_are_no_numbers(storage, dtype, columns):
+    """More new rows than a length holds: the first rows see no key and get
+    zeros, whatever the values hold that other rows of their tile see."""
+    import torch
+    for lengths, new in (([3, 1], [5, 7]), ([70, 300], [150, 310])):
+        pages = pages_of(lengths, 16)
+        cache = make_cache(storage, pages, 2, 16, 64, 501)
+        batch, starts = make_batch(lengths, new, 16, pages, 502, columns=columns)
+        for s, n in enumerate(lengths):
+            for position in (0, n - 1):
+                page, row = place(cache, batch, s, position)
+                if storage in EIGHT:
+                    cache.value_scales[page, :, row] = 255
+                else:
+                    cache.values[page, :, row, 3] = math.nan
+                    cache.values[page, :, row, 60] = math.inf
+        q = queries(int(starts[-1]), 4, 64, dtype, 503)
+        out, lse = cache.attend(batch, q, return_lse=True)
+        for s, n in enumerate(lengths):
+            a = int(starts[s])
+            b = a + new[s] - n
+            assert bool((out[a:b] == 0).all()) and bool(torch.isneginf(lse[a:b]).all()), s
+        check(cache, batch, starts, q, out, lse, 0.125)
+        cache.check()

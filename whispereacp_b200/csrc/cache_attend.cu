@@ -768,10 +768,11 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
             }
             const TileRow r = tile_row(a, p.q, p.head, p.tile * kRows + row);
             if (!r.valid) continue;
-            const float inverse = r.seen > 0 ? 1.f / all : 0.f;
+            // A row without a key is zeros whatever the tile's other rows met.
+            const float inverse = 1.f / all;
             const long long at = (long long)p.q.first + r.token;
-            v.x *= inverse;
-            v.y *= inverse;
+            v.x = r.seen > 0 ? v.x * inverse : 0.f;
+            v.y = r.seen > 0 ? v.y * inverse : 0.f;
             *reinterpret_cast<uint32_t*>(a.out + at * a.o_row + r.head * a.o_head + d * 2) = Half16<T>::pack2(v.x, v.y);
             if (a.lse && d == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (top + log2f(all)) * kLn2 : -INFINITY;
             if (!(fabsf(v.x) + fabsf(v.y) < INFINITY) && r.seen > 0) {

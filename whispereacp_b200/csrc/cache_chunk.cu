@@ -837,7 +837,8 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             tmem_fence_after();
         }
         const bool whole = p.block == 0 && last == p.blocks;
-        const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
+        const bool some = r.seen > 0;  // a row without a key is zeros whatever the tile's other rows met
+        const float inverse = 1.f / sum;
         const float log_sum = unset ? -INFINITY : from;
         float* part = cut_partials(a.workspace, gridDim.x) + ((long long)blockIdx.x * 2 + (p.block > 0 ? 0 : 1)) * partial_floats<D>(Layout::rows);
         bool fine = true;
@@ -857,7 +858,8 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                         uint32_t w[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float x = __uint_as_float(o[e + 2 * i]) * inverse, y = __uint_as_float(o[e + 2 * i + 1]) * inverse;
+                            const float x = some ? __uint_as_float(o[e + 2 * i]) * inverse : 0.f;
+                            const float y = some ? __uint_as_float(o[e + 2 * i + 1]) * inverse : 0.f;
                             fine = fine && fabsf(x) + fabsf(y) < INFINITY;
                             w[i] = Half16<T>::pack2(x, y);
                         }
@@ -871,13 +873,13 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                 }
             }
         }
-        if (r.valid && whole && a.lse) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (log_sum + log2f(sum)) * kLn2 : -INFINITY;
+        if (r.valid && whole && a.lse) a.lse[at * a.query_heads + r.head] = some ? (log_sum + log2f(sum)) * kLn2 : -INFINITY;
         if (r.valid && !whole) {
             part[Layout::rows * D + t * kTile + row] = log_sum;
             part[Layout::rows * (D + 1) + t * kTile + row] = sum;
         }
         // Rows that are no numbers (attend_row).
-        unsigned again = __ballot_sync(0xffffffffu, whole && r.valid && !fine && r.seen > 0);
+        unsigned again = __ballot_sync(0xffffffffu, whole && r.valid && !fine && some);
         while (again) {
             const int i = __ffs(again) - 1;
             again &= again - 1;

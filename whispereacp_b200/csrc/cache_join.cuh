@@ -108,18 +108,19 @@ __global__ void __launch_bounds__(kThreads)
     if (!active || sub != 0) return;
     const TileRow r = tile_row(a, q, cut.head, cut.tile * tile_rows + row);
     if (!r.valid) return;
-    const float inverse = r.seen > 0 ? 1.f / sum : 0.f;
+    const bool some = r.seen > 0;  // a row without a key is zeros whatever the tile's other rows met
+    const float inverse = 1.f / sum;
     const long long at = (long long)q.first + r.token;
     unsigned char* op = a.out + at * a.o_row + r.head * a.o_head + lane * (kPer * 2);
     bool fine = true;
 #pragma unroll
     for (int e = 0; e < kPer; e += 2) {
-        const float x = o[e] * inverse, y = o[e + 1] * inverse;
+        const float x = some ? o[e] * inverse : 0.f, y = some ? o[e + 1] * inverse : 0.f;
         fine = fine && fabsf(x) + fabsf(y) < INFINITY;
         *reinterpret_cast<uint32_t*>(op + e * 2) = Half16<T>::pack2(x, y);
     }
-    if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = r.seen > 0 ? (m + log2f(sum)) * kLn2 : -INFINITY;
-    if (__any_sync(0xffffffffu, !fine) && r.seen > 0)
+    if (a.lse && lane == 0) a.lse[at * a.query_heads + r.head] = some ? (m + log2f(sum)) * kLn2 : -INFINITY;
+    if (__any_sync(0xffffffffu, !fine) && some)
         attend_row<T, S, D>(a, cut.sequence, q.first, q.before, q.length, r.token, r.head, nullptr);
 }
 
