@@ -6,7 +6,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_gpu_cache import CHUNKS, EIGHT, FEW, PAIRS, TOKENS, dt, held_rows, make_batch, make_cache, queries
+from tests.test_gpu_cache import CHUNKS, EIGHT, FEW, PAIRS, TOKENS, dt, held_rows, make_batch, make_cache, queries, scale_of
 
 pytestmark = pytest.mark.gpu
 
@@ -18,10 +18,16 @@ def place(cache, batch, s, position):
     return int(batch.page_table[s, position // cache.page_rows]), position % cache.page_rows
 
 
-def definition(q, k, v, scale, causal, first):
+def definition(q, k, v, scale, causal, first, sizes=None):
     """(out, lse, tolerance of out, of lse) of one sequence's rows, in 64 bits,
     with the tolerances of tests/test_gpu_cache.py's `expected`, all rows at
-    once.  Values that are no numbers count where a row sees them only."""
+    once.  Values that are no numbers count where a row sees them only.
+
+    `sizes` are the scales [length, heads] of 8-bit values, for rows whose
+    probabilities span more than an fp16 does: P times its value's scale is one
+    fp16, where the row's largest stands at 2^6 at least and a half step is 2^-25,
+    so each value v held as v / size is off by up to 2^-31 max_j(p_j size_j) /
+    size of itself."""
     import torch
     n, heads, width = q.shape
     length, group = k.shape[0], heads // k.shape[1]
@@ -51,13 +57,18 @@ def definition(q, k, v, scale, causal, first):
     each = (width + 3) * 2.0 ** -24 * big + 2.0 ** -18
     count = seen.sum(1).double()
     tol = u * out.abs() + (u + 2 * each + count * 2.0 ** -24)[..., None] * a + tiny
+    if sizes is not None:
+        sizes = sizes.repeat_interleave(group, 1).T                                # [heads, length]
+        weight = (p * sizes[:, None]).amax(2, keepdim=True)
+        tol = tol + 2.0 ** -31 * weight * (of @ (finite.abs() / sizes[..., None]))
     lse_tol = each + count * 2.0 ** -24 + 2.0 ** -23 * lse.abs()
     return out.transpose(0, 1), lse.T, tol.transpose(0, 1), lse_tol.T
 
 
-def check(cache, batch, starts, q, out, lse, scale, causal=True):
+def check(cache, batch, starts, q, out, lse, scale, causal=True, spread=False):
     """The sequences' rows against the definition; a result that is above the
-    type's largest, by its tolerance too, has to be an infinity."""
+    type's largest, by its tolerance too, has to be an infinity.  `spread`: the
+    probabilities span more than an fp16 does."""
     import torch
     got, got_lse = out.double(), lse.double()
     for s in range(len(starts) - 1):
@@ -66,7 +77,11 @@ def check(cache, batch, starts, q, out, lse, scale, causal=True):
             continue
         length = int(batch.lengths[s])
         k, v = held_rows(cache, batch.page_table[s], length)
-        o, l, tol, lse_tol = definition(q[a:b], k, v, scale, causal, length - (b - a))
+        sizes = None
+        if spread and length:
+            pages = batch.page_table[s, :-(-length // cache.page_rows)].long()
+            sizes = scale_of(cache.value_scales[pages]).transpose(1, 2).reshape(-1, cache.heads)[:length]
+        o, l, tol, lse_tol = definition(q[a:b], k, v, scale, causal, length - (b - a), sizes)
         at, largest = (s, length, b - a), torch.finfo(q.dtype).max
         assert torch.equal(torch.isnan(got[a:b]), torch.isnan(o)), at
         infinite = torch.isinf(o) | (o.abs() - tol > largest)
@@ -154,3 +169,68 @@ def test_rows_that_see_nothing_beside_values_that_are_no_numbers(storage, dtype,
             assert bool((out[a:b] == 0).all()) and bool(torch.isneginf(lse[a:b]).all()), s
         check(cache, batch, starts, q, out, lse, 0.125)
         cache.check()
+
+
+@pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("jump", [24, 40, 80])
+@pytest.mark.parametrize("rows,columns", [(FEW, None), (FEW, 600), (CHUNKS, None), (CHUNKS, 9600)])
+def test_a_large_value_behind_a_row_cannot_change_it(storage, dtype, width, jump, rows, columns):
+    """The last new row's values are 2^jump times the others."""
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, width, 531)
+    batch, starts = make_batch(lengths, new, 16, pages, 532, columns=columns)
+    q = queries(int(starts[-1]), 4, width, dtype, 533)
+    for s, n in enumerate(lengths):
+        if new[s] > 1:
+            page, row = place(cache, batch, s, n - 1)
+            cache.value_scales[page, :, row] += jump
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, width ** -0.5)
+
+
+@pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("jump", [30, 60, 90])
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_a_large_value_of_little_weight(storage, dtype, width, jump, rows, columns):
+    """A seen key whose probability is about 2^-60 of the others' and whose
+    value is 2^jump times theirs."""
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, width, 541)
+    batch, starts = make_batch(lengths, new, 16, pages, 542, columns=columns)
+    q = queries(int(starts[-1]), 4, width, dtype, 543).abs()
+    for s, n in enumerate(lengths):
+        if n > 3:
+            for position in (1, n // 2):
+                page, row = place(cache, batch, s, position)
+                # -100 a column: scores of -60 in log2 at |q| of 0.8 each
+                cache.keys[page, :, row] = -100 if storage == "int8" else -96.0
+                size = 60 * math.log(2) / (width ** -0.5 * 0.8 * width * 100)
+                cache.key_scales[page, :, row] = 127 + round(math.log2(size))
+                cache.value_scales[page, :, row] += jump
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, width ** -0.5, spread=True)
+
+
+@pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_value_scales_over_their_whole_range(storage, dtype, width, rows, columns):
+    """Every row's values at a scale of its own, from 2^-100 to 2^0, their
+    largest first and last, and columns in which the large rows hold zeros."""
+    import torch
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, width, 551)
+    batch, starts = make_batch(lengths, new, 16, pages, 552, columns=columns)
+    g = torch.Generator("cuda").manual_seed(553)
+    cache.value_scales.copy_(torch.randint(27, 128, cache.value_scales.shape, generator=g, device="cuda").to(torch.uint8))
+    large = cache.value_scales > 60
+    values = cache.values.view(torch.uint8)
+    values[..., 7] = torch.where(large, torch.zeros_like(values[..., 7]), values[..., 7])
+    q = queries(int(starts[-1]), 4, width, dtype, 554)
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, width ** -0.5)

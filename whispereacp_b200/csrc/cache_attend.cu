@@ -26,15 +26,17 @@
 // the rescaling of o are rare.  The warps' results meet once per item.
 //
 // 8-bit keys and values become fp16 exactly (both types fit) and are
-// multiplied unscaled.  A key's scale multiplies its score; a value's scale
-// multiplies its probability, relative to the warp's largest so far, so that
-// the product stays in fp16's range whatever the scales are; P is one fp16
-// here, whose 2^-11 is below what 8 bits leave of a value.  bf16 queries
-// become fp16 after a power of two a row brings them near 1.
+// multiplied unscaled.  A key's scale multiplies its score, a value's scale its
+// P, and the reference of a row's exponentials follows the largest of these
+// products, over the keys that the row sees: one that it does not see, or that
+// weighs nothing, leaves it alone whatever its scale.  P is one fp16 here,
+// rounded by 2^-11 at most down to 2^-21 of the row's largest and by 2^-32 of
+// that below (a hi + lo cost 3 us of 56 on 64 windows over int8 cross rows).
+// bf16 queries become fp16 after a power of two a row brings them near 1.
 //
 // Measured (6.54 TB/s is a copy's rate): one token of 12 sequences of up to
 // 32768 bf16 rows, 128 wide, 148 us for 967 MB, 6.5 TB/s; of 64 windows x 20
-// heads over 1500 int8 rows 53 us for 250 MB, 4.7 TB/s, where the widening's
+// heads over 1500 int8 rows 52 us for 250 MB, 4.8 TB/s, where the widening's
 // instructions fill the issue slots beside the copies (57 % of them, 3 CTAs an
 // SM); of 64 windows over up to 448 bf16 rows 18 us for 66 MB, of which the
 // launch, the search of the list and an item's 2500 cycles are the most; of
@@ -250,6 +252,23 @@ __device__ __forceinline__ void load_queries(const CacheAttendArgs& a, const Pla
     }
 }
 
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Over 8-bit values the reference of a row's exponentials is such that the
+// largest product of P and a value's scale stands between 2^7 and 2^15, unless P
+// itself would pass 2^kFar and 2^8 of it (rows of zeros have scales of next to
+// nothing), which sums of 2^31 keys bear.
+constexpr float kFar = 80.f;
+// A row is computed again alone where that leaves its sum below kLeastSum, so
+// that smaller P underflow, or where the row's sum times the least scale among
+// its keys is below kLeastScaled: columns in which the values of large scales are
+// zeros are the small ones' alone.  The second takes scales 2^13 apart.
+constexpr float kLeastSum = 0x1p-95f, kLeastScaled = 0x1p-6f;
+
 // bf16 queries of an 8-bit cache as fp16, which holds a bf16 exactly between
 // 2^-14 and 2^15: a power of two brings the row's largest to 2^8.., and its
 // inverse is returned.
@@ -462,6 +481,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         }
         // Keys below `clear` are seen by every row of the tile.
         const int clear = a.causal ? tile_row(a, p.q, p.head, p.tile * kRows).seen : p.q.length;
+        const int reach = tile_row(a, p.q, p.head, p.tile * kRows + valid - 1).seen;  // and below this by its last
         uint32_t qn[NT][kSteps][2];  // the next item's
         Place pn = p;
         if (!a.uncut && left <= item_cost<Layout::keys>()) left = 0;  // nothing behind this item but a cost
@@ -477,13 +497,14 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[k][j][e] = 0.f;
         // The reference of the exponentials (0 until a key is seen), how far
-        // above it a score may be, and the sum of this lane's keys.
+        // above it a score may be, and the sum of this lane's keys.  Over 8
+        // bits, the least byte above 8, less 9, that a row of the tile met.
         float from[NT][2], limit[NT][2], sum[NT][2];
+        uint32_t least = 0xffffffffu;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) from[j][e] = sum[j][e] = 0.f, limit[j][e] = -INFINITY;
-        int largest = 8;  // the value scales' largest byte so far
 
         for (int t = p.unit; t < last; ++t) {
             cache_wait(full + stage, parity, abort, a.status, kWaitFull);
@@ -547,6 +568,24 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                 // x = log2 of the probability, relative; s stays.
                 float x[MK][NT][4], factor[MK][2];
                 const bool masked = key0 + kWarpKeys > clear;
+                // What a score counts beside: log2 of its value's scale less 7,
+                // so that the largest P, scaled, is brought to 2^7; and P alone
+                // to 2^kFar at most.
+                float beside[kEight ? MK : 1][2];
+                if constexpr (kEight)
+#pragma unroll
+                    for (int i = 0; i < MK; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t byte = scales[Layout::keys + warp * kWarpKeys + i * 16 + g + 8 * h];
+                            factor[i][h] = __uint_as_float(byte << 23);  // infinity for 255
+                            beside[i][h] = fmaxf(log2_fast(factor[i][h]) - 7.f, -kFar);
+                            if (!masked || key0 + i * 16 + g + 8 * h < reach) least = min(least, byte - 9u);
+                        }
+                const auto counted = [&](float v, int i, int h) {
+                    if constexpr (kEight) return v + beside[i][h];
+                    else return v;
+                };
                 const auto relative = [&] {
 #pragma unroll
                     for (int i = 0; i < MK; ++i)
@@ -570,47 +609,25 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(x[0][j][e], x[0][j][e + 2]);
+                        float top = fmaxf(counted(x[0][j][e], 0, 0), counted(x[0][j][e + 2], 0, 1));
 #pragma unroll
-                        for (int i = 1; i < MK; ++i) top = fmaxf(top, fmaxf(x[i][j][e], x[i][j][e + 2]));
+                        for (int i = 1; i < MK; ++i) top = fmaxf(top, fmaxf(counted(x[i][j][e], i, 0), counted(x[i][j][e + 2], i, 1)));
                         above |= top > limit[j][e];
                     }
-                if constexpr (kEight) {
-#pragma unroll
-                    for (int i = 0; i < MK; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int at = warp * kWarpKeys + i * 16 + g + 8 * h;
-                            int byte = scales[Layout::keys + at];
-                            if (masked && key0 + i * 16 + g + 8 * h >= p.q.length) byte = 0;
-                            factor[i][h] = cache_scale(byte);  // a NaN for 255, and so is what meets it
-                            above |= byte > largest && byte < 255;
-                        }
-                }
                 if (__any_sync(0xffffffffu, above)) {
-                    float fit = 1.f;
-                    if constexpr (kEight) {
-                        float top = 0.f;
+                    if constexpr (kEight)  // a scale that stands for NaN makes its P one
 #pragma unroll
                         for (int i = 0; i < MK; ++i)
 #pragma unroll
                             for (int h = 0; h < 2; ++h)
-                                if (factor[i][h] < INFINITY) top = fmaxf(top, factor[i][h]);
-                        top = warp_max(top);
-                        const int byte = max(largest, (int)(__float_as_uint(top) >> 23));
-                        if (byte > largest) {
-                            const int drop = byte - largest;
-                            fit = drop < 127 ? __uint_as_float((uint32_t)(127 - drop) << 23) : 0.f;
-                            largest = byte;
-                        }
-                    }
+                                if (factor[i][h] == INFINITY) factor[i][h] = NAN, beside[i][h] = -kFar;
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float top = fmaxf(x[0][j][e], x[0][j][e + 2]);
+                            float top = fmaxf(counted(x[0][j][e], 0, 0), counted(x[0][j][e + 2], 0, 1));
 #pragma unroll
-                            for (int i = 1; i < MK; ++i) top = fmaxf(top, fmaxf(x[i][j][e], x[i][j][e + 2]));
+                            for (int i = 1; i < MK; ++i) top = fmaxf(top, fmaxf(counted(x[i][j][e], i, 0), counted(x[i][j][e + 2], i, 1)));
 #pragma unroll
                             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                             float keep = 1.f;
@@ -621,7 +638,6 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                                 limit[j][e] = kLazy;
                             }
                             sum[j][e] *= keep;
-                            keep *= fit;
 #pragma unroll
                             for (int k = 0; k < kSteps; ++k) o[k][j][e] *= keep, o[k][j][e + 2] *= keep;
                         }
@@ -637,15 +653,12 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                         sum[j][1] += x[i][j][1] + x[i][j][3];
                     }
                 if constexpr (kEight) {
-                    // 2^7 for the largest: P stays below 2^15, and its hi + lo
-                    // in fp16 reaches 2^-32 of it
-                    const float near = __uint_as_float((uint32_t)min(254, 261 - largest) << 23);
 #pragma unroll
                     for (int i = 0; i < MK; ++i) {
-                        const float f0 = factor[i][0] * near, f1 = factor[i][1] * near;
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
-                            x[i][j][0] *= f0, x[i][j][1] *= f0, x[i][j][2] *= f1, x[i][j][3] *= f1;
+                            x[i][j][0] *= factor[i][0], x[i][j][1] *= factor[i][0];
+                            x[i][j][2] *= factor[i][1], x[i][j][3] *= factor[i][1];
                             if (masked)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
@@ -712,8 +725,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         }
 
         // ------------------------------------------- the warps' results meet
-        float unit = 1.f;
-        if constexpr (kEight) unit = __uint_as_float((uint32_t)max(254 - min(254, 261 - largest), 1) << 23);
+        if constexpr (kEight) least = __reduce_min_sync(0xffffffffu, least);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -722,6 +734,19 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) all += __shfl_xor_sync(0xffffffffu, all, w);
                 const int row = 8 * j + 2 * t4 + e;
+                float unit = 1.f;
+                if constexpr (kEight) {
+                    // References carry scales: a power of two a row brings the
+                    // sum to 1, so that those of the warps can meet.
+                    const int power = min(max((int)(__float_as_uint(all) >> 23), 1), 253);
+                    const bool far = all < kLeastSum ||
+                                     (least < 246u && all * __uint_as_float((least + 9u) << 23) < kLeastScaled);
+                    if (limit[j][e] > -INFINITY) {
+                        unit = __uint_as_float((uint32_t)(254 - power) << 23);
+                        from[j][e] += (float)(power - 127);
+                        all = far ? NAN : all * unit;
+                    }
+                }
                 if (g == 0) {
                     ml[(warp * kRows + row) * 2] = limit[j][e] == -INFINITY ? -INFINITY : from[j][e];
                     ml[(warp * kRows + row) * 2 + 1] = all;
