@@ -234,3 +234,25 @@ def test_value_scales_over_their_whole_range(storage, dtype, width, rows, column
     q = queries(int(starts[-1]), 4, width, dtype, 554)
     out, lse = cache.attend(batch, q, return_lse=True)
     check(cache, batch, starts, q, out, lse, width ** -0.5)
+
+
+@pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("scales,size", [((137, 147), 2.0 ** -16), ((95, 100), 2.0 ** 14), ((90, 150), 2.0 ** -16),
+                                         ((1, 20), 2.0 ** 15)])
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_key_scales_beyond_the_queries_type(storage, dtype, width, scales, size, rows, columns):
+    """Keys whose elements are above 65504 or below fp16's smallest step, under
+    queries that make ordinary scores of them."""
+    import torch
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, width, 561)
+    batch, starts = make_batch(lengths, new, 16, pages, 562, columns=columns)
+    g = torch.Generator("cuda").manual_seed(563)
+    cache.key_scales.copy_(torch.randint(scales[0], scales[1] + 1, cache.key_scales.shape, generator=g, device="cuda").to(torch.uint8))
+    q = queries(int(starts[-1]), 4, width, "float32", 564) * size
+    q = q.clamp(-65000, 65000).to(dt(dtype))
+    for causal in (True, False):
+        out, lse = cache.attend(batch, q, causal=causal, return_lse=True)
+        check(cache, batch, starts, q, out, lse, width ** -0.5, causal, spread=True)

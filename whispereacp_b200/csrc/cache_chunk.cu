@@ -62,7 +62,15 @@ constexpr int kTile = 128;               // rows of a tile
 constexpr int kHalfBytes = kTile * 128;  // 128 rows of 64 16-bit columns
 
 enum ChunkWait : int { kWaitBlock = 11, kWaitSlot = 12, kWaitScores = 13, kWaitP = 14, kWaitQueries = 15, kWaitO = 16,
-                       kWaitDone = 17, kWaitFirst = 18 };
+                       kWaitDone = 17, kWaitFirst = 18, kWaitPower = 19 };
+
+// Whether a block's keys, widened to the queries' type, share a power of two that
+// the scores are multiplied by: fp16 would not hold all scaled keys.  bf16 does,
+// each value exactly.
+template <typename T, int S>
+constexpr bool keys_share() {
+    return cache_eight(S) && std::is_same<T, __half>::value;
+}
 
 template <int S, int D>
 struct ChunkLayout {
@@ -85,9 +93,13 @@ struct ChunkLayout {
     static constexpr int held_bytes = kBlockKeys * (D + 1) + 16;  // and how many of the keys are seen
     static constexpr int held_at = ring_at + stages * tile_bytes;
     static constexpr int bar_at = held_at + depth * held_bytes;
-    // full, empty; per tile: scores, P's halves, first half, queries, O; done
-    static constexpr int bars = 2 * stages + 6 * tiles + 1;
-    static constexpr int bytes = bar_at + bars * 8 + kBarrierWords * 4;
+    // And the powers of two of as many blocks' keys as can have scores under way.
+    static constexpr int powers = cache_eight(S) ? stages / 2 + 1 : 0;
+    // full, empty; per tile: scores, P's halves, first half, queries, O; done;
+    // powers
+    static constexpr int bars = 2 * stages + 6 * tiles + 1 + powers;
+    static constexpr int powers_at = bar_at + bars * 8 + kBarrierWords * 4;
+    static constexpr int bytes = powers_at + powers * 4;
 };
 
 // ------------------------------------------------------------ the block list
@@ -354,7 +366,7 @@ __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence
 // ---------------------------------------------------------------- the roles
 
 struct ChunkBars {
-    uint64_t *full, *empty, *scores, *p, *first, *queries, *o, *done;
+    uint64_t *full, *empty, *scores, *p, *first, *queries, *o, *done, *powers;
 };
 
 template <int S, int D>
@@ -435,10 +447,58 @@ __device__ __forceinline__ void widen_piece(const uint4& raw, uint32_t scale, ui
     }
 }
 
+// What the scores of fp16 queries over a block of 8-bit keys are multiplied by,
+// log2(e) and the keys' power of two in it; a masked score of -infinity stays
+// one at a scale of 0.
+__device__ __forceinline__ float scores_factor(float scale, uint32_t power) {
+    return fmaxf(fabsf(scale) * kLog2e * __uint_as_float(power << 23), 0x1p-126f);
+}
+
+// The scale byte of a key relative to its block's power of two, which stands
+// kUp below the block's largest byte: fp16 holds the largest scaled value (448 x
+// 2^7, 128 x 2^8) then, and whole every value of a scale down to kDown below the
+// power.  Keys further down (2^22 or 2^32 below the largest; zeros aside) become
+// NaN, and the rows that see one are computed again alone.  Blocks whose bytes
+// are all 112 to 127, rows whose largest lies between 2^-6 and 2^6 among them,
+// need no power (it is 127, 2^0).
+template <int S> constexpr uint32_t kUp = S == kCacheE4m3 ? 7 : 8;
+template <int S> constexpr uint32_t kDown = S == kCacheE4m3 ? 15 : 24;
+template <int S>
+__device__ __forceinline__ uint32_t shared_scale(uint32_t byte, uint32_t power) {
+    if (byte == 255u) return byte;
+    if (byte + kDown<S> < power) return byte <= 8u ? 0u : 255u;
+    return byte + 127u - power;
+}
+
+// The power of a block of `keys` keys, by every warp of the kThreads that widen
+// it: kUp below the largest scale byte that stands for a number (25 at least).
+// `four` are the lane's four bytes at `bytes`, in whose place the first warp puts
+// them relative to the power.  Rare, and kept out of the loop's instructions.
+template <int S, int kThreads>
+__device__ __noinline__ uint32_t share_power(uint32_t* bytes, uint32_t four, int keys, int warp, int lane) {
+    uint32_t most = 25, relative = 0;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t byte = (four >> (8 * i)) & 255u;
+        if (lane * 4 + i < keys && byte != 255u) most = max(most, byte);
+    }
+    const uint32_t power = __reduce_max_sync(0xffffffffu, most) - kUp<S>;
+    for (int i = 0; i < 4; ++i) relative |= (shared_scale<S>((four >> (8 * i)) & 255u, power) & 255u) << (8 * i);
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    if (warp == 0) bytes[lane] = relative;
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    return power;
+}
+
 // 8-bit caches: the warps bring the blocks in as they are held, four tiles
 // (keys or values of a block) deep, and write them into the ring widened to the
-// queries' type, each value times its scale (a power of two: exact in bf16, and
-// in fp16 wherever fp16 holds the result).
+// queries' type, each value times its scale (a power of two: exact in bf16; fp16
+// rounds what it does not hold whole by as much as it rounds the results, and
+// makes an infinity of what is above 65504: rows that meet one are computed
+// again alone).  Keys for fp16 queries are taken relative to their block's power
+// of two, which goes to the softmax.  Block n's lies in place n % powers: its
+// keys' tile, number 2 n of the ring, is written when tile 2 n - stages is
+// released, and so the values of block n - powers, which every tile's softmax
+// has then passed.
 template <typename T, int S, int D>
 __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const ChunkBars& bar, volatile int* abort,
                             ChunkPlace p, long long begin, long long end, int warp, int lane) {
@@ -510,10 +570,21 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
         asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
         asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
         ask();
-        if (n >= Layout::stages) cache_wait(bar.empty + stage, parity, abort, a.status, kWaitSlot);
-        const unsigned char* held = smem + Layout::held_at + (n % kDepth) * Layout::held_bytes;
+        unsigned char* held = smem + Layout::held_at + (n % kDepth) * Layout::held_bytes;
         const int keys = *reinterpret_cast<const int*>(held + kPieces * 16 + kBlockKeys);  // seen; the others are zeros
+        const uint32_t four = reinterpret_cast<const uint32_t*>(held + kPieces * 16)[lane];  // of the scale bytes
+        if (n >= Layout::stages) cache_wait(bar.empty + stage, parity, abort, a.status, kWaitSlot);
         unsigned char* tile = smem + Layout::ring_at + stage * Layout::tile_bytes;
+        if (keys_share<T, S>() && (n & 1) == 0) {
+            uint32_t power = 127;
+            if (__any_sync(0xffffffffu, lane * 4 < keys && (four & 0xf0f0f0f0u) != 0x70707070u))
+                power = share_power<S, kThreads>(reinterpret_cast<uint32_t*>(held + kPieces * 16), four, keys, warp, lane);
+            if (me == 0) {
+                const int at = (n >> 1) % Layout::powers;
+                reinterpret_cast<float*>(smem + Layout::powers_at)[at] = scores_factor(a.scale, power);
+                cache_arrive(bar.powers + at);
+            }
+        }
 #pragma unroll 1
         for (int piece = me; piece < kPieces; piece += kThreads) {
             const int key = piece / (D / 16), c = piece % (D / 16);
@@ -662,8 +733,9 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
     const uint32_t lanes = (uint32_t)(row & ~31) << 16;
     const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + Layout::out_column + t * D + lanes;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // the sign goes into the queries
-    const float to_log2 = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-126f);  // a masked score of -infinity stays one at scale 0
+    float to_log2 = scores_factor(a.scale, 127u);
     uint32_t s_parity = 0, o_parity = 0, h_parity = 0;
+    int passed = 0;  // blocks of the run before the item
     // The row's queries, swizzled as the copy engine does it.
     const auto give_queries = [&](const ChunkPlace& p, const TileRow& r) {
         const unsigned char* qp = a.queries + ((long long)p.q.first + r.token) * a.q_row + r.head * a.q_head;
@@ -702,6 +774,11 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             // Keys below `clear` are seen by every row of the tile.
             const int clear = tile_row(a, p.q, p.head, packed).seen;
             for (int j = p.block; j < blocks; ++j) {
+                if constexpr (keys_share<T, S>()) {
+                    const int n = passed + j - p.block, at = n % Layout::powers;
+                    cache_wait(bar.powers + at, (uint32_t)(n / Layout::powers) & 1u, abort, a.status, kWaitPower);
+                    to_log2 = reinterpret_cast<const volatile float*>(smem + Layout::powers_at)[at];
+                }
                 cache_wait(bar.scores + t, s_parity, abort, a.status, kWaitScores);
                 s_parity ^= 1;
                 tmem_fence_after();
@@ -889,6 +966,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
         }
         tmem_fence_before();  // this tile's reads, before the products that the next arrival lets run
         if (last_n == 0) break;
+        passed += last - p.block;
         p = pn;
         last = last_n;
         blocks = blocks_n;
@@ -905,7 +983,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
     uint64_t* tile_bars = bars + 2 * Layout::stages;
     constexpr int kTiles = Layout::tiles;
     const ChunkBars bar = {bars, bars + Layout::stages, tile_bars, tile_bars + kTiles, tile_bars + 3 * kTiles,
-                           tile_bars + 4 * kTiles, tile_bars + 5 * kTiles, tile_bars + 6 * kTiles};
+                           tile_bars + 4 * kTiles, tile_bars + 5 * kTiles, tile_bars + 6 * kTiles, tile_bars + 6 * kTiles + 1};
     volatile int* abort = reinterpret_cast<volatile int*>(bars + Layout::bars);
     uint32_t* slot = reinterpret_cast<uint32_t*>(bars + Layout::bars) + kOwnWord;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -923,6 +1001,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
             cache_barrier_init(bar.o + t, 1);
         }
         cache_barrier_init(bar.done, 1);
+        for (int i = 0; i < Layout::powers; ++i) cache_barrier_init(bar.powers + i, 1);
         *abort = abort[kBeatWord] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
