@@ -256,3 +256,18 @@ def test_key_scales_beyond_the_queries_type(storage, dtype, width, scales, size,
     for causal in (True, False):
         out, lse = cache.attend(batch, q, causal=causal, return_lse=True)
         check(cache, batch, starts, q, out, lse, width ** -0.5, causal, spread=True)
+
+
+@pytest.mark.parametrize("storage", ["int8", "float8_e4m3fn"])
+@pytest.mark.parametrize("low", [100, 110, 118])
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_tiny_queries_over_large_keys(storage, low, rows, columns):
+    """bf16 queries of 2^-low over keys of 2^low: ordinary scores."""
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, 64, 571)
+    batch, starts = make_batch(lengths, new, 16, pages, 572, columns=columns)
+    cache.key_scales.fill_(120 + low)
+    q = (queries(int(starts[-1]), 4, 64, "float32", 573) * 2.0 ** -low).to(dt("bfloat16"))
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, 0.125)

@@ -284,8 +284,10 @@ __device__ __forceinline__ float narrow_queries(uint32_t (&qf)[D / 16][2]) {
         }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = (int)(__float_as_uint(top) >> 23);  // biased; 255: not finite
-    const bool fine = e < 255 && e > 20;
+    // Biased; 255: not finite; 9 is the least whose power of two is fp32's, and
+    // brings a row below 2^-118 as near.
+    const int e = max((int)(__float_as_uint(top) >> 23), 9);
+    const bool fine = e < 255;
     const float down = fine ? __uint_as_float((uint32_t)(262 - e) << 23) : 1.f;  // 2^(135 - e)
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                     cache_proxy_fence();
                     __syncwarp();
                 }
-                float s[MK][NT][4];
+                float s[MK][NT][4], size[kEight ? MK : 1][2];  // 8-bit keys' scales
 #pragma unroll
                 for (int i = 0; i < MK; ++i) {
 #pragma unroll
@@ -559,10 +561,8 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                                 for (int j = 0; j < NT; ++j) mma_16816<MT>(s[i][j], f, qf[j][k + h]);
                             }
                         }
-                        const float k0 = cache_scale(scales[warp * kWarpKeys + i * 16 + g]);
-                        const float k1 = cache_scale(scales[warp * kWarpKeys + i * 16 + g + 8]);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) s[i][j][0] *= k0, s[i][j][1] *= k0, s[i][j][2] *= k1, s[i][j][3] *= k1;
+                        size[i][0] = cache_scale(scales[warp * kWarpKeys + i * 16 + g]);
+                        size[i][1] = cache_scale(scales[warp * kWarpKeys + i * 16 + g + 8]);
                     }
                 }
                 // x = log2 of the probability, relative; s stays.
@@ -586,6 +586,11 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                     if constexpr (kEight) return v + beside[i][h];
                     else return v;
                 };
+                // The scales first: large keys may meet small queries.
+                const auto score_factor = [&](int i, int j, int e) {
+                    if constexpr (kEight) return size[i][e >> 1] * to_log2[j][e & 1];
+                    else return to_log2[j][e & 1];
+                };
                 const auto relative = [&] {
 #pragma unroll
                     for (int i = 0; i < MK; ++i)
@@ -593,7 +598,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                         for (int j = 0; j < NT; ++j)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                x[i][j][e] = fmaf(s[i][j][e], to_log2[j][e & 1], -from[j][e & 1]);
+                                x[i][j][e] = fmaf(s[i][j][e], score_factor(i, j, e), -from[j][e & 1]);
                     if (masked)
 #pragma unroll
                         for (int i = 0; i < MK; ++i)
