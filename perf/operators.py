@@ -284,7 +284,8 @@ def run(state):
             return {"keys": state["keys"], "values": state["values"]}
         if kind == "store":
             cache.append(batch, state["k"], state["v"])
-        keys, values = cache.read(batch, dtype=DTYPES[case["dtype"]])
+        # How many rows there are the program knows; asking the batch for them waits for the device.
+        keys, values = cache.read(batch, dtype=DTYPES[case["dtype"]], rows=state["rows"])
     else:
         if kind == "attend":
             out, lse = _plain_attend(state)
