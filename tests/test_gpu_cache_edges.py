@@ -271,3 +271,36 @@ def test_tiny_queries_over_large_keys(storage, low, rows, columns):
     q = (queries(int(starts[-1]), 4, 64, "float32", 573) * 2.0 ** -low).to(dt("bfloat16"))
     out, lse = cache.attend(batch, q, return_lse=True)
     check(cache, batch, starts, q, out, lse, 0.125)
+
+
+def test_a_batch_whose_starts_change_is_read_as_it_stands():
+    """read without a number of rows after starts were updated in place, to
+    more and to fewer."""
+    import torch
+    cache = make_cache("float16", 30, 2, 16, 64, 581)
+    batch, _ = make_batch([40, 60], [5, 7], 16, 30, 582)
+    held = [held_rows(cache, batch.page_table[s], n)[0] for s, n in enumerate((40, 60))]
+    for new in ((5, 7), (30, 41), (2, 1), (0, 0), (0, 6)):
+        batch.starts.copy_(torch.tensor([0, new[0], sum(new)], dtype=torch.int32))
+        k, v = cache.read(batch)
+        assert k.shape == v.shape == (sum(new), 2, 64) and batch.rows() == sum(new)
+        want = torch.cat([held[s][len(held[s]) - n:] for s, n in enumerate(new)])
+        assert torch.equal(k.double(), want)
+
+
+@pytest.mark.parametrize("storage,dtype", [("float16", "float16"), ("int8", "bfloat16")])
+@pytest.mark.parametrize("columns", [None, 600])
+def test_starts_that_grow_past_the_bound_of_their_batch(storage, dtype, columns):
+    """max_rows chooses kernels: results are the definition's all the same."""
+    import torch
+    from whispereacp_b200 import CacheBatch
+    lengths, new = CHUNKS
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, 64, 585)
+    made, starts = make_batch(lengths, new, 16, pages, 586, columns=columns)
+    batch = CacheBatch(made.page_table, made.lengths, torch.zeros_like(made.starts))
+    assert batch.max_rows == 0
+    batch.starts.copy_(made.starts)
+    q = queries(int(starts[-1]), 4, 64, dtype, 587)
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, 0.125)

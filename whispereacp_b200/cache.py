@@ -81,13 +81,11 @@ class CacheBatch:
                               sequences, max_rows)
         self._ref = ctypes.byref(self._c)
         self.columns = page_table.shape[1]
-        self._rows = None
 
     def rows(self) -> int:
-        """The rows of the calls' arrays, starts[-1]: asked of the device once."""
-        if self._rows is None:
-            self._rows = int(self.starts[-1])
-        return self._rows
+        """The rows of the calls' arrays, starts[-1] as it stands: waits for the
+        device."""
+        return int(self.starts[-1])
 
 
 class PagedCache:
@@ -181,7 +179,8 @@ class PagedCache:
         the values they stand for.  Without `keys` and `values` to fill, new
         tensors of `dtype` (None: the cache's; float32 for 8-bit storage);
         `rows`, then, is how many there are (None: taken from the batch's
-        starts, once, which waits for the device)."""
+        starts as they stand, which waits for the device, and so cannot be
+        captured)."""
         if (keys is None) != (values is None):
             raise ValueError("keys and values to fill are given together")
         handle = self._usable(batch)
