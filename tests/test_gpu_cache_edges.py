@@ -304,3 +304,23 @@ def test_starts_that_grow_past_the_bound_of_their_batch(storage, dtype, columns)
     q = queries(int(starts[-1]), 4, 64, dtype, 587)
     out, lse = cache.attend(batch, q, return_lse=True)
     check(cache, batch, starts, q, out, lse, 0.125)
+
+
+def test_tensors_that_require_gradients_are_refused():
+    """The operators have no gradient; results that silently lack one would
+    train nothing.  Without grad mode they are taken as they are."""
+    import torch
+    cache = make_cache("float16", 8, 2, 16, 64, 591)
+    batch, _ = make_batch([20], [2], 16, 8, 592)
+    plain = queries(2, 2, 64, "float16", 593)
+    leaf = plain.clone().requires_grad_()
+    for call in (lambda x: cache.attend(batch, x), lambda x: cache.append(batch, x, plain),
+                 lambda x: cache.append(batch, plain, x), lambda x: cache.attend(batch, plain, out=x),
+                 lambda x: cache.read(batch, x, plain.clone()), lambda x: cache.read(batch, plain.clone(), x),
+                 lambda x: cache.attend(batch, plain, lse=torch.zeros(2, 2, device="cuda", requires_grad=True))):
+        with pytest.raises(ValueError, match="gradient"):
+            call(leaf)
+    with torch.no_grad():
+        assert torch.equal(cache.attend(batch, leaf), cache.attend(batch, plain))
+        cache.append(batch, leaf, leaf)
+    assert torch.equal(cache.attend(batch, leaf.detach()), cache.attend(batch, plain))

@@ -10,7 +10,8 @@ the tensors of a batch contain is read when the work runs, so one batch serves
 every step whose tensors are updated in place, in a captured CUDA graph too.
 
 Calls queue on torch's current stream of the cache's device, or on ``stream``,
-and return without waiting.
+and return without waiting.  They have no gradients: in grad mode tensors that
+require one are refused.
 """
 from __future__ import annotations
 
@@ -45,6 +46,13 @@ def _row_type(dtype) -> int:
         raise ValueError(f"rows are float32, float16 or bfloat16, not {_name(dtype)}")
     _codes[dtype] = code
     return code
+
+
+def _refuse_gradient(name: str) -> None:
+    """In grad mode a tensor that requires a gradient would silently get none."""
+    if _torch().is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and the cache's operators have none: detach it, or call them "
+                         "under torch.no_grad()")
 
 
 class CacheBatch:
@@ -240,6 +248,8 @@ class PagedCache:
             elif lse.shape != (rows, heads) or lse.dtype != torch.float32 or not lse.is_contiguous() or \
                     lse.get_device() != self._index:
                 raise ValueError(f"lse must be a contiguous float32 tensor [{rows}, {heads}] on the cache's device")
+            elif lse.requires_grad:
+                _refuse_gradient("lse")
             workspace = self._workspace(needed, stream) if needed else None
         check(self._lib.wsp_cache_attend(handle, batch._ref, rows, heads, ctypes.byref(q), ctypes.byref(o),
                                          lse.data_ptr() if lse is not None else None,
@@ -263,6 +273,8 @@ class PagedCache:
     def _rows(self, t, name: str, rows: int, heads: int) -> CCacheRows:
         if t.get_device() != self._index:
             raise ValueError(f"{name} must be on {self.device}, not {t.device}")
+        if t.requires_grad:
+            _refuse_gradient(name)
         if t.shape != (rows, heads, self.head_width):
             raise ModelError(f"{name} must be [{rows}, {heads}, {self.head_width}], not {list(t.shape)}")
         row_stride, head_stride, step = t.stride()
