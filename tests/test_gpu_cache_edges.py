@@ -324,3 +324,32 @@ def test_tensors_that_require_gradients_are_refused():
         assert torch.equal(cache.attend(batch, leaf), cache.attend(batch, plain))
         cache.append(batch, leaf, leaf)
     assert torch.equal(cache.attend(batch, leaf.detach()), cache.attend(batch, plain))
+
+
+def test_caches_of_a_thread_and_stream_share_a_workspace():
+    """A decoder's layers follow one another on one stream: their caches need
+    one workspace, not one each; a thread's ends with it."""
+    import threading
+    import torch
+    caches = [make_cache("float16", 80, 2, 16, 64, 601 + i) for i in range(6)]
+    batch, starts = make_batch([600, 500], [200, 1], 16, 80, 602, columns=9600)
+    q = queries(201, 2, 64, "float16", 603)
+    out, lse = torch.empty_like(q), torch.empty(201, 2, device="cuda")
+
+    def step():
+        for cache in caches:
+            cache.attend(batch, q, out=out, lse=lse)
+
+    caches[0].attend(batch, q, out=out, lse=lse)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    step()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+    check(caches[-1], batch, starts, q, out, lse, 0.125)
+    for _ in range(3):
+        thread = threading.Thread(target=step)
+        thread.start()
+        thread.join()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before

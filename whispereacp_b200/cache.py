@@ -29,6 +29,7 @@ CACHE_STORAGE = {"float16": WSP_CACHE_FLOAT16, "bfloat16": WSP_CACHE_BFLOAT16, "
                  "int8": WSP_CACHE_INT8}
 _ROW_TYPES = {"float32": WSP_FLOAT32, "float16": WSP_FLOAT16, "bfloat16": WSP_BFLOAT16}
 _codes: dict = {}  # torch dtype -> its code, filled as dtypes are met
+_workspaces = threading.local()  # (device, stream) -> this thread's workspace there
 
 
 def _torch():
@@ -145,7 +146,6 @@ class PagedCache:
         self._index = keys.device.index
         self._scale = 1.0 / math.sqrt(width)
         self._workspace_bytes: dict = {}
-        self._workspaces: dict = {}
         self._raw_stream = getattr(_torch()._C, "_cuda_getCurrentRawStream", None) or \
             (lambda index: _torch().cuda.current_stream(index).cuda_stream)
 
@@ -294,16 +294,17 @@ class PagedCache:
 
     def _workspace(self, needed: int, stream):
         """A call's workspace.  Calls of one host thread on one of torch's
-        streams follow one another, so they share it; a captured call, whose
-        graph may run next to others, and a call on a given stream get their
-        own, which torch's allocator keeps for that stream's later work."""
+        streams follow one another, whichever cache they are of, so they share
+        it, and it ends with the thread; a captured call, whose graph may run
+        next to others, and a call on a given stream get their own, which
+        torch's allocator keeps for that stream's later work."""
         torch = _torch()
         if stream is not None or torch.cuda.is_current_stream_capturing():
             return torch.empty(needed, dtype=torch.uint8, device=self.device)
-        key = (threading.get_ident(), self._raw_stream(self._index))
-        held = self._workspaces.get(key)
+        key = (self._index, self._raw_stream(self._index))
+        held = _workspaces.__dict__.get(key)
         if held is None or held.numel() < needed:
-            held = self._workspaces[key] = torch.empty(needed, dtype=torch.uint8, device=self.device)
+            held = _workspaces.__dict__[key] = torch.empty(needed, dtype=torch.uint8, device=self.device)
         return held
 
     def _allocating(self, stream):
