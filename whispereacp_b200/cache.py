@@ -299,13 +299,22 @@ class PagedCache:
         next to others, and a call on a given stream get their own, which
         torch's allocator keeps for that stream's later work."""
         torch = _torch()
-        if stream is not None or torch.cuda.is_current_stream_capturing():
+        if stream is not None or self._capturing():
             return torch.empty(needed, dtype=torch.uint8, device=self.device)
         key = (self._index, self._raw_stream(self._index))
         held = _workspaces.__dict__.get(key)
         if held is None or held.numel() < needed:
             held = _workspaces.__dict__[key] = torch.empty(needed, dtype=torch.uint8, device=self.device)
         return held
+
+    def _capturing(self) -> bool:
+        """Whether the current stream of the cache's device, which need not be
+        the current device, is being captured."""
+        torch = _torch()
+        if torch.cuda.current_device() == self._index:
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self._index):
+            return torch.cuda.is_current_stream_capturing()
 
     def _allocating(self, stream):
         """The context in which a call's tensors are allocated: its own stream,
