@@ -156,7 +156,9 @@ int wsp_cache_attend_workspace(const wsp_cache* cache, const wsp_cache_batch* ba
 
 /*
  * Waits for the device's queued work and reports a wait inside a kernel that
- * gave up (WSP_CUDA_ERROR; none should).
+ * gave up after 2 s (WSP_CUDA_ERROR; none should).  The attention's calls do
+ * not say so themselves: rows that such a wait held up are computed again
+ * without waits, slowly.
  */
 int wsp_cache_check(wsp_cache* cache);
 

@@ -57,3 +57,18 @@ def test_a_call_beside_a_capture_on_another_device_shares_its_thread_s(monkeypat
     first, second = cache._workspace(4096, None), cache._workspace(2048, None)
     assert first.data_ptr() == second.data_ptr()
     assert cache_on(index)._workspace(4096, None).data_ptr() == first.data_ptr()
+
+
+@pytest.mark.gpu
+def test_waits_that_give_up(tmp_path):
+    import os
+    import shutil
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    program, library = os.path.join(str(tmp_path), "cache_wait_test"), os.path.join(root, "whispereacp_b200")
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O1", "-ccbin", "g++",
+                    "--expt-relaxed-constexpr", "-o", program, os.path.join(root, "tests", "cpp", "cache_wait_test.cu"),
+                    "-L", library, "-lwsp_b200", "-Xlinker", f"-rpath={library}"], check=True)
+    run = subprocess.run([program], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr

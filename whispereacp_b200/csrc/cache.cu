@@ -9,6 +9,8 @@
 #include <algorithm>
 #include <atomic>
 #include <memory>
+#include <tuple>
+#include <utility>
 
 namespace wsp {
 namespace {
@@ -346,7 +348,8 @@ struct wsp_cache {
     int device = 0;
     int sms = 0;
     wsp::DeviceBuffer owned[4];
-    int* status = nullptr;  // which wait of a kernel gave up
+    int* status = nullptr;  // which wait of a kernel gave up: the kind of the last, and the mark of its cache
+    int mark = 0;
 };
 
 namespace wsp {
@@ -400,16 +403,18 @@ CacheBatchView batch_view(const wsp_cache_batch& b) {
 }
 
 // The caches' status words: static device memory, one after another, so that
-// making a cache allocates and waits for nothing.  A word is 0 unless a wait
-// gave up and nobody has asked since; caches 1024 apart share one.
+// making a cache allocates and waits for nothing.  Caches 1024 apart share one,
+// which then holds the last wait that gave up: their marks tell whose it was
+// (2^22 of them, so that none is used again while a cache of it lives).
 constexpr int kStatusWords = 1024;
 __device__ int status_words[kStatusWords];
 
-int* status_word() {
+std::pair<int*, int> next_status() {
     static std::atomic<unsigned> made{0};
     void* words = nullptr;
     CUDA_CHECK(cudaGetSymbolAddress(&words, status_words));
-    return static_cast<int*>(words) + made++ % kStatusWords;
+    const unsigned n = made++;
+    return {static_cast<int*>(words) + n % kStatusWords, (int)((n % (1u << 22) + 1) << 8)};
 }
 
 using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
@@ -551,7 +556,7 @@ int wsp_cache_create(const wsp_cache_shape* shape, int device, const wsp_cache_m
         c->maps.keys = wsp::pool_map(s, m, m.keys);
         c->maps.values = wsp::pool_map(s, m, m.values);
         wsp::prepare_cache_attend(s.storage, s.head_width);
-        c->status = wsp::status_word();
+        std::tie(c->status, c->mark) = wsp::next_status();
         *out = c.release();
     });
 }
@@ -628,6 +633,7 @@ int wsp_cache_attend(wsp_cache* cache, const wsp_cache_batch* batch, int rows, i
         a.scale = scale;
         a.causal = causal != 0;
         a.status = c.status;
+        a.mark = c.mark;
         a.workspace = static_cast<unsigned char*>(workspace);
         wsp::CurrentDevice device(c.device);
         wsp::launch_cache_attend(a, c.maps, wsp::attend_shape(c, queries->dtype, *batch),
@@ -642,9 +648,9 @@ int wsp_cache_check(wsp_cache* cache) {
         wsp::cuda_check(cudaDeviceSynchronize(), "wsp_cache_check");
         int status = 0;
         wsp::cuda_check(cudaMemcpy(&status, c.status, sizeof status, cudaMemcpyDeviceToHost), "wsp_cache_check");
-        if (!status) return;
+        if ((status & ~255) != c.mark) return;
         wsp::cuda_check(cudaMemset(c.status, 0, sizeof status), "wsp_cache_check");
-        throw wsp::CudaFailure("a wait of the cache's attention gave up (" + std::to_string(status) + ")", false);
+        throw wsp::CudaFailure("a wait of the cache's attention gave up (" + std::to_string(status & 255) + ")", false);
     });
 }
 

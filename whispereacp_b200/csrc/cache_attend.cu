@@ -418,6 +418,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
             cache_barrier_init(empty + i, kWorkers);
         }
         *abort = abort[kBeatWord] = 0;
+        abort[kMarkWord] = a.mark;
         *redo = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -775,7 +776,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
         float* part = partials + ((long long)blockIdx.x * 2 + (p.unit > 0 ? 0 : 1)) * partial_floats<D>(kRows);
         for (int row = threadIdx.x / kRowThreads; row < valid; row += 128 / kRowThreads) {
             const int d = (threadIdx.x % kRowThreads) * 2;
-            float top = -INFINITY, all = 0.f;
+            float top = -INFINITY, all = *abort ? NAN : 0.f;
             float2 v = make_float2(0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWorkers; ++w) top = fmaxf(top, ml[(w * kRows + row) * 2]);

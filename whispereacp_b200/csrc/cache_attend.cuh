@@ -23,8 +23,9 @@ struct CacheAttendArgs {
     int causal;
     int uncut;                     // the few-row kernel's CTAs take whole items
     int behind;                    // the few-row kernel runs behind the chunks', which waited for what is before
+    int mark;                      // the cache's, a multiple of 256: caches may share the status word
     long long few;                 // rows * group up to which a sequence is the few-row kernel's
-    int* status;                   // which wait gave up, 0: none
+    int* status;                   // where a wait that gives up is recorded: its kind, and the mark
     unsigned char* workspace;
 };
 

@@ -708,7 +708,7 @@ __device__ void chunk_products(const CacheAttendArgs& a, unsigned char* smem, co
         const unsigned long long start = cache_clock_ns();
         while (!cache_phase_done(bar.done, 0))
             if (cache_clock_ns() - start > kCacheTimeoutNs) {
-                atomicCAS(a.status, 0, kWaitDone);
+                atomicExch(a.status, a.mark | kWaitDone);
                 break;
             }
     }
@@ -914,6 +914,7 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             tmem_fence_after();
         }
         const bool whole = p.block == 0 && last == p.blocks;
+        if (*abort) sum = NAN;
         const bool some = r.seen > 0;  // a row without a key is zeros whatever the tile's other rows met
         const float inverse = 1.f / sum;
         const float log_sum = unset ? -INFINITY : from;
@@ -1003,6 +1004,7 @@ __global__ void __launch_bounds__(ChunkLayout<S, D>::threads, ChunkLayout<S, D>:
         cache_barrier_init(bar.done, 1);
         for (int i = 0; i < Layout::powers; ++i) cache_barrier_init(bar.powers + i, 1);
         *abort = abort[kBeatWord] = 0;
+        abort[kMarkWord] = a.mark;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == Layout::mma_warp) {

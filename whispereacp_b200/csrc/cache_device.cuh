@@ -34,14 +34,16 @@ __device__ __forceinline__ bool cache_phase_done(uint64_t* bar, uint32_t parity)
     return done != 0;
 }
 
-// The words behind a CTA's barriers: whether a wait has given up, a word of
-// the kernel's own, and one that changes while a warp does a row alone.
-constexpr int kAbortWord = 0, kOwnWord = 1, kBeatWord = 2, kBarrierWords = 4;
+// The words behind a CTA's barriers: first whether a wait has given up (`abort`),
+// then a word of the kernel's own, one that changes while a warp does a row
+// alone, and the cache's mark.
+constexpr int kOwnWord = 1, kBeatWord = 2, kMarkWord = 3, kBarrierWords = 4;
 
 // Waits for the phase of `parity`.  After 2 s, or once another wait of the CTA
 // has given up, it records `kind` and returns false, and so does every later
 // wait at once: the roles then run through their loops without waiting, so
-// all meet at the barriers between them, and the results are void.  A warp of
+// all meet at the barriers between them, and the sums become NaN, so that the
+// rows are computed again alone, which takes no waits.  A warp of
 // the CTA that does rows alone may take longer over a long context; the 2 s
 // count from its last sign (its loops end by themselves).
 static __device__ __noinline__ bool cache_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
@@ -59,7 +61,7 @@ static __device__ __noinline__ bool cache_wait_slow(uint64_t* bar, uint32_t pari
                 start = cache_clock_ns();
                 continue;
             }
-            atomicCAS(status, 0, kind);
+            atomicExch(status, abort[kMarkWord] | kind);
             *abort = 1;
             return false;
         }
