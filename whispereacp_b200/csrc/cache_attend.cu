@@ -265,9 +265,11 @@ __device__ __forceinline__ float log2_fast(float x) {
 constexpr float kFar = 80.f;
 // A row is computed again alone where that leaves its sum below kLeastSum, so
 // that smaller P underflow, or where the row's sum times the least scale among
-// its keys is below kLeastScaled: columns in which the values of large scales are
-// zeros are the small ones' alone.  The second takes scales 2^13 apart.
+// its keys is below kLeastScaled, scales 2^13 apart at least, and a column shows
+// it: where the values of large scales are zeros the small ones' are the
+// result, and P's 2^-25 a key may be more than 2^-11 of that.
 constexpr float kLeastSum = 0x1p-95f, kLeastScaled = 0x1p-6f;
+template <int S> constexpr float kLeastColumn = (S == kCacheE4m3 ? 448.f : 128.f) * 0x1p-14f;
 
 // bf16 queries of an 8-bit cache as fp16, which holds a bf16 exactly between
 // 2^-14 and 2^15: a power of two brings the row's largest to 2^8.., and its
@@ -745,8 +747,16 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                     // References carry scales: a power of two a row brings the
                     // sum to 1, so that those of the warps can meet.
                     const int power = min(max((int)(__float_as_uint(all) >> 23), 1), 253);
-                    const bool far = all < kLeastSum ||
-                                     (least < 246u && all * __uint_as_float((least + 9u) << 23) < kLeastScaled);
+                    bool far = least < 246u && all * __uint_as_float((least + 9u) << 23) < kLeastScaled;
+                    if (__any_sync(0xffffffffu, far)) {
+                        float low = INFINITY;
+#pragma unroll
+                        for (int k = 0; k < kSteps; ++k) low = fminf(low, fminf(fabsf(o[k][j][e]), fabsf(o[k][j][e + 2])));
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, w));
+                        far = far && low < (float)((last - p.unit) * kWarpKeys) * kLeastColumn<S>;
+                    }
+                    far = far || all < kLeastSum;
                     if (limit[j][e] > -INFINITY) {
                         unit = __uint_as_float((uint32_t)(254 - power) << 23);
                         from[j][e] += (float)(power - 127);
