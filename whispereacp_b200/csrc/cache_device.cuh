@@ -136,18 +136,25 @@ __device__ __forceinline__ void widen4(uint32_t bytes, bool interleaved, uint32_
 
 // ------------------------------------------------- a row that is done alone
 
-// One row of one query head by one warp, key by key: o = sum_j p_j v_j / sum_j
-// p_j with p_j = exp(s_j - max), the maximum and both sums running.  Only keys
-// the row sees are read.  The tiled kernels multiply whole tiles by P of 16
-// bits, or of two: an infinity or NaN among the values of a key behind the row
-// (0 times it) makes the row NaN there, and so may a seen infinity (P's lower
-// half is 0 or negative).  Rows whose results are not finite come here, and
-// have here what the definition says.  16 keys share a page, and 4 of them are
-// on their way at once.  `beat` (null: nobody waits) changes every 16 keys.
+// One row of one query head by one warp: o = sum_j p_j v_j / sum_j p_j with p_j =
+// exp(s_j - max), the maximum and both sums running, all in fp32.  Only keys the
+// row sees are read.  The tiled kernels multiply whole tiles by P of 16 bits, or
+// of two: an infinity or NaN among the values of a key behind the row (0 times
+// it) makes the row NaN there, and so may a seen infinity (P's lower half is 0 or
+// negative).  Rows whose results are not finite come here, with those whose
+// scales the 16 bits do not reach, and have here what the definition says.
+//
+// 32 keys at a time: a lane scores a key, its 16-byte pieces one after another
+// against queries handed round; then the lanes share out the columns and go over
+// the keys, 8 values on their way.  Latency bounds it; how long a call takes in
+// which many rows come here is told beside the kernels.  `beat` (null: nobody
+// waits) changes every 32 keys.
 template <typename T, int S, int D>
 __device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int first, int before, int length, int i,
                                         int head, volatile int* beat) {
-    constexpr int kPer = D / 32;  // a lane's elements
+    constexpr int kPer = D / 32;  // a lane's columns
+    constexpr int kPiece = 16 / cache_bytes(S);  // values of 16 bytes
+    constexpr int kAtOnce = 8;
     using Pair = typename std::conditional<cache_eight(S), uint16_t, uint32_t>::type;
     const int lane = threadIdx.x & 31;
     const int keys = a.causal ? min(before + i + 1, length) : length;
@@ -163,57 +170,71 @@ __device__ __noinline__ void attend_row(const CacheAttendArgs& a, int s, int fir
         o[e] = o[e + 1] = 0.f;
     }
     float top = -INFINITY, total = 0.f;
-    for (int j16 = 0; j16 < keys; j16 += 16) {
-        const int page = cache_page(a.cache, a.batch, s, j16);
+    for (int j0 = 0; j0 < keys; j0 += 32) {
         if (beat && lane == 0) *beat = *beat + 1;
-        for (int j = j16; j < min(j16 + 16, keys); j += 4) {
-            Pair k[4][kPer / 2], v[4][kPer / 2];
-            uint8_t ks[4], vs[4];
+        const int j = j0 + lane, count = min(32, keys - j0);
+        const int page = lane < count ? cache_page(a.cache, a.batch, s, j) : -1;
+        long long at = -1;  // the key's row in the pools, -1: zeros
+        float by = 1.f, score = 0.f;  // its value's scale
+        if (page >= 0) {
+            const int slot = j & ((1 << a.cache.page_shift) - 1);
+            at = cache_offset(a.cache, page, kv, slot);
+            if constexpr (cache_eight(S)) {
+                const long long si = cache_scale_index(a.cache, page, kv, slot);
+                score = cache_scale(a.cache.key_scales[si]);
+                by = cache_scale(a.cache.value_scales[si]);
+            } else {
+                score = 1.f;
+            }
+        }
+        float dot = 0.f;
+#pragma unroll 2
+        for (int c = 0; c < D / kPiece; ++c) {
+            uint4 piece = make_uint4(0, 0, 0, 0);
+            if (at >= 0) piece = *reinterpret_cast<const uint4*>(a.cache.keys + at + c * 16);
+            const uint32_t words[4] = {piece.x, piece.y, piece.z, piece.w};
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                ks[n] = vs[n] = 0;
+            for (int e = 0; e < kPiece; e += 2) {
+                const uint32_t bits = cache_eight(S) ? (words[e / 4] >> (8 * (e & 2))) & 0xffffu : words[e / 2];
+                const float2 f = cache_pair<S>(bits);
+                const int from = (c * kPiece + e) / kPer;
+                dot += __shfl_sync(0xffffffffu, qv[e % kPer], from) * f.x;
+                dot += __shfl_sync(0xffffffffu, qv[e % kPer + 1], from) * f.y;
+            }
+        }
+        score = lane < count ? dot * score * a.scale : -INFINITY;
+        const float higher = fmaxf(top, warp_max(score));
+        const float from = higher == -INFINITY ? 0.f : higher;
+        const float keep = expf(top - from), p = expf(score - from);
+        total = total * keep + warp_sum(p);
+        if (!(total == total)) break;  // and so it stays, and every sum of it
+        top = higher;
 #pragma unroll
-                for (int e = 0; e < kPer / 2; ++e) k[n][e] = v[n][e] = 0;
-                if (page < 0 || j + n >= keys) continue;
-                const int slot = (j + n) & ((1 << a.cache.page_shift) - 1);
-                const long long at = cache_offset(a.cache, page, kv, slot) + lane * kPer * cache_bytes(S);
+        for (int e = 0; e < kPer; ++e) o[e] *= keep;
+        for (int n0 = 0; n0 < count; n0 += kAtOnce) {
+            Pair v[kAtOnce][kPer / 2];
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n) {
+                const long long of = __shfl_sync(0xffffffffu, at, n0 + n);
 #pragma unroll
                 for (int e = 0; e < kPer / 2; ++e) {
-                    k[n][e] = *reinterpret_cast<const Pair*>(a.cache.keys + at + 2 * e * cache_bytes(S));
-                    v[n][e] = *reinterpret_cast<const Pair*>(a.cache.values + at + 2 * e * cache_bytes(S));
-                }
-                if constexpr (cache_eight(S)) {
-                    const long long si = cache_scale_index(a.cache, page, kv, slot);
-                    ks[n] = a.cache.key_scales[si];
-                    vs[n] = a.cache.value_scales[si];
+                    v[n][e] = 0;
+                    if (of >= 0)
+                        v[n][e] = *reinterpret_cast<const Pair*>(a.cache.values + of +
+                                                                 (lane * kPer + 2 * e) * cache_bytes(S));
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                if (j + n >= keys) break;
-                float dot = 0.f;
-#pragma unroll
-                for (int e = 0; e < kPer / 2; ++e) {
-                    const float2 f = cache_pair<S>(k[n][e]);
-                    dot += qv[2 * e] * f.x;
-                    dot += qv[2 * e + 1] * f.y;
-                }
-                const float score = warp_sum(dot) * (cache_eight(S) ? cache_scale(ks[n]) : 1.f) * a.scale;
-                const float higher = fmaxf(top, score);
-                const float from = higher == -INFINITY ? 0.f : higher;
-                const float keep = expf(top - from), p = expf(score - from);
-                const float by = cache_eight(S) ? cache_scale(vs[n]) : 1.f;
-                total = total * keep + p;
+            for (int n = 0; n < kAtOnce; ++n) {
+                const float pn = __shfl_sync(0xffffffffu, p, n0 + n), bn = __shfl_sync(0xffffffffu, by, n0 + n);
 #pragma unroll
                 for (int e = 0; e < kPer / 2; ++e) {
                     const float2 f = cache_pair<S>(v[n][e]);
-                    o[2 * e] = o[2 * e] * keep + p * (f.x * by);
-                    o[2 * e + 1] = o[2 * e + 1] * keep + p * (f.y * by);
+                    o[2 * e] += pn * (f.x * bn);
+                    o[2 * e + 1] += pn * (f.y * bn);
                 }
-                top = higher;
             }
         }
-        if (!(total == total)) break;  // and so it stays, and every sum of it
     }
     const float inverse = keys > 0 ? 1.f / total : 0.f;
     unsigned char* op = a.out + row * a.o_row + head * a.o_head + lane * (kPer * 2);
