@@ -239,7 +239,7 @@ def test_value_scales_over_their_whole_range(storage, dtype, width, rows, column
 @pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
 @pytest.mark.parametrize("width", [64, 128])
 @pytest.mark.parametrize("scales,size", [((137, 147), 2.0 ** -16), ((95, 100), 2.0 ** 14), ((90, 150), 2.0 ** -16),
-                                         ((1, 20), 2.0 ** 15)])
+                                         ((90, 150), 2.0 ** -7), ((1, 20), 2.0 ** 15)])
 @pytest.mark.parametrize("rows,columns", SHAPES)
 def test_key_scales_beyond_the_queries_type(storage, dtype, width, scales, size, rows, columns):
     """Keys whose elements are above 65504 or below fp16's smallest step, under

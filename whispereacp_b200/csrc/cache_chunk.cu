@@ -457,23 +457,26 @@ __device__ __forceinline__ float scores_factor(float scale, uint32_t power) {
 // The scale byte of a key relative to its block's power of two, which stands
 // kUp below the block's largest byte: fp16 holds the largest scaled value (448 x
 // 2^7, 128 x 2^8) then, and whole every value of a scale down to kDown below the
-// power.  Keys further down (2^22 or 2^32 below the largest; zeros aside) become
-// NaN, and the rows that see one are computed again alone.  Blocks whose bytes
-// are all 112 to 127, rows whose largest lies between 2^-6 and 2^6 among them,
-// need no power (it is 127, 2^0).
+// power.  Values of keys further down (2^22 or 2^32 below the largest) are off by
+// up to 2^-25, kKeyStep: a row whose queries make more than kScoreStep of a score
+// of that is computed again alone, which takes scores of thousands.  Blocks whose
+// bytes are all 112 to 127, rows whose largest lies between 2^-6 and 2^6 among
+// them, need no power (it is 127, 2^0).
+constexpr float kKeyStep = 0x1p-25f, kScoreStep = 0x1p-20f;
 template <int S> constexpr uint32_t kUp = S == kCacheE4m3 ? 7 : 8;
 template <int S> constexpr uint32_t kDown = S == kCacheE4m3 ? 15 : 24;
 template <int S>
 __device__ __forceinline__ uint32_t shared_scale(uint32_t byte, uint32_t power) {
     if (byte == 255u) return byte;
-    if (byte + kDown<S> < power) return byte <= 8u ? 0u : 255u;
-    return byte + 127u - power;
+    return byte + 126u < power ? 0u : byte + 127u - power;
 }
 
 // The power of a block of `keys` keys, by every warp of the kThreads that widen
-// it: kUp below the largest scale byte that stands for a number (25 at least).
+// it: kUp below the largest scale byte that stands for a number (25 at least),
+// and kFarKeys if a key lies further below than kDown, rows of zeros aside.
 // `four` are the lane's four bytes at `bytes`, in whose place the first warp puts
 // them relative to the power.  Rare, and kept out of the loop's instructions.
+constexpr uint32_t kFarKeys = 256;
 template <int S, int kThreads>
 __device__ __noinline__ uint32_t share_power(uint32_t* bytes, uint32_t four, int keys, int warp, int lane) {
     uint32_t most = 25, relative = 0;
@@ -482,11 +485,28 @@ __device__ __noinline__ uint32_t share_power(uint32_t* bytes, uint32_t four, int
         if (lane * 4 + i < keys && byte != 255u) most = max(most, byte);
     }
     const uint32_t power = __reduce_max_sync(0xffffffffu, most) - kUp<S>;
-    for (int i = 0; i < 4; ++i) relative |= (shared_scale<S>((four >> (8 * i)) & 255u, power) & 255u) << (8 * i);
+    bool far = false;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t byte = (four >> (8 * i)) & 255u;
+        relative |= (shared_scale<S>(byte, power) & 255u) << (8 * i);
+        far |= lane * 4 + i < keys && byte > 8u && byte + kDown<S> < power;
+    }
     asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
     if (warp == 0) bytes[lane] = relative;
     asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
-    return power;
+    return power | (__any_sync(0xffffffffu, far) ? kFarKeys : 0u);
+}
+
+// The sum of the magnitudes of a row's queries as they lie in a tile; rare too.
+template <int kHalves>
+__device__ __noinline__ float queries_sum(const unsigned char* tile, int row) {
+    float sum = 0.f;
+    for (int i = 0; i < kHalves * 64; i += 2) {
+        const float2 q = Half16<__half>::pair_to_float2(
+            *reinterpret_cast<const uint32_t*>(tile + (i / 64) * kHalfBytes + row * 128 + (i % 64) * 2));
+        sum += fabsf(q.x) + fabsf(q.y);
+    }
+    return sum;
 }
 
 // 8-bit caches: the warps bring the blocks in as they are held, four tiles
@@ -581,7 +601,8 @@ __device__ void chunk_widen(const CacheAttendArgs& a, unsigned char* smem, const
                 power = share_power<S, kThreads>(reinterpret_cast<uint32_t*>(held + kPieces * 16), four, keys, warp, lane);
             if (me == 0) {
                 const int at = (n >> 1) % Layout::powers;
-                reinterpret_cast<float*>(smem + Layout::powers_at)[at] = scores_factor(a.scale, power);
+                const float factor = scores_factor(a.scale, power & 255u);
+                reinterpret_cast<float*>(smem + Layout::powers_at)[at] = power & kFarKeys ? -factor : factor;
                 cache_arrive(bar.powers + at);
             }
         }
@@ -778,6 +799,11 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                     const int n = passed + j - p.block, at = n % Layout::powers;
                     cache_wait(bar.powers + at, (uint32_t)(n / Layout::powers) & 1u, abort, a.status, kWaitPower);
                     to_log2 = reinterpret_cast<const volatile float*>(smem + Layout::powers_at)[at];
+                    if (to_log2 < 0.f) {  // there are keys far below the largest
+                        to_log2 = -to_log2;
+                        const float most = queries_sum<Layout::halves>(smem + t * Layout::tile_bytes, row) * kKeyStep;
+                        if (j * kBlockKeys < r.seen && !(most * to_log2 < kScoreStep)) sum = NAN;
+                    }
                 }
                 cache_wait(bar.scores + t, s_parity, abort, a.status, kWaitScores);
                 s_parity ^= 1;
