@@ -188,7 +188,8 @@ class PagedCache:
         tensors of `dtype` (None: the cache's; float32 for 8-bit storage);
         `rows`, then, is how many there are (None: taken from the batch's
         starts as they stand, which waits for the device, and so cannot be
-        captured)."""
+        captured).  Rows of no sequence are left alone: in new tensors they
+        hold anything."""
         if (keys is None) != (values is None):
             raise ValueError("keys and values to fill are given together")
         handle = self._usable(batch)
@@ -221,7 +222,8 @@ class PagedCache:
         None is 1 / sqrt(head_width).  Returns out (new, or the one given), or
         (out, lse) with return_lse or an `lse` to fill: float32 [rows,
         query_heads], the log of the sum of exponentials.  A row without a key
-        gets zeros and -inf.
+        gets zeros and -inf; rows of no sequence are left alone (in a new out
+        they hold anything).
         """
         shape = queries.shape
         if len(shape) != 3:

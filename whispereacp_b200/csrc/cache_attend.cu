@@ -36,11 +36,14 @@
 //
 // Measured (6.54 TB/s is a copy's rate): one token of 12 sequences of up to
 // 32768 bf16 rows, 128 wide, 148 us for 967 MB, 6.5 TB/s; of 64 windows x 20
-// heads over 1500 int8 rows 52 us for 250 MB, 4.8 TB/s, where the widening's
-// instructions fill the issue slots beside the copies (57 % of them, 3 CTAs an
-// SM); of 64 windows over up to 448 bf16 rows 18 us for 66 MB, of which the
-// launch, the search of the list and an item's 2500 cycles are the most; of
-// one window 5.6 us, all latency.
+// heads over 1500 int8 rows 52 us for 250 MB, 4.8 TB/s, where no unit is full
+// (DRAM 61 %, issue slots 58 %) and a warp waits as long for its own last
+// instruction as for the copies; of 64 windows over up to 448 bf16 rows 18 us for
+// 66 MB, of which the launch, the search of the list and an item's 2500 cycles
+// are the most; of one window 5.8 us, all latency.  Rows that are computed again
+// alone take a warp each and cost far more: if every row of 64 tokens x 20 heads
+// over 1500 fp16 rows sees an infinity, 1360 us for 84; one token of 8 heads over
+// 32768 int8 rows 3.8 ms for 15 us.
 #include "cache_join.cuh"
 
 #include <algorithm>
@@ -396,6 +399,9 @@ __device__ __forceinline__ void token_producer(const CacheAttendArgs& a, const C
         }
 }
 
+// With 128 registers a thread for three CTAs an SM, and 168 for two, only tiles of
+// 16 rows spill: 260 bytes a thread at 128 wide over 16 bits, 340 to 450 over 8,
+// 44 to 92 at 64 wide over 8.
 template <typename T, int S, int D, int NT>
 __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     cache_tokens_kernel(const __grid_constant__ CacheAttendArgs a, const __grid_constant__ CacheMaps maps) {
@@ -878,9 +884,9 @@ CutPart launch_tokens(const CacheAttendArgs& a, const CacheMaps& maps, int sms, 
 // 8-bit blocks the widening besides.  16 x 1500 keys x 8 heads, few-row and
 // chunk kernel: 32 fp16 rows 22 and 28 us (64 wide), 39 and 46 (128 wide, where
 // 4 x 8192 keys take 57 and 51, and 4 x 32768 171 and 113); 48 fp16 rows 28.5 and
-// 28.8 (4 x 8192 31.6 and 31.3); 64 int8 rows 34 and 46 (64 x 450 keys 50 and
-// 59); 128 wide 48 int8 rows 46 and 64 (64 x 450 78 and 82), 64 of them 57 and
-// 65 but 94 and 84.
+// 28.8 (4 x 8192 31.6 and 31.3); 64 int8 rows 35 and 48 (64 x 450 keys 51 and
+// 61); 128 wide 48 int8 rows 48 and 66 (64 x 450 82 and 86), 64 of them 61 and
+// 68 but 99 and 87.
 static long long few_rows(const CacheAttendShape& shape) {
     if (cache_eight(shape.storage)) return shape.width == 64 ? 64 : 48;
     return shape.width == 64 ? 32 : 16;
@@ -888,14 +894,17 @@ static long long few_rows(const CacheAttendShape& shape) {
 // And up to which a sequence is the few-row kernel's, in tiles of 8, beside
 // sequences of more.  One of 48 sequences of up to 1200 keys x 8 heads has 200
 // rows, 11 have these, the others one, taken by the few-row and by the chunk
-// kernel: 20 int8 rows 35.0 and 40.3 us (64 wide), 53 and 54.5 (128 wide), 32 of
-// them 42.2 and 40.6, 56 and 55; 20 fp16 rows 34.6 and 31.1, 55 and 51.
+// kernel: 20 int8 rows 35.6 and 41.1 us (64 wide), 55 and 57 (128 wide), 32 of
+// them 42.2 and 41.4, 57 and 57; 20 fp16 rows 34.7 and 31.1, 58 and 53.
 static long long few_rows_beside(const CacheAttendShape& shape) { return cache_eight(shape.storage) ? 24 : 16; }
 // Calls whose units, 16 rows each, come to this many for each of two CTAs an SM
 // at most are the few-row kernel's too, whatever their rows: it starts sooner.
-// One window's 224 rows over 450 keys x 20 heads, few-row and chunk kernel: fp16
-// 11.5 and 17.9 us; with 15 units a CTA 21 and 23 us (64 wide) but 37 and 29
-// (128 wide), with 30 34 and 27.
+// Few-row and chunk kernel by units a CTA, 64 wide: 3.8 (one window's 224 rows
+// over 450 keys x 20 heads) int8 11.7 and 23.3 us, 7.6 fp16 11.4 and 18.1, int8
+// (two windows) 18.2 and 27.0, 15 fp16 21.3 and 22.8 but int8 35.0 and 29.8.
+// 128 wide: 7 (128 rows over 4 x 450 keys x 8 heads) fp16 22.7 and 22.3, int8 22.3
+// and 27.5, 9 (224 rows over 1500 keys x 8 heads) 23.7 and 24.0, 23.1 and 29.5, 12
+// 31.5 and 26.5, 31.2 and 32.4, 15 35.6 and 28.2, 35.0 and 33.9.
 constexpr int kSmallUnits = 10;
 static bool few_alone(const CacheAttendArgs& a, const CacheAttendShape& shape) {
     if ((long long)shape.max_rows * a.group <= few_rows(shape)) return true;

@@ -28,7 +28,9 @@
 //                   its own latency, so their number counts: 8 sequences of
 //                   8192 int8 keys, 128 wide, 256 rows, took 231 us with three
 //                   warps, 198 with four, 151 with seven (at 128 registers a
-//                   thread, where the softmax has no scores on their way).
+//                   thread, of which 64 to 104 bytes spill, where the softmax
+//                   has no scores on their way; 155 under fp16 queries since
+//                   their keys share a power of two).
 //
 // 16-bit 64-wide heads have items of one tile, and an SM two CTAs, which then
 // are the two that take turns: ragged prompts of 32 windows 42 us against 47.
@@ -50,6 +52,10 @@
 // turn do not hide all of that.  Ragged prompts of 32 windows (fp16, 64 wide,
 // 450 keys) 34.6 us, nearly all of it what an item and a launch cost; a mixed
 // batch of 48 sequences over e4m3, the few-row kernel's share behind it, 72 us.
+// Rows that are computed again alone take a warp each: if all of 256 rows x 8
+// heads over 16 x 1500 keys are, 9.9 ms for 48 us (fp16, infinities among the
+// values) or 7.8 ms for 60 (int8 values above 65504 under fp16 queries, which
+// come to fp16 results above or near its largest).
 #include "cache_join.cuh"
 
 #include <algorithm>
