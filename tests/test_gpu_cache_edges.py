@@ -310,6 +310,7 @@ def test_tensors_that_require_gradients_are_refused():
     """The operators have no gradient; results that silently lack one would
     train nothing.  Without grad mode they are taken as they are."""
     import torch
+    from whispereacp_b200 import PagedCache
     cache = make_cache("float16", 8, 2, 16, 64, 591)
     batch, _ = make_batch([20], [2], 16, 8, 592)
     plain = queries(2, 2, 64, "float16", 593)
@@ -320,6 +321,10 @@ def test_tensors_that_require_gradients_are_refused():
                  lambda x: cache.attend(batch, plain, lse=torch.zeros(2, 2, device="cuda", requires_grad=True))):
         with pytest.raises(ValueError, match="gradient"):
             call(leaf)
+    pool = cache.keys.clone().requires_grad_()
+    for pools in ((pool, cache.values), (cache.keys, pool)):
+        with pytest.raises(ValueError, match="gradient"):
+            PagedCache(*pools)
     with torch.no_grad():
         assert torch.equal(cache.attend(batch, leaf), cache.attend(batch, plain))
         cache.append(batch, leaf, leaf)
@@ -353,3 +358,22 @@ def test_caches_of_a_thread_and_stream_share_a_workspace():
         thread.join()
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
+@pytest.mark.parametrize("byte", [10, 20, 40, 80, 180, 230, 245])
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_value_scales_of_any_size(storage, dtype, byte, rows, columns):
+    """All values tiny, or all large, beside a page of zeros as untouched memory
+    holds them (scale byte 0)."""
+    lengths, new = rows
+    pages = pages_of(lengths, 16)
+    cache = make_cache(storage, pages, 2, 16, 64, 621)
+    batch, starts = make_batch(lengths, new, 16, pages, 622, columns=columns)
+    cache.value_scales.fill_(byte)
+    for s, n in enumerate(lengths):
+        if n > 20:
+            cache.value_scales[int(batch.page_table[s, 0])] = 0
+    q = queries(int(starts[-1]), 4, 64, dtype, 623)
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, 0.125)

@@ -114,6 +114,9 @@ class PagedCache:
         if values.shape != keys.shape or values.dtype != keys.dtype or values.device != keys.device or \
                 values.stride() != keys.stride():
             raise ValueError("keys and values must be alike")
+        for name, t in (("keys", keys), ("values", values)):
+            if t.requires_grad:
+                _refuse_gradient(name)
         storage = CACHE_STORAGE.get(_name(keys.dtype))
         if storage is None:
             raise ValueError(f"a cache holds one of {sorted(CACHE_STORAGE)}, not {_name(keys.dtype)}")
