@@ -377,3 +377,25 @@ def test_value_scales_of_any_size(storage, dtype, byte, rows, columns):
     q = queries(int(starts[-1]), 4, 64, dtype, 623)
     out, lse = cache.attend(batch, q, return_lse=True)
     check(cache, batch, starts, q, out, lse, 0.125)
+
+
+@pytest.mark.parametrize("storage", ["int8", "float8_e4m3fn"])
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("most", [100, 200])
+def test_key_scales_of_every_sequence_s_own(storage, width, most):
+    """Items of one tile of rows between items of two, over keys of a scale for
+    each sequence: no tile takes another block's."""
+    import torch
+    new = [most if s % 3 else 300 for s in range(36)]
+    lengths = [n + 97 * (s % 11) for s, n in enumerate(new)]
+    pages = pages_of(lengths, 32)
+    cache = make_cache(storage, pages, 6, 32, width, 631)
+    batch, starts = make_batch(lengths, new, 32, pages, 632)
+    byte = torch.empty(pages, dtype=torch.uint8, device="cuda")
+    for s, n in enumerate(lengths):
+        byte[batch.page_table[s, :-(-n // 32)].long()] = 104 + 5 * s % 23
+    cache.key_scales.copy_(byte[:, None, None].expand_as(cache.key_scales))
+    q = queries(int(starts[-1]), 6, width, "float16", 633)
+    for causal in (True, False):
+        out, lse = cache.attend(batch, q, causal=causal, return_lse=True)
+        check(cache, batch, starts, q, out, lse, width ** -0.5, causal, spread=True)

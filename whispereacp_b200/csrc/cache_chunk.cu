@@ -801,7 +801,13 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
             // Keys below `clear` are seen by every row of the tile.
             const int clear = tile_row(a, p.q, p.head, packed).seen;
             for (int j = p.block; j < blocks; ++j) {
+                cache_wait(bar.scores + t, s_parity, abort, a.status, kWaitScores);
+                s_parity ^= 1;
+                tmem_fence_after();
+                const bool masked = (j + 1) * kBlockKeys > clear;
                 if constexpr (keys_share<T, S>()) {
+                    // Behind the scores' wait: a tile that passes items by would
+                    // take an older phase of the place for its own.
                     const int n = passed + j - p.block, at = n % Layout::powers;
                     cache_wait(bar.powers + at, (uint32_t)(n / Layout::powers) & 1u, abort, a.status, kWaitPower);
                     to_log2 = reinterpret_cast<const volatile float*>(smem + Layout::powers_at)[at];
@@ -811,10 +817,6 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
                         if (j * kBlockKeys < r.seen && !(most * to_log2 < kScoreStep)) sum = NAN;
                     }
                 }
-                cache_wait(bar.scores + t, s_parity, abort, a.status, kWaitScores);
-                s_parity ^= 1;
-                tmem_fence_after();
-                const bool masked = (j + 1) * kBlockKeys > clear;
                 // 32 scores at a time, the next 32 on their way.  Half a block's
                 // P goes out at a time, so that the products of the first 64
                 // keys' run while the second 64 are computed; its check, its
