@@ -361,7 +361,7 @@ def test_caches_of_a_thread_and_stream_share_a_workspace():
 
 
 @pytest.mark.parametrize("storage,dtype", EIGHT_PAIRS)
-@pytest.mark.parametrize("byte", [10, 20, 40, 80, 180, 230, 245])
+@pytest.mark.parametrize("byte", [2, 6, 20, 40, 80, 180, 230, 245])
 @pytest.mark.parametrize("rows,columns", SHAPES)
 def test_value_scales_of_any_size(storage, dtype, byte, rows, columns):
     """All values tiny, or all large, beside a page of zeros as untouched memory

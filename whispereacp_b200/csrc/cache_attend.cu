@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                 for (int e = 0; e < 4; ++e) o[k][j][e] = 0.f;
         // The reference of the exponentials (0 until a key is seen), how far
         // above it a score may be, and the sum of this lane's keys.  Over 8
-        // bits, the least byte above 8, less 9, that a row of the tile met.
+        // bits, the least byte above 1 (rows of zeros), less 2, that a row of the tile met.
         float from[NT][2], limit[NT][2], sum[NT][2];
         uint32_t least = 0xffffffffu;
 #pragma unroll
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                             const uint32_t byte = scales[Layout::keys + warp * kWarpKeys + i * 16 + g + 8 * h];
                             factor[i][h] = __uint_as_float(byte << 23);  // infinity for 255
                             beside[i][h] = fmaxf(log2_fast(factor[i][h]) - 7.f, -kFar);
-                            if (!masked || key0 + i * 16 + g + 8 * h < reach) least = min(least, byte - 9u);
+                            if (!masked || key0 + i * 16 + g + 8 * h < reach) least = min(least, byte - 2u);
                         }
                 const auto counted = [&](float v, int i, int h) {
                     if constexpr (kEight) return v + beside[i][h];
@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
                     // References carry scales: a power of two a row brings the
                     // sum to 1, so that those of the warps can meet.
                     const int power = min(max((int)(__float_as_uint(all) >> 23), 1), 253);
-                    bool far = least < 246u && all * __uint_as_float((least + 9u) << 23) < kLeastScaled;
+                    bool far = least < 253u && all * __uint_as_float((least + 2u) << 23) < kLeastScaled;
                     if (__any_sync(0xffffffffu, far)) {
                         float low = INFINITY;
 #pragma unroll

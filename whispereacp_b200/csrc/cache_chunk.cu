@@ -495,7 +495,7 @@ __device__ __noinline__ uint32_t share_power(uint32_t* bytes, uint32_t four, int
     for (int i = 0; i < 4; ++i) {
         const uint32_t byte = (four >> (8 * i)) & 255u;
         relative |= (shared_scale<S>(byte, power) & 255u) << (8 * i);
-        far |= lane * 4 + i < keys && byte > 8u && byte + kDown<S> < power;
+        far |= lane * 4 + i < keys && byte > 1u && byte + kDown<S> < power;
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
     if (warp == 0) bytes[lane] = relative;
