@@ -145,7 +145,7 @@ int wsp_cache_read(wsp_cache* cache, const wsp_cache_batch* batch, int rows, con
  * values a row does not see cannot change its result, whatever they hold.
  * Scores, softmax and sums are kept in fp32.  A probability (over 8 bits, times
  * its value's scale) meets its value rounded to 16 bits or to two of them: by
- * 2^-8 (bf16) or 2^-11 (fp16, and over 8 bits) of itself at most, fp16 by 2^-25
+ * 2^-8 (bf16) or 2^-11 (fp16, and over 8 bits) of itself at most, fp16 by 2^-32
  * of the row's largest where that is more.  A row whose result is not finite, or
  * whose numbers the 16 bits do not reach, is computed again alone in fp32, at
  * up to some hundred times the cost.

@@ -399,3 +399,23 @@ def test_key_scales_of_every_sequence_s_own(storage, width, most):
     for causal in (True, False):
         out, lse = cache.attend(batch, q, causal=causal, return_lse=True)
         check(cache, batch, starts, q, out, lse, width ** -0.5, causal, spread=True)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("gap", [10.5, 16.47, 20.47])
+@pytest.mark.parametrize("rows,columns", [(1, None), (5, None), (5, 600), (130, None), (130, 9600)])
+def test_large_values_of_small_probabilities(dtype, gap, rows, columns):
+    """One key of nearly all the probability and small values before 400 keys of
+    2^-gap each and values of ten thousands, which are the result."""
+    import torch
+    width = 64
+    cache = make_cache(dtype, 40, 2, 16, width, 641)
+    batch, starts = make_batch([400 + rows], [rows], 16, 40, 642, columns=columns)
+    cache.keys.zero_()
+    cache.values.abs_().mul_(1e4)
+    page, row = place(cache, batch, 0, 0)
+    cache.keys[page, :, row] = gap * math.log(2) / (width * 0.125)
+    cache.values[page, :, row] = 1e-3
+    q = torch.ones(rows, 2, width, dtype=dt(dtype), device="cuda")
+    out, lse = cache.attend(batch, q, return_lse=True)
+    check(cache, batch, starts, q, out, lse, 0.125)

@@ -21,7 +21,8 @@
 // rows as B, so a single token costs an eighth of the products, not a
 // sixteenth, and 16 scores of a lane's two rows are its whole softmax; then o^T
 // by 16 value columns as A and P as B, P as two 16-bit halves, hi + lo: no
-// rounding that shows.  The running maximum moves only when a score is more
+// rounding that shows down to 2^-32 of the largest (fp16 starts at 2^7 for that).
+// The running maximum moves only when a score is more
 // than 2^8 above it, which a vote finds: P may reach 2^8, and the shuffles and
 // the rescaling of o are rare.  The warps' results meet once per item.
 //
@@ -409,6 +410,9 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
     using MT = typename std::conditional<cache_eight(S), __half, T>::type;  // the products' type
     constexpr bool kEight = cache_eight(S);
     constexpr bool kNarrow = kEight && std::is_same<T, __nv_bfloat16>::value;
+    // fp16 P start at 2^7, so that the small ones keep their bits; over 8 bits the
+    // values' scales are counted with it.
+    constexpr float kRaise = !kEight && std::is_same<T, __half>::value ? 7.f : 0.f;
     constexpr int kSteps = D / 16;                       // k16 steps of a score, 16-wide groups of values
     constexpr int kWarpKeys = Layout::keys / kWorkers;   // of a unit
     constexpr int MK = kWarpKeys / 16;
@@ -645,11 +649,12 @@ __global__ void __launch_bounds__(kTokenThreads, TokenLayout<S, D, NT>::ctas)
 #pragma unroll
                             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                             float keep = 1.f;
+                            top -= kRaise;
                             if (top > (limit[j][e] == -INFINITY ? -INFINITY : 0.f)) {
                                 const float higher = from[j][e] + top;
                                 keep = limit[j][e] == -INFINITY ? 0.f : exp2_fast(-top);
                                 from[j][e] = higher;
-                                limit[j][e] = kLazy;
+                                limit[j][e] = kLazy + kRaise;
                             }
                             sum[j][e] *= keep;
 #pragma unroll

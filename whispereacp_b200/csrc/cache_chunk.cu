@@ -749,9 +749,9 @@ __device__ void chunk_softmax(const CacheAttendArgs& a, unsigned char* smem, con
     // The reference of a row's exponentials comes from the maximum of the first
     // block it sees and stays as long as a block's sum of P says that no P left
     // the 16-bit type's range: fp16 keeps 2^-14 .. 2^15 whole, so P starts at
-    // 2^4 at most; bf16 has fp32's range.
+    // 2^8 at most, and 64 of them sum up to 2^14; bf16 has fp32's range.
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    constexpr float kShift = kHalf ? 4.f : 0.f;
+    constexpr float kShift = kHalf ? 8.f : 0.f;
     constexpr float kMost = kHalf ? 32768.f : 0x1p60f;
     // The next 32 scores on their way while 32 are worked on, where the
     // registers reach for it; 8-bit caches' 512 threads have 128 each.
